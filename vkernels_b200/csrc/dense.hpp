@@ -1,0 +1,99 @@
+// dense.hpp - dense feed-forward operators in 16 bits: the gated projection and the linear projection with bias, activation
+// and residual in its epilogue, each with its backward pass. Host-side types and launchers.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace vkernels::kernels::cuda {
+
+enum DenseType { kDenseBf16 = 0, kDenseFp16 = 1 };
+// activation of the linear projection
+enum DenseAct { kActNone = 0, kActSilu = 1, kActGelu = 2, kActGeluTanh = 3 };
+
+// One 16-bit operand of a product: element (i, k) is p[i * ld + k], or p[k * ld + i] if mn_major (the index that is NOT
+// reduced over is the contiguous one).
+struct DenseOperand {
+  const uint16_t* p;
+  int64_t ld;
+  bool mn_major;
+};
+
+// out[m, n] = act(sum_k A[m, k] B[n, k] + bias[n]) + residual[m, n], or the gated form: B has 2 N rows (gate rows, then up
+// rows), bias 2 N entries, out[m, n] = gate(z[m, n]) * up(z[m, N + n]). preact (optional) receives z, [M, N] or [M, 2 N],
+// rounded to the type without changing side of the clamp's limit.
+struct DenseGemm {
+  DenseType type;
+  DenseOperand a, b;
+  int M, N, K;
+  bool gated;
+  int act;                    // linear: DenseAct; gated: 0 SwiGLU, 1 SiTU
+  float limit, beta, linear_beta;
+  const uint16_t* bias;       // or null
+  const uint16_t* residual;   // or null
+  int64_t ldr;
+  uint16_t* out;
+  int64_t ldo;
+  uint16_t* preact;           // or null
+  int64_t ldp;
+};
+
+// Gradient of the pre-activations: dz = dy * act'(z), [T, rows] (linear) or [T, 2 ispp] (gated) at pitch ldz; with no
+// activation a copy of dy. dz may be null (only the column sums are wanted). partial (optional) receives the column sums of
+// each chunk of rows in fp32, [dense_sum_chunks(T), rows].
+struct DenseGrad {
+  DenseType type;
+  const uint16_t* dy;
+  int64_t lddy;
+  const uint16_t* preact;     // null: no activation
+  int64_t ldp;
+  uint16_t* dz;
+  int64_t ldz;
+  float* partial;
+  int T, N;                   // N: columns of dy; the gated form has 2 N columns of dz
+  bool gated;
+  int act;
+  float limit, beta, linear_beta;
+};
+
+int dense_sum_chunks(int T);
+void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream);
+void launch_dense_simt(const DenseGemm& g, cudaStream_t stream);
+void launch_dense_grad(const DenseGrad& g, cudaStream_t stream);
+// db[n] = sum over the chunks of partial[chunk, n], in order.
+void launch_dense_sum(DenseType type, const float* partial, int chunks, int cols, uint16_t* db, cudaStream_t stream);
+// dst[r, c] = src[r, c] at another pitch.
+void launch_dense_copy_rows(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t ldd, int rows, int cols, cudaStream_t stream);
+
+// ---- the operators ----
+struct DenseForward {
+  DenseType type;
+  const uint16_t *x, *w, *bias, *residual;
+  int64_t ldx, ldw, ldr;
+  uint16_t *y, *preact;
+  int64_t ldy, ldp;
+  int T, n_in, n_out;
+  bool gated;
+  int act;
+  float limit, beta, linear_beta;
+};
+struct DenseBackward {
+  DenseType type;
+  const uint16_t *dy, *x, *w, *preact;
+  int64_t lddy, ldx, ldw, ldp;
+  uint16_t *dx, *dw, *db;     // each may be null
+  int64_t lddx, lddw;
+  int T, n_in, n_out;
+  bool gated;
+  int act;
+  float limit, beta, linear_beta;
+  void* workspace;
+  size_t workspace_bytes;
+};
+void dense_forward(const DenseForward& f, cudaStream_t stream);
+void dense_backward(const DenseBackward& f, cudaStream_t stream);
+size_t dense_backward_workspace_bytes(int T, int n_out, bool gated);
+
+}  // namespace vkernels::kernels::cuda

@@ -1,0 +1,123 @@
+// dense_math.cuh - element arithmetic of the dense feed-forward operators: 16-bit conversions, activations and their slopes.
+#pragma once
+
+#include "common.cuh"
+#include "dense.hpp"
+
+namespace vkernels::kernels::cuda {
+
+namespace {
+
+template <int TYPE>
+__device__ __forceinline__ float dense_to_f32(uint16_t v) {
+  if constexpr (TYPE == kDenseBf16) return __uint_as_float((uint32_t)v << 16);
+  return __half2float(__ushort_as_half(v));
+}
+template <int TYPE>
+__device__ __forceinline__ uint16_t dense_from_f32(float v) {
+  if constexpr (TYPE == kDenseBf16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  return __half_as_ushort(__float2half_rn(v));
+}
+template <int TYPE>
+__device__ __forceinline__ uint32_t dense_pack(float lo, float hi) {
+  if constexpr (TYPE == kDenseBf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <int TYPE>
+__device__ __forceinline__ float2 dense_unpack(uint32_t v) {
+  return make_float2(dense_to_f32<TYPE>((uint16_t)(v & 0xFFFFu)), dense_to_f32<TYPE>((uint16_t)(v >> 16)));
+}
+
+// A pre-activation kept for the backward pass: the nearest 16-bit value on the same side of the clamp's limit, so that the
+// slope of a clamped input is 0 exactly where the forward pass clamped it (limit = inf: no clamp). A finite value beyond
+// fp16's range becomes the largest finite one: the slopes there are those of the limit, where inf would give inf - inf.
+template <int TYPE>
+__device__ __forceinline__ uint16_t dense_round_preact(float v, float limit) {
+  uint16_t r = dense_from_f32<TYPE>(v);
+  if (TYPE == kDenseFp16 && (r & 0x7FFFu) == 0x7C00u && fabsf(v) <= 3.402823466e38f) r -= 1;
+  const float m = fabsf(dense_to_f32<TYPE>(r));
+  if (fabsf(v) > limit) {
+    if (!(m > limit)) r += 1;
+  } else if (m > limit) {
+    r -= 1;
+  }
+  return r;
+}
+
+// 1 / (1 + exp(-v)) by the hardware's exp2 and reciprocal (relative error about 1e-6, a bf16 half step is 4e-3, an fp16 one
+// 5e-4); 1 at +inf, 0 at -inf, NaN stays.
+__device__ __forceinline__ float dense_sigmoid(float v) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
+
+constexpr float kSqrtHalf = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f;
+// 0.5 (1 + tanh(y)) = sigmoid(2 y), y = sqrt(2 / pi) (z + 0.044715 z^3)
+constexpr float kGeluC = 1.5957691216057308f, kGeluA = 0.044715f;
+
+// Activation of the linear projection.
+__device__ __forceinline__ float dense_act(int act, float z) {
+  switch (act) {
+    case kActSilu: return z * dense_sigmoid(z);
+    case kActGelu: return 0.5f * z * (1.0f + erff(z * kSqrtHalf));
+    case kActGeluTanh: return z * dense_sigmoid(kGeluC * (z + kGeluA * z * z * z));
+    default: return z;
+  }
+}
+// Its slope, finite for every finite z: z z is kept below 1e8 where it stands beside 1 - p, which is 0 long before.
+__device__ __forceinline__ float dense_act_slope(int act, float z) {
+  switch (act) {
+    case kActSilu: {
+      const float p = dense_sigmoid(z);
+      return p + z * p * (1.0f - p);
+    }
+    case kActGelu: return 0.5f * (1.0f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * __expf(-0.5f * z * z);
+    case kActGeluTanh: {
+      const float p = dense_sigmoid(kGeluC * (z + kGeluA * z * z * z));
+      return p + z * p * (1.0f - p) * kGeluC * (1.0f + 3.0f * kGeluA * fminf(z * z, 1e8f));
+    }
+    default: return 1.0f;
+  }
+}
+
+// The gated product of one feature; `limit` = inf for no clamp. min.NaN / max.NaN: a NaN stays NaN.
+__device__ __forceinline__ float dense_gated(int act, float g, float u, float limit, float beta, float linear_beta) {
+  if (act == 1) {
+    const float up = linear_beta > 0.0f ? linear_beta * tanhf(u / linear_beta) : u;
+    return beta * tanhf(g / beta) * dense_sigmoid(g) * up;
+  }
+  float lo = -limit;
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(g) : "f"(limit));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(u) : "f"(limit));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(u) : "f"(lo));
+  return g * dense_sigmoid(g) * u;
+}
+// Its gradient with respect to both pre-activations, for the gradient dh of the product.
+__device__ __forceinline__ void dense_gated_grad(int act, float dh, float g, float u, float limit, float beta, float linear_beta,
+                                                 float& dg, float& du) {
+  if (act == 1) {
+    const float p = dense_sigmoid(g), a = tanhf(g / beta);
+    const float b = linear_beta > 0.0f ? tanhf(u / linear_beta) : 0.0f;
+    const float up = linear_beta > 0.0f ? linear_beta * b : u;
+    dg = dh * up * ((1.0f - a * a) * p + beta * a * p * (1.0f - p));
+    du = dh * (beta * a * p) * (1.0f - b * b);
+    return;
+  }
+  float gc = g, uc = u, lo = -limit;
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(gc) : "f"(limit));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(uc) : "f"(limit));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(uc) : "f"(lo));
+  const float p = dense_sigmoid(gc), gate = gc * p;
+  dg = g > limit ? 0.0f : dh * uc * (p + gate * (1.0f - p));
+  du = fabsf(u) > limit ? 0.0f : dh * gate;
+}
+
+}  // namespace
+
+}  // namespace vkernels::kernels::cuda

@@ -1,0 +1,246 @@
+// dense_simple.cu - dense feed-forward operators: the cross-check product on CUDA cores and the element-wise kernels of the
+// backward pass.
+#include "dense.hpp"
+#include "dense_math.cuh"
+
+namespace vkernels::kernels::cuda {
+
+namespace {
+
+__device__ __forceinline__ uint16_t operand_at(const DenseOperand& o, int i, int k) {
+  return o.mn_major ? o.p[(int64_t)k * o.ld + i] : o.p[(int64_t)i * o.ld + k];
+}
+
+constexpr int kTile = 64, kStep = 16;
+
+// One CTA per 64 x 64 tile of the result (64 x 32 gated: 32 gate rows and their 32 up rows), 16 x 16 threads with 4 x 4 sums
+// each, products added in ascending k in fp32 (fused multiply-add). The cross-check of the tensor-core kernels, selected only
+// explicitly: any pitch, order and alignment, about 20 TFLOP/s.
+template <int TYPE, bool GATED>
+__global__ void __launch_bounds__(256) dense_simt_kernel(DenseGemm g) {
+  __shared__ float sa[kStep][kTile + 4], sb[kStep][kTile + 4];
+  constexpr int kCols = GATED ? kTile / 2 : kTile;
+  const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kCols;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float acc[4][4] = {};
+  for (int k0 = 0; k0 < g.K; k0 += kStep) {
+#pragma unroll
+    for (int i = 0; i < kTile * kStep / 256; ++i) {
+      const int e = threadIdx.x + i * 256;
+      const int k = e % kStep, r = e / kStep;
+      const int m = m0 + r;
+      // gated: rows 0..31 of the tile are gate rows, 32..63 the up rows of the same features
+      const int f = n0 + (GATED ? r % kCols : r);
+      const int brow = GATED && r >= kCols ? g.N + f : f;
+      sa[k][r] = m < g.M && k0 + k < g.K ? dense_to_f32<TYPE>(operand_at(g.a, m, k0 + k)) : 0.0f;
+      sb[k][r] = f < g.N && k0 + k < g.K ? dense_to_f32<TYPE>(operand_at(g.b, brow, k0 + k)) : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kStep; ++k) {
+      float av[4], bv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) av[i] = sa[k][ty * 4 + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bv[j] = sb[k][GATED ? tx * 2 + (j & 1) + (j >> 1) * kCols : tx * 4 + j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = m0 + ty * 4 + i;
+    if (m >= g.M) continue;
+    if constexpr (GATED) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int n = n0 + tx * 2 + j;
+        if (n >= g.N) continue;
+        float zg = acc[i][j], zu = acc[i][j + 2];
+        if (g.bias) {
+          zg += dense_to_f32<TYPE>(g.bias[n]);
+          zu += dense_to_f32<TYPE>(g.bias[g.N + n]);
+        }
+        if (g.preact) {
+          g.preact[(int64_t)m * g.ldp + n] = dense_round_preact<TYPE>(zg, g.limit);
+          g.preact[(int64_t)m * g.ldp + g.N + n] = dense_round_preact<TYPE>(zu, g.limit);
+        }
+        g.out[(int64_t)m * g.ldo + n] = dense_from_f32<TYPE>(dense_gated(g.act, zg, zu, g.limit, g.beta, g.linear_beta));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = n0 + tx * 4 + j;
+        if (n >= g.N) continue;
+        float z = acc[i][j] + (g.bias ? dense_to_f32<TYPE>(g.bias[n]) : 0.0f);
+        if (g.preact) g.preact[(int64_t)m * g.ldp + n] = dense_round_preact<TYPE>(z, g.limit);
+        z = dense_act(g.act, z);
+        if (g.residual) z += dense_to_f32<TYPE>(g.residual[(int64_t)m * g.ldr + n]);
+        g.out[(int64_t)m * g.ldo + n] = dense_from_f32<TYPE>(z);
+      }
+    }
+  }
+}
+
+// Eight neighbouring values of a row, as one 16-byte access where the row allows it.
+struct Eight {
+  uint16_t v[8];
+};
+__device__ __forceinline__ Eight load_eight(const uint16_t* p, int n, bool vec) {
+  Eight e;
+  if (vec && n >= 8) {
+    *reinterpret_cast<uint4*>(e.v) = *reinterpret_cast<const uint4*>(p);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e.v[j] = j < n ? p[j] : (uint16_t)0;
+  }
+  return e;
+}
+__device__ __forceinline__ void store_eight(uint16_t* p, const Eight& e, int n, bool vec) {
+  if (vec && n >= 8) {
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e.v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = e.v[j];
+  }
+}
+
+constexpr int kGradCols = 256, kGradThreads = 256;   // 32 threads across the columns, eight each; 8 rows at a time
+
+// dz = dy * act'(z) and the column sums of a chunk of rows, in one pass: one CTA per 256 columns of dy and chunk. A column's
+// sum is added by one thread per eighth row in fp32, the eighths in order, the chunks by dense_sum_kernel: no atomics, the
+// same result every time. The sums are of the unrounded gradients. Bound by memory: dy and z in, dz out.
+template <int TYPE, bool GATED>
+__global__ void __launch_bounds__(kGradThreads) dense_grad_kernel(DenseGrad g, int rows_per_chunk, bool vec) {
+  __shared__ float sums[GATED ? 2 : 1][8][kGradCols];
+  const int c0 = blockIdx.x * kGradCols + (threadIdx.x & 31) * 8, sub = threadIdx.x >> 5;
+  const int left = g.N - c0;
+  const int r_end = min(g.T, (int)(blockIdx.y + 1) * rows_per_chunk);
+  float sg[8] = {}, su[8] = {};
+  if (left > 0) {
+    for (int r = blockIdx.y * rows_per_chunk + sub; r < r_end; r += 8) {
+      const Eight dy = load_eight(g.dy + (int64_t)r * g.lddy + c0, left, vec);
+      if constexpr (GATED) {
+        const Eight zg = load_eight(g.preact + (int64_t)r * g.ldp + c0, left, vec);
+        const Eight zu = load_eight(g.preact + (int64_t)r * g.ldp + g.N + c0, left, vec);
+        Eight og, ou;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float dg, du;
+          dense_gated_grad(g.act, dense_to_f32<TYPE>(dy.v[j]), dense_to_f32<TYPE>(zg.v[j]), dense_to_f32<TYPE>(zu.v[j]), g.limit,
+                           g.beta, g.linear_beta, dg, du);
+          sg[j] += dg;
+          su[j] += du;
+          og.v[j] = dense_from_f32<TYPE>(dg);
+          ou.v[j] = dense_from_f32<TYPE>(du);
+        }
+        if (g.dz) {
+          store_eight(g.dz + (int64_t)r * g.ldz + c0, og, left, vec);
+          store_eight(g.dz + (int64_t)r * g.ldz + g.N + c0, ou, left, vec);
+        }
+      } else {
+        Eight z = dy, o;
+        if (g.preact) z = load_eight(g.preact + (int64_t)r * g.ldp + c0, left, vec);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float d = dense_to_f32<TYPE>(dy.v[j]);
+          if (g.preact) d *= dense_act_slope(g.act, dense_to_f32<TYPE>(z.v[j]));
+          sg[j] += d;
+          o.v[j] = dense_from_f32<TYPE>(d);
+        }
+        if (g.dz) store_eight(g.dz + (int64_t)r * g.ldz + c0, o, left, vec);
+      }
+    }
+  }
+  if (g.partial == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    sums[0][sub][(threadIdx.x & 31) * 8 + j] = sg[j];
+    if constexpr (GATED) sums[GATED ? 1 : 0][sub][(threadIdx.x & 31) * 8 + j] = su[j];
+  }
+  __syncthreads();
+  const int col = blockIdx.x * kGradCols + threadIdx.x;
+  if (col >= g.N) return;
+  const int rows = GATED ? 2 * g.N : g.N;
+#pragma unroll
+  for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += sums[h][i][threadIdx.x];
+    g.partial[(int64_t)blockIdx.y * rows + h * g.N + col] = s;
+  }
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(128) dense_sum_kernel(const float* __restrict__ partial, int chunks, int cols, uint16_t* __restrict__ db) {
+  const int c = blockIdx.x * 128 + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.0f;
+  for (int i = 0; i < chunks; ++i) s += partial[(int64_t)i * cols + c];
+  db[c] = dense_from_f32<TYPE>(s);
+}
+
+__global__ void __launch_bounds__(256) dense_copy_rows_kernel(const uint16_t* __restrict__ src, int64_t lds, uint16_t* __restrict__ dst,
+                                                              int64_t ldd, int rows, int cols) {
+  for (int r = blockIdx.y; r < rows; r += gridDim.y)
+    for (int c = blockIdx.x * 256 + threadIdx.x; c < cols; c += gridDim.x * 256) dst[(int64_t)r * ldd + c] = src[(int64_t)r * lds + c];
+}
+
+bool aligned16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
+
+template <int TYPE>
+void grad_of_type(const DenseGrad& g, int chunks, cudaStream_t stream) {
+  bool vec = aligned16(g.dy, g.lddy) && (g.preact == nullptr || aligned16(g.preact, g.ldp)) && (g.dz == nullptr || aligned16(g.dz, g.ldz));
+  if (g.gated) vec = vec && g.N % 8 == 0;
+  const dim3 grid((g.N + kGradCols - 1) / kGradCols, chunks);
+  const int rows = (g.T + chunks - 1) / chunks;
+  if (g.gated)
+    dense_grad_kernel<TYPE, true><<<grid, kGradThreads, 0, stream>>>(g, rows, vec);
+  else
+    dense_grad_kernel<TYPE, false><<<grid, kGradThreads, 0, stream>>>(g, rows, vec);
+  VK_CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace
+
+// Chunks of at least 32 rows and at most 128 of them: with 256 columns a CTA, 2880 columns of 4096 rows give 12 x 128 CTAs.
+int dense_sum_chunks(int T) { return T <= 32 ? 1 : T >= 4096 ? 128 : (T + 31) / 32; }
+
+void launch_dense_simt(const DenseGemm& g, cudaStream_t stream) {
+  const dim3 grid((g.N + (g.gated ? kTile / 2 : kTile) - 1) / (g.gated ? kTile / 2 : kTile), (g.M + kTile - 1) / kTile);
+  expects(grid.y <= 65535u, "dense product: at most 4194240 rows on the cross-check kernels");
+  if (g.type == kDenseBf16) {
+    if (g.gated) dense_simt_kernel<kDenseBf16, true><<<grid, 256, 0, stream>>>(g);
+    else dense_simt_kernel<kDenseBf16, false><<<grid, 256, 0, stream>>>(g);
+  } else {
+    if (g.gated) dense_simt_kernel<kDenseFp16, true><<<grid, 256, 0, stream>>>(g);
+    else dense_simt_kernel<kDenseFp16, false><<<grid, 256, 0, stream>>>(g);
+  }
+  VK_CUDA_CHECK(cudaGetLastError());
+}
+
+void launch_dense_grad(const DenseGrad& g, cudaStream_t stream) {
+  const int chunks = dense_sum_chunks(g.T);
+  if (g.type == kDenseBf16) grad_of_type<kDenseBf16>(g, chunks, stream);
+  else grad_of_type<kDenseFp16>(g, chunks, stream);
+}
+
+void launch_dense_sum(DenseType type, const float* partial, int chunks, int cols, uint16_t* db, cudaStream_t stream) {
+  const int grid = (cols + 127) / 128;
+  if (type == kDenseBf16) dense_sum_kernel<kDenseBf16><<<grid, 128, 0, stream>>>(partial, chunks, cols, db);
+  else dense_sum_kernel<kDenseFp16><<<grid, 128, 0, stream>>>(partial, chunks, cols, db);
+  VK_CUDA_CHECK(cudaGetLastError());
+}
+
+void launch_dense_copy_rows(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t ldd, int rows, int cols, cudaStream_t stream) {
+  if (rows <= 0 || cols <= 0) return;
+  const dim3 grid((cols + 255) / 256 < 16 ? (cols + 255) / 256 : 16, rows < 16384 ? rows : 16384);
+  dense_copy_rows_kernel<<<grid, 256, 0, stream>>>(src, lds, dst, ldd, rows, cols);
+  VK_CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace vkernels::kernels::cuda

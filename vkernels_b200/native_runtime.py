@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_int32, c_size_t, c_void_p
+from ctypes import c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 IN_TREE = os.path.join(_HERE, "lib", "libvkernels_b200.so")
@@ -89,6 +89,15 @@ _SIGNATURES = {
     "vk_cuda_fused_moe_mxfp4_rows": (c_int, [c_void_p] * 8 + [c_int] * 4 + [c_void_p] * 2 +
                                      [c_int, c_float, c_int, c_float, c_float, c_void_p, c_void_p,
                                       c_int, c_void_p]),
+    "vk_cuda_gated_linear": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64] +
+                             [c_int] * 5 + [c_float] * 3 + [c_void_p]),
+    "vk_cuda_fused_linear": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p] + [c_void_p, c_int64] * 3 + [c_int] * 5 +
+                             [c_void_p]),
+    "vk_cuda_dense_backward_workspace_bytes": (c_size_t, [c_int] * 3),
+    "vk_cuda_gated_linear_backward": (c_int, [c_void_p, c_int64] * 6 + [c_void_p] + [c_int] * 5 + [c_float] * 3 +
+                                      [c_void_p, c_size_t, c_void_p]),
+    "vk_cuda_fused_linear_backward": (c_int, [c_void_p, c_int64] * 6 + [c_void_p] + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
+    "vk_cuda_dense_copy_rows": (c_int, [c_void_p, c_int64] * 2 + [c_int] * 2 + [c_void_p]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -1,0 +1,334 @@
+"""Dense feed-forward operators in 16 bits: what a mixture-of-experts model computes beside its routed experts (dense layers, an
+always-on expert that the checkpoint keeps in bf16 or fp16), forward and backward.
+
+``gated_linear``  both projections, the activation and the product in one kernel; weight order and activations are the routed
+                  layer's (``w13``: gate rows, then up rows; SwiGLU with its limit, or SiTU)
+``fused_linear``  a projection with bias, activation and residual in its epilogue
+
+Tensors are bf16 or fp16, one type per call, on one GPU; sums are fp32 and rounded once. Rows may have any pitch, the values of a
+row must be neighbours. An operand whose rows do not start on 16 bytes is first copied to rows that do. Calls run on the current
+stream, allocate through torch only, and may be captured.
+
+Called with gradients enabled and an input that requires one, the two operators record themselves for ``backward()``; that
+form cannot be captured into a CUDA graph (capture ``*_backward`` instead, which record nothing).
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
+
+from .. import native_runtime as nr
+from ._dispatch import require
+from .moe_fused_mxfp4 import SITU, SWIGLU
+
+_DTYPE = {torch.bfloat16: 0, torch.float16: 1}
+_LINEAR_ACT = {None: 0, "none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
+
+
+def _call(name, device, *args):
+    """The C entry on the current stream of `device`, which becomes the current device for the call."""
+    fn = getattr(nr.load_library(), name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if rc:
+        nr.check(rc, name)
+
+
+def _check(name, t, dtype, device):
+    require(t.dtype == dtype, f"{name} must be {dtype}, like the other tensors of the call, got {t.dtype}")
+    require(t.device == device, f"{name} must be on {device}, got {t.device}")
+
+
+def _pitch(name, t):
+    """Elements from one row of a 2-D tensor to the next."""
+    T, n = t.shape
+    require(n <= 1 or t.stride(1) == 1, f"the values of a row of {name} must be neighbours in memory")
+    if T <= 1:
+        return (n + 7) // 8 * 8
+    require(t.stride(0) >= n, f"the rows of {name} must not overlap")
+    return t.stride(0)
+
+
+def _operand(name, t):
+    """(tensor to keep, pointer, pitch) of a matrix that the products read: rows on 16 bytes, copied there if they are not."""
+    ld = _pitch(name, t)
+    p = t.data_ptr()
+    if (p & 15) == 0 and (ld & 7) == 0:
+        return t, p, ld
+    T, n = t.shape
+    wide = torch.empty((T, (n + 7) // 8 * 8), dtype=t.dtype, device=t.device)
+    _call("vk_cuda_dense_copy_rows", t.device, p, ld, wide.data_ptr(), wide.shape[1], T, n)
+    return wide, wide.data_ptr(), wide.shape[1]
+
+
+def _span(t):
+    """First byte and the one behind the last of a tensor's memory."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _apart(name, out, others):
+    a, b = _span(out)
+    for other_name, t in others:
+        if t is not None:
+            c, d = _span(t)
+            require(b <= c or d <= a, f"{name} must not overlap {other_name}")
+
+
+def _rows2d(name, t, cols):
+    """A result tensor of the caller, or a tensor that goes with the result, as [T, cols] without a copy."""
+    require(t.dim() >= 1 and t.shape[-1] == cols, f"{name} must have {cols} columns")
+    if t.dim() == 2:
+        return t
+    try:
+        return t.view(-1, cols)
+    except RuntimeError:
+        require(False, f"{name} must be viewable as rows of {cols}")
+
+
+def _inputs(x, w, rows, what):
+    require(isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor), f"{what}: tensors expected")
+    require(x.dtype in _DTYPE, f"x must be bfloat16 or float16, got {x.dtype}")
+    _check("the weight", w, x.dtype, x.device)
+    require(x.dim() >= 1 and w.dim() == 2 and w.shape[1] == x.shape[-1], f"{what}: x [..., n_in] and a weight [rows, n_in] expected")
+    require(w.shape[1] > 0 and w.shape[0] > 0, f"{what}: feature counts must be positive")
+    require(rows != 2 or w.shape[0] % 2 == 0, "w13 must hold gate rows followed by up rows: an even row count")
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    require(x2.shape[0] < 2 ** 30 and w.shape[0] < 2 ** 30 and w.shape[1] <= 2 ** 30, f"{what}: more rows or features than the kernels index")
+    return x2
+
+
+def _bias(bias, rows, x):
+    if bias is None:
+        return None
+    _check("the bias", bias, x.dtype, x.device)
+    require(bias.shape == (rows,) and (rows == 1 or bias.stride(0) == 1), f"the bias must be contiguous [{rows}]")
+    return bias.data_ptr()
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _no_capture():
+    require(not torch.cuda.is_current_stream_capturing(),
+            "recording for backward() cannot be captured into a CUDA graph: capture the forward call with return_preact=True "
+            "on detached tensors and its *_backward")
+
+
+def _resident(x):
+    require(x.is_cuda, "inputs must be CUDA-resident (there is no CPU path)")
+
+
+def _given_out(out, shape, x, others):
+    """A result tensor of the caller, as rows."""
+    _check("out", out, x.dtype, x.device)
+    require(tuple(out.shape) == tuple(shape), f"out must be {tuple(shape)}, got {tuple(out.shape)}")
+    _apart("out", out, others)
+    out2 = _rows2d("out", out, shape[-1])
+    _pitch("out", out2)
+    return out2
+
+
+def _result(out, out2, shape, x):
+    """The result tensor, as the caller sees it and as rows."""
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        return out, out if out.dim() == 2 else out.view(-1, shape[-1])
+    increment_version(out)
+    return out, out2
+
+
+# ---------------------------------------------------------------------------
+# gated projection
+# ---------------------------------------------------------------------------
+
+def _gated_kind(activation, swiglu_limit, beta):
+    require(activation in (SWIGLU, SITU), "activation must be SWIGLU or SITU")
+    require(swiglu_limit >= 0, "swiglu_limit must not be negative (0 for none)")
+    require(activation == SWIGLU or beta > 0, "SiTU needs a positive beta")
+
+
+def gated_linear(x: torch.Tensor, w13: torch.Tensor, b13: torch.Tensor | None = None, *, activation: int = SWIGLU,
+                 swiglu_limit: float = 0.0, beta: float = 4.0, linear_beta: float = 25.0, out: torch.Tensor | None = None,
+                 return_preact: bool = False):
+    """``h [..., ispp] = act(x Wg^T + bg) * (x Wu^T + bu)`` for x ``[..., hidden]`` and w13 ``[2 * ispp, hidden]`` (gate rows, then
+    up rows; b13 ``[2 * ispp]`` likewise). SwiGLU: gate * sigmoid(gate) * up, the gate clamped from above and up from both sides
+    at `swiglu_limit` if that is positive; SiTU: beta tanh(gate / beta) sigmoid(gate) * linear_beta tanh(up / linear_beta).
+
+    ``return_preact``: also return what ``gated_linear_backward`` needs, the pre-activations ``[T, 2 * ispp]`` in the type of x
+    (T: all leading dimensions of x together)."""
+    x2 = _inputs(x, w13, 2, "gated_linear")
+    _gated_kind(activation, swiglu_limit, beta)
+    rows, ispp = w13.shape[0], w13.shape[0] // 2
+    b = _bias(b13, rows, x)
+    T, hidden = x2.shape
+    shape = (*x.shape[:-1], ispp)
+    out2 = None if out is None else _given_out(out, shape, x, (("x", x), ("w13", w13), ("b13", b13)))
+    _resident(x)
+    if _wants_grad(x, w13, b13, out):
+        require(out is None and not return_preact, "gated_linear: out and return_preact are for calls that record no gradient")
+        return _GatedLinear.apply(x, w13, b13, activation, swiglu_limit, beta, linear_beta)
+    h, h2 = _result(out, out2, shape, x)
+    preact = torch.empty((T, rows), dtype=x.dtype, device=x.device) if return_preact else None
+    if T > 0:
+        xk, xp, ldx = _operand("x", x2)
+        wk, wp, ldw = _operand("w13", w13)
+        _call("vk_cuda_gated_linear", x.device, xp, ldx, wp, ldw, b, h2.data_ptr(), _pitch("out", h2),
+              None if preact is None else preact.data_ptr(), rows, _DTYPE[x.dtype], T, hidden, ispp, activation, swiglu_limit, beta,
+              linear_beta)
+    return (h, preact) if return_preact else h
+
+
+def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w13: torch.Tensor, preact: torch.Tensor, *, activation: int = SWIGLU,
+                          swiglu_limit: float = 0.0, beta: float = 4.0, linear_beta: float = 25.0, bias_grad: bool = False,
+                          x_grad: bool = True, w_grad: bool = True):
+    """``(dx, dw13, db13)`` for the gradient dh of ``gated_linear``'s result; ``preact`` as that call returned it, the other
+    arguments as it was given. What is not asked for is None."""
+    x2 = _inputs(x, w13, 2, "gated_linear_backward")
+    _gated_kind(activation, swiglu_limit, beta)
+    ispp = w13.shape[0] // 2
+    require(preact is not None, "gated_linear_backward needs the forward call's pre-activations")
+    return _backward("vk_cuda_gated_linear_backward", dh, x, x2, w13, preact, ispp, True, bias_grad, x_grad, w_grad,
+                     (activation, swiglu_limit, beta, linear_beta))
+
+
+# ---------------------------------------------------------------------------
+# projection with epilogue
+# ---------------------------------------------------------------------------
+
+def _linear_kind(activation):
+    kind = _LINEAR_ACT.get(activation) if activation is None or isinstance(activation, str) else None
+    require(kind is not None, f"activation must be None, 'silu', 'gelu' or 'gelu_tanh', got {activation!r}")
+    return kind
+
+
+def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None,
+                 residual: torch.Tensor | None = None, out: torch.Tensor | None = None, return_preact: bool = False):
+    """``y [..., n_out] = act(x w^T + bias) + residual`` for x ``[..., n_in]``, w ``[n_out, n_in]``; activation None, "silu",
+    "gelu" (erf) or "gelu_tanh"; residual of y's shape (not broadcast). ``out`` may be the residual itself.
+
+    ``return_preact``: also return what ``fused_linear_backward`` needs: the pre-activations ``[T, n_out]``, or None where there
+    is no activation."""
+    x2 = _inputs(x, w, 1, "fused_linear")
+    act = _linear_kind(activation)
+    n_out = w.shape[0]
+    b = _bias(bias, n_out, x)
+    shape = (*x.shape[:-1], n_out)
+    r2, ldr = None, 0
+    if residual is not None:
+        _check("the residual", residual, x.dtype, x.device)
+        require(tuple(residual.shape) == shape, f"the residual must be {shape}, got {tuple(residual.shape)}")
+        r2 = _rows2d("the residual", residual, n_out)
+        ldr = _pitch("the residual", r2)
+    out2 = None
+    if out is not None:
+        in_place = residual is not None and out.data_ptr() == residual.data_ptr() and out.stride() == residual.stride()
+        out2 = _given_out(out, shape, x, (("x", x), ("w", w), ("the bias", bias), ("the residual", None if in_place else residual)))
+    _resident(x)
+    if _wants_grad(x, w, bias, residual, out):
+        require(out is None and not return_preact, "fused_linear: out and return_preact are for calls that record no gradient")
+        return _FusedLinear.apply(x, w, bias, residual, activation)
+    T, n_in = x2.shape
+    y, y2 = _result(out, out2, shape, x)
+    preact = torch.empty((T, n_out), dtype=x.dtype, device=x.device) if return_preact and act else None
+    if T > 0:
+        xk, xp, ldx = _operand("x", x2)
+        wk, wp, ldw = _operand("w", w)
+        _call("vk_cuda_fused_linear", x.device, xp, ldx, wp, ldw, b, None if r2 is None else r2.data_ptr(), ldr, y2.data_ptr(), _pitch("out", y2),
+              None if preact is None else preact.data_ptr(), n_out, _DTYPE[x.dtype], T, n_in, n_out, act)
+    return (y, preact) if return_preact else y
+
+
+def fused_linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, preact: torch.Tensor | None = None, *,
+                          activation: str | None = None, bias_grad: bool = False, x_grad: bool = True, w_grad: bool = True):
+    """``(dx, dw, dbias)`` for the gradient dy of ``fused_linear``'s result; ``preact`` as that call returned it (None without an
+    activation). What is not asked for is None. The residual's gradient is dy."""
+    x2 = _inputs(x, w, 1, "fused_linear_backward")
+    act = _linear_kind(activation)
+    require(act == 0 or preact is not None, "fused_linear_backward needs the forward call's pre-activations")
+    return _backward("vk_cuda_fused_linear_backward", dy, x, x2, w, preact if act else None, w.shape[0], False, bias_grad, x_grad,
+                     w_grad, (act,))
+
+
+def _backward(entry, dy, x, x2, w, preact, n_out, gated, bias_grad, x_grad, w_grad, kind):
+    rows, (T, n_in) = w.shape[0], x2.shape
+    dtype, device = x.dtype, x.device
+    _check("the result's gradient", dy, dtype, device)
+    require(tuple(dy.shape) == (*x.shape[:-1], n_out), f"the result's gradient must be {(*x.shape[:-1], n_out)}, got {tuple(dy.shape)}")
+    dy2 = dy if dy.dim() == 2 else dy.reshape(-1, n_out)
+    if preact is not None:
+        _check("preact", preact, dtype, device)
+        require(tuple(preact.shape) == (T, rows), f"preact must be {(T, rows)}, got {tuple(preact.shape)}")
+    ld_dy, ld_p = _pitch("the result's gradient", dy2), 0 if preact is None else _pitch("preact", preact)
+    _resident(x)
+    dx = torch.empty(x.shape, dtype=dtype, device=device) if x_grad else None
+    dw = torch.empty((rows, n_in), dtype=dtype, device=device) if w_grad else None
+    db = torch.empty(rows, dtype=dtype, device=device) if bias_grad else None
+    if dx is None and dw is None and db is None:
+        return None, None, None
+    nbytes = nr.load_library().vk_cuda_dense_backward_workspace_bytes(T, n_out, int(gated))
+    work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    xk, xp, ldx = _operand("x", x2) if w_grad and T > 0 else (x2, None, 0)
+    wk, wp, ldw = _operand("the weight", w) if x_grad and T > 0 else (w, None, 0)
+    _call(entry, device, dy2.data_ptr(), ld_dy, xp, ldx, wp, ldw, None if preact is None else preact.data_ptr(), ld_p,
+          None if dx is None else dx.data_ptr(), n_in, None if dw is None else dw.data_ptr(), n_in, None if db is None else db.data_ptr(),
+          _DTYPE[dtype], T, n_in, n_out, *kind, work.data_ptr(), nbytes)
+    return dx, dw, db
+
+
+# ---------------------------------------------------------------------------
+# recording for backward()
+# ---------------------------------------------------------------------------
+
+def _plain_rows(t):
+    """A gradient as autograd hands it over (it may be an expanded number), with rows that the kernels take."""
+    return t if t.stride(-1) == 1 and (t.dim() < 2 or t.stride(-2) >= t.shape[-1]) else t.contiguous()
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w13, b13, activation, swiglu_limit, beta, linear_beta):
+        _no_capture()
+        ctx.kw = dict(activation=activation, swiglu_limit=swiglu_limit, beta=beta, linear_beta=linear_beta)
+        with torch.no_grad():
+            h, preact = gated_linear(x, w13, b13, return_preact=True, **ctx.kw)
+        ctx.save_for_backward(x, w13, preact)
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        _no_capture()
+        x, w13, preact = ctx.saved_tensors
+        nx, nw, nb = ctx.needs_input_grad[:3]
+        dx, dw, db = gated_linear_backward(_plain_rows(dh), x, w13, preact, x_grad=nx, w_grad=nw, bias_grad=nb, **ctx.kw)
+        return dx, dw, db, None, None, None, None
+
+
+class _FusedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, activation):
+        _no_capture()
+        ctx.activation = activation
+        with torch.no_grad():
+            y, preact = fused_linear(x, w, bias, activation=activation, residual=residual, return_preact=True)
+        ctx.save_for_backward(x, w, preact)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _no_capture()
+        x, w, preact = ctx.saved_tensors
+        nx, nw, nb, nr_, _ = ctx.needs_input_grad
+        dx, dw, db = fused_linear_backward(_plain_rows(dy), x, w, preact, activation=ctx.activation, x_grad=nx, w_grad=nw,
+                                           bias_grad=nb)
+        return dx, dw, db, dy if nr_ else None, None
