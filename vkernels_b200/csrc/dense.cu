@@ -40,7 +40,8 @@ float effective_limit(bool gated, int act, float limit) { return gated && act ==
 
 void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream) {
   if (g.M == 0 || g.N == 0) return;
-  launch_dense_simt(g, stream);
+  if (get_moe_impl() == MoeImpl::kSimt) launch_dense_simt(g, stream);
+  else launch_dense_wide(g, stream);
 }
 
 void dense_forward(const DenseForward& f, cudaStream_t stream) {

@@ -60,6 +60,7 @@ struct DenseGrad {
 
 int dense_sum_chunks(int T);
 void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream);
+void launch_dense_wide(const DenseGemm& g, cudaStream_t stream);   // dense_gemm.cu
 void launch_dense_simt(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_grad(const DenseGrad& g, cudaStream_t stream);
 // db[n] = sum over the chunks of partial[chunk, n], in order.
