@@ -389,40 +389,41 @@ int vk_cuda_fused_moe_mxfp4_rows(const uint64_t* a_rows, const uint8_t* w13, con
                                  int block_size, void* stream);
 
 /* Dense feed-forward in 16 bits (additive): the layers of a mixture-of-experts model that are not routed - its dense layers, and
- * an always-on expert that the checkpoint keeps in bf16 or fp16. dtype: 0 = bf16, 1 = fp16, the type of every tensor of a call.
- * Matrices are row-major with a row pitch (ld*, in elements). x and w (w13) must start on 16 bytes and have a pitch that is a
- * multiple of 8 (vk_cuda_dense_copy_rows brings others there); all other pointers need only the alignment of their type.
- * Results and inputs must not overlap, except that y may be the residual itself (same address and pitch). Sums are fp32; one
- * rounding at the end. No atomics: a call gives the same bits every time. The calls allocate nothing and use no library
- * scratch, so any number of them may run or be captured at once. T = 0 is no work (weight gradients become zero).
+ * an always-on expert that the checkpoint keeps in bf16 or fp16. dtype: 0 = bf16, 1 = fp16, the type of every tensor of a call
+ * but preact. Matrices are row-major with a row pitch (ld*, in elements, at least the row); pointers need the alignment of
+ * their type. Results and inputs must not overlap, except that y may be the residual itself (same address and pitch). Sums are
+ * fp32 and rounded once at the end. No atomics: a call gives the same bits every time. The calls allocate nothing and use no
+ * library scratch, so any number of them may run or be captured at once, each with a workspace of its own (on 16 bytes, the
+ * caller's until the work is done). T = 0 is no work (weight gradients become zero).
  *
  * vk_cuda_gated_linear: z = x [T, hidden] . w13 [2*ispp, hidden]^T + b13 [2*ispp] (or NULL), gate columns first;
  *   h [T, ispp] = act(z): activation 0 = SwiGLU (inputs clamped at swiglu_limit when > 0, as in the routed layer), 1 = SiTU(beta,
- *   linear_beta). preact (or NULL) [T, 2*ispp] receives z for the backward pass, rounded to the type on its side of the limit.
+ *   linear_beta). preact (or NULL) [T, 2*ispp] fp32 receives z for the backward pass.
  * vk_cuda_fused_linear: z = x [T, n_in] . w [n_out, n_in]^T + bias [n_out] (or NULL); y [T, n_out] = act(z) + residual [T, n_out]
- *   (or NULL): activation 0 = none, 1 = silu, 2 = gelu (erf), 3 = gelu (tanh form). preact (or NULL) [T, n_out] receives z.
+ *   (or NULL): activation 0 = none, 1 = silu, 2 = gelu (erf), 3 = gelu (tanh form). preact (or NULL) [T, n_out] fp32 receives z.
+ *   Both take x and w as they lie where they start on 16 bytes and have a pitch that is a multiple of 8; others are copied
+ *   first, into a workspace of vk_cuda_dense_forward_workspace_bytes bytes (0: none needed, NULL will do).
  * *_backward: gradients for the gradient of the result (dh / dy); each of dx, dw (dw13), db (db13) may be NULL. The activation
  *   arguments and preact are those of the forward call (preact unused for activation 0 of the linear form); the residual's
- *   gradient is dy. The gradient of z is rounded to the type once, as the products' operand, in `workspace`
- *   (vk_cuda_dense_backward_workspace_bytes bytes, on 16 bytes, the caller's until the work is done); db sums it unrounded. */
+ *   gradient is dy. The gradient of z is rounded to the type once, as the products' operand, in the workspace
+ *   (vk_cuda_dense_backward_workspace_bytes bytes); db sums it unrounded. */
 int vk_cuda_gated_linear(const void* x, int64_t ldx, const void* w13, int64_t ldw, const void* b13, void* h, int64_t ldh,
-                         void* preact, int64_t ldp, int dtype, int T, int hidden, int ispp, int activation, float swiglu_limit,
-                         float beta, float linear_beta, void* stream);
+                         float* preact, int64_t ldp, int dtype, int T, int hidden, int ispp, int activation, float swiglu_limit,
+                         float beta, float linear_beta, void* workspace, size_t workspace_bytes, void* stream);
 int vk_cuda_fused_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
-                         int64_t ldr, void* y, int64_t ldy, void* preact, int64_t ldp, int dtype, int T, int n_in, int n_out,
-                         int activation, void* stream);
-size_t vk_cuda_dense_backward_workspace_bytes(int T, int n_out, int gated);
+                         int64_t ldr, void* y, int64_t ldy, float* preact, int64_t ldp, int dtype, int T, int n_in, int n_out,
+                         int activation, void* workspace, size_t workspace_bytes, void* stream);
+size_t vk_cuda_dense_forward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int w_rows);
+size_t vk_cuda_dense_backward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int n_out,
+                                              int gated);
 int vk_cuda_gated_linear_backward(const void* dh, int64_t lddh, const void* x, int64_t ldx, const void* w13, int64_t ldw,
-                                  const void* preact, int64_t ldp, void* dx, int64_t lddx, void* dw13, int64_t lddw, void* db13,
+                                  const float* preact, int64_t ldp, void* dx, int64_t lddx, void* dw13, int64_t lddw, void* db13,
                                   int dtype, int T, int hidden, int ispp, int activation, float swiglu_limit, float beta,
                                   float linear_beta, void* workspace, size_t workspace_bytes, void* stream);
 int vk_cuda_fused_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
-                                  const void* preact, int64_t ldp, void* dx, int64_t lddx, void* dw, int64_t lddw, void* db,
+                                  const float* preact, int64_t ldp, void* dx, int64_t lddx, void* dw, int64_t lddw, void* db,
                                   int dtype, int T, int n_in, int n_out, int activation, void* workspace,
                                   size_t workspace_bytes, void* stream);
-/* dst[r, c] = src[r, c] for 16-bit values, any alignment, pitches in elements. */
-int vk_cuda_dense_copy_rows(const void* src, int64_t src_ld, void* dst, int64_t dst_ld, int rows, int cols, void* stream);
-
 #ifdef __cplusplus
 }
 #endif

@@ -21,7 +21,7 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(ops.OpNotEligible, match="CUDA"):
         ops.fused_linear(t(2, 8), t(16, 8))
     with pytest.raises(ops.OpNotEligible, match="CUDA"):
-        ops.gated_linear_backward(t(2, 8), t(2, 8), t(16, 8), t(2, 16))
+        ops.gated_linear_backward(t(2, 8), t(2, 8), t(16, 8), t(2, 16, dtype=torch.float32))
     with pytest.raises(ops.OpNotEligible, match="CUDA"):
         ops.fused_linear_backward(t(2, 16), t(2, 8), t(16, 8))
     with pytest.raises(ops.OpNotEligible, match="CUDA"):
@@ -53,8 +53,9 @@ def test_cpu_tensors_are_refused():
     ("like the other", lambda: ops.fused_linear(t(2, 8), t(16, 8), out=t(2, 16, dtype=torch.float16))),
     ("neighbours", lambda: ops.fused_linear(t(2, 8), t(16, 8), out=t(16, 2).T)),
     ("overlap", lambda: ops.fused_linear(t(2, 8), t(16, 8), out=t(1, 16).expand(2, 16))),
-    ("gradient must be", lambda: ops.gated_linear_backward(t(2, 16), t(2, 8), t(16, 8), t(2, 16))),
-    ("preact must be", lambda: ops.gated_linear_backward(t(2, 8), t(2, 8), t(16, 8), t(2, 8))),
+    ("gradient must be", lambda: ops.gated_linear_backward(t(2, 16), t(2, 8), t(16, 8), t(2, 16, dtype=torch.float32))),
+    ("preact must be", lambda: ops.gated_linear_backward(t(2, 8), t(2, 8), t(16, 8), t(2, 8, dtype=torch.float32))),
+    ("preact must be", lambda: ops.gated_linear_backward(t(2, 8), t(2, 8), t(16, 8), t(2, 16))),
     ("pre-activations", lambda: ops.gated_linear_backward(t(2, 8), t(2, 8), t(16, 8), None)),
     ("pre-activations", lambda: ops.fused_linear_backward(t(2, 16), t(2, 8), t(16, 8), activation="silu")),
     ("overlap", lambda: ops.fused_linear_backward(t(1, 16).expand(2, 16), t(2, 8), t(16, 8))),
@@ -84,14 +85,14 @@ P = 1 << 20      # an aligned address that is never followed: every call below i
 
 def linear_args(**k):
     a = dict(x=P, ldx=64, w=P, ldw=64, bias=None, residual=None, ldr=0, y=P, ldy=64, preact=None, ldp=0, dtype=0, T=4, n_in=64,
-             n_out=64, act=0, stream=None)
+             n_out=64, act=0, work=None, nbytes=0, stream=None)
     assert not set(k) - set(a)
     return list({**a, **k}.values())
 
 
 def gated_args(**k):
     a = dict(x=P, ldx=64, w=P, ldw=64, bias=None, h=P, ldh=64, preact=None, ldp=0, dtype=0, T=4, n_in=64, ispp=64, act=0, limit=0.0,
-             beta=4.0, lbeta=25.0, stream=None)
+             beta=4.0, lbeta=25.0, work=None, nbytes=0, stream=None)
     assert not set(k) - set(a)
     return list({**a, **k}.values())
 
@@ -104,10 +105,11 @@ def linear_back_args(**k):
 
 
 @pytest.mark.parametrize("bad,word", [
-    (dict(dtype=2), b"dtype"), (dict(T=-1), b"T"), (dict(n_in=0), b"positive"), (dict(n_out=0), b"positive"), (dict(x=None), b"x is null"),
-    (dict(w=None), b"w is null"), (dict(x=P + 2), b"16 bytes"), (dict(w=P + 8), b"16 bytes"), (dict(ldx=68), b"multiple of 8"),
+    (dict(dtype=2), b"dtype"), (dict(T=-1), b"T"), (dict(n_in=0), b"positive"), (dict(n_out=0), b"positive"), (dict(x=None), b"null"),
+    (dict(w=None), b"null"), (dict(x=P + 1), b"odd"), (dict(x=P + 2), b"workspace"), (dict(w=P + 8), b"workspace"),
+    (dict(ldx=68), b"workspace"), (dict(x=P + 2, work=P, nbytes=511), b"workspace"), (dict(ldw=66, work=P + 8, nbytes=1 << 20), b"workspace"),
     (dict(ldw=56), b"pitch"), (dict(y=None), b"null"), (dict(y=P + 1), b"odd"), (dict(ldy=63), b"pitch"), (dict(bias=P + 1), b"bias"),
-    (dict(residual=P + 1, ldr=64), b"odd"), (dict(residual=P, ldr=63), b"pitch"), (dict(preact=P, ldp=63), b"pitch"),
+    (dict(residual=P + 1, ldr=64), b"odd"), (dict(residual=P, ldr=63), b"pitch"), (dict(preact=P, ldp=63), b"pitch"), (dict(preact=P + 2, ldp=64), b"preact"),
     (dict(act=4), b"activation"), (dict(act=-1), b"activation"), (dict(n_in=(1 << 30) + 1), b"sizes")])
 def test_linear_entry_refuses(bad, word):
     lib = nr.load_library()
@@ -116,7 +118,7 @@ def test_linear_entry_refuses(bad, word):
 
 @pytest.mark.parametrize("bad,word", [
     (dict(dtype=-1), b"dtype"), (dict(act=2), b"SwiGLU"), (dict(limit=-1.0), b"limit"), (dict(limit=float("nan")), b"limit"),
-    (dict(act=1, beta=0.0), b"beta"), (dict(preact=P, ldp=127), b"pitch"), (dict(ldh=63), b"pitch"), (dict(x=P + 4), b"16 bytes")])
+    (dict(act=1, beta=0.0), b"beta"), (dict(preact=P, ldp=127), b"pitch"), (dict(ldh=63), b"pitch"), (dict(x=P + 4), b"workspace")])
 def test_gated_entry_refuses(bad, word):
     lib = nr.load_library()
     assert lib.vk_cuda_gated_linear(*gated_args(**bad)) == 1 and word in lib.vk_last_error(), lib.vk_last_error()
@@ -125,7 +127,8 @@ def test_gated_entry_refuses(bad, word):
 @pytest.mark.parametrize("bad,word", [
     (dict(preact=None), b"pre-activations"), (dict(dy=None), b"null"), (dict(lddy=63), b"pitch"), (dict(dx=P + 1), b"odd"),
     (dict(lddw=63), b"pitch"), (dict(db=P + 1), b"odd"), (dict(work=None), b"workspace"), (dict(work=P + 8), b"workspace"),
-    (dict(nbytes=16), b"workspace"), (dict(x=P + 2), b"16 bytes"), (dict(w=P + 2), b"16 bytes"), (dict(x=None), b"x is null")])
+    (dict(nbytes=16), b"workspace"), (dict(x=P + 1), b"odd"), (dict(w=P + 1), b"odd"), (dict(x=None), b"null"),
+    (dict(preact=P + 2), b"preact")])
 def test_linear_backward_entry_refuses(bad, word):
     lib = nr.load_library()
     assert lib.vk_cuda_fused_linear_backward(*linear_back_args(**bad)) == 1 and word in lib.vk_last_error(), lib.vk_last_error()
@@ -137,11 +140,18 @@ def test_no_tokens_and_nothing_asked_are_no_work():
     assert lib.vk_cuda_gated_linear(*gated_args(T=0, x=None, h=None)) == 0
     assert lib.vk_cuda_fused_linear_backward(*linear_back_args(dx=None, dw=None, db=None, work=None)) == 0
     assert lib.vk_cuda_fused_linear_backward(*linear_back_args(T=0, dw=None, db=None)) == 0
-    assert lib.vk_cuda_dense_backward_workspace_bytes(-1, 8, 0) == 0 and lib.vk_last_error_code() == 1
-    assert lib.vk_cuda_dense_backward_workspace_bytes(100, 13, 1) >= 100 * 32 * 2 + 26 * 4
-    assert lib.vk_cuda_dense_copy_rows(None, 8, None, 8, 0, 8, None) == 0
-    assert lib.vk_cuda_dense_copy_rows(None, 8, P, 8, 1, 8, None) == 1
-    assert lib.vk_cuda_dense_copy_rows(P, 7, P, 8, 1, 8, None) == 1
+
+
+def test_workspace_sizes():
+    lib = nr.load_library()
+    fwd, back = lib.vk_cuda_dense_forward_workspace_bytes, lib.vk_cuda_dense_backward_workspace_bytes
+    assert fwd(P, 64, P, 64, 4, 64, 64) == 0 and fwd(P + 2, 64, P, 64, 0, 64, 64) == 0
+    assert fwd(P + 2, 64, P, 64, 4, 64, 64) == 4 * 64 * 2 and fwd(P, 64, P, 70, 4, 60, 3) == 512   # 3 rows of 64, in whole 256 bytes
+    assert back(P, 64, P, 64, 100, 64, 13, 1) >= 100 * 32 * 2 + 26 * 4
+    assert back(P + 2, 64, P, 64, 100, 64, 13, 1) >= back(P, 64, P, 64, 100, 64, 13, 1) + 100 * 64 * 2
+    assert fwd(P, 64, P, 64, -1, 64, 64) == 0 and lib.vk_last_error_code() == 1
+    lib.vk_set_last_error(0, b"")
+    assert back(P, 64, P, 64, -1, 64, 8, 0) == 0 and lib.vk_last_error_code() == 1
 
 
 @pytest.mark.parametrize("kind,limit,linear_beta", [("swiglu", 0.0, 25.0), ("swiglu", 1.0, 25.0), ("situ", 0.0, 25.0), ("situ", 0.0, 0.0)])

@@ -594,8 +594,8 @@ int32_t vk_fused_moe_mxfp4(const uint16_t* A, const uint8_t* w13, const uint8_t*
 /* ---------------- dense feed-forward operators ---------------- */
 
 int vk_cuda_gated_linear(const void* x, int64_t ldx, const void* w13, int64_t ldw, const void* b13, void* h, int64_t ldh,
-                         void* preact, int64_t ldp, int dtype, int T, int hidden, int ispp, int activation, float swiglu_limit,
-                         float beta, float linear_beta, void* stream) {
+                         float* preact, int64_t ldp, int dtype, int T, int hidden, int ispp, int activation, float swiglu_limit,
+                         float beta, float linear_beta, void* workspace, size_t workspace_bytes, void* stream) {
   VK_TRY
   vkc::DenseForward f{};
   f.type = static_cast<vkc::DenseType>(dtype);
@@ -603,17 +603,18 @@ int vk_cuda_gated_linear(const void* x, int64_t ldx, const void* w13, int64_t ld
   f.w = static_cast<const uint16_t*>(w13);
   f.bias = static_cast<const uint16_t*>(b13);
   f.y = static_cast<uint16_t*>(h);
-  f.preact = static_cast<uint16_t*>(preact);
+  f.preact = preact;
   f.ldx = ldx, f.ldw = ldw, f.ldy = ldh, f.ldp = ldp;
   f.T = T, f.n_in = hidden, f.n_out = ispp;
   f.gated = true, f.act = activation, f.limit = swiglu_limit, f.beta = beta, f.linear_beta = linear_beta;
+  f.workspace = workspace, f.workspace_bytes = workspace_bytes;
   vkc::dense_forward(f, static_cast<cudaStream_t>(stream));
   VK_CATCH(return VK_OK, VK_RETURN_CODE)
 }
 
 int vk_cuda_fused_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
-                         int64_t ldr, void* y, int64_t ldy, void* preact, int64_t ldp, int dtype, int T, int n_in, int n_out,
-                         int activation, void* stream) {
+                         int64_t ldr, void* y, int64_t ldy, float* preact, int64_t ldp, int dtype, int T, int n_in, int n_out,
+                         int activation, void* workspace, size_t workspace_bytes, void* stream) {
   VK_TRY
   vkc::DenseForward f{};
   f.type = static_cast<vkc::DenseType>(dtype);
@@ -622,23 +623,32 @@ int vk_cuda_fused_linear(const void* x, int64_t ldx, const void* w, int64_t ldw,
   f.bias = static_cast<const uint16_t*>(bias);
   f.residual = static_cast<const uint16_t*>(residual);
   f.y = static_cast<uint16_t*>(y);
-  f.preact = static_cast<uint16_t*>(preact);
+  f.preact = preact;
   f.ldx = ldx, f.ldw = ldw, f.ldr = ldr, f.ldy = ldy, f.ldp = ldp;
   f.T = T, f.n_in = n_in, f.n_out = n_out;
   f.act = activation;
+  f.workspace = workspace, f.workspace_bytes = workspace_bytes;
   vkc::dense_forward(f, static_cast<cudaStream_t>(stream));
   VK_CATCH(return VK_OK, VK_RETURN_CODE)
 }
 
-size_t vk_cuda_dense_backward_workspace_bytes(int T, int n_out, int gated) {
+size_t vk_cuda_dense_forward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int w_rows) {
   size_t n = 0;
   VK_TRY
-  n = vkc::dense_backward_workspace_bytes(T, n_out, gated != 0);
+  n = vkc::dense_forward_workspace_bytes(x, ldx, w, ldw, T, n_in, w_rows);
+  VK_CATCH(return n, VK_RETURN_ZERO)
+}
+
+size_t vk_cuda_dense_backward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int n_out,
+                                              int gated) {
+  size_t n = 0;
+  VK_TRY
+  n = vkc::dense_backward_workspace_bytes(x, ldx, w, ldw, T, n_in, n_out, gated != 0);
   VK_CATCH(return n, VK_RETURN_ZERO)
 }
 
 int vk_cuda_gated_linear_backward(const void* dh, int64_t lddh, const void* x, int64_t ldx, const void* w13, int64_t ldw,
-                                  const void* preact, int64_t ldp, void* dx, int64_t lddx, void* dw13, int64_t lddw, void* db13,
+                                  const float* preact, int64_t ldp, void* dx, int64_t lddx, void* dw13, int64_t lddw, void* db13,
                                   int dtype, int T, int hidden, int ispp, int activation, float swiglu_limit, float beta,
                                   float linear_beta, void* workspace, size_t workspace_bytes, void* stream) {
   VK_TRY
@@ -647,7 +657,7 @@ int vk_cuda_gated_linear_backward(const void* dh, int64_t lddh, const void* x, i
   f.dy = static_cast<const uint16_t*>(dh);
   f.x = static_cast<const uint16_t*>(x);
   f.w = static_cast<const uint16_t*>(w13);
-  f.preact = static_cast<const uint16_t*>(preact);
+  f.preact = preact;
   f.dx = static_cast<uint16_t*>(dx);
   f.dw = static_cast<uint16_t*>(dw13);
   f.db = static_cast<uint16_t*>(db13);
@@ -660,7 +670,7 @@ int vk_cuda_gated_linear_backward(const void* dh, int64_t lddh, const void* x, i
 }
 
 int vk_cuda_fused_linear_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
-                                  const void* preact, int64_t ldp, void* dx, int64_t lddx, void* dw, int64_t lddw, void* db,
+                                  const float* preact, int64_t ldp, void* dx, int64_t lddx, void* dw, int64_t lddw, void* db,
                                   int dtype, int T, int n_in, int n_out, int activation, void* workspace,
                                   size_t workspace_bytes, void* stream) {
   VK_TRY
@@ -669,7 +679,7 @@ int vk_cuda_fused_linear_backward(const void* dy, int64_t lddy, const void* x, i
   f.dy = static_cast<const uint16_t*>(dy);
   f.x = static_cast<const uint16_t*>(x);
   f.w = static_cast<const uint16_t*>(w);
-  f.preact = static_cast<const uint16_t*>(preact);
+  f.preact = preact;
   f.dx = static_cast<uint16_t*>(dx);
   f.dw = static_cast<uint16_t*>(dw);
   f.db = static_cast<uint16_t*>(db);
@@ -678,15 +688,6 @@ int vk_cuda_fused_linear_backward(const void* dy, int64_t lddy, const void* x, i
   f.act = activation;
   f.workspace = workspace, f.workspace_bytes = workspace_bytes;
   vkc::dense_backward(f, static_cast<cudaStream_t>(stream));
-  VK_CATCH(return VK_OK, VK_RETURN_CODE)
-}
-
-int vk_cuda_dense_copy_rows(const void* src, int64_t src_ld, void* dst, int64_t dst_ld, int rows, int cols, void* stream) {
-  VK_TRY
-  vkc::expects(rows >= 0 && cols >= 0 && src_ld >= cols && dst_ld >= cols, "dense_copy_rows: bad sizes or pitches");
-  vkc::expects(rows == 0 || cols == 0 || (src != nullptr && dst != nullptr), "dense_copy_rows: null pointer");
-  vkc::launch_dense_copy_rows(static_cast<const uint16_t*>(src), src_ld, static_cast<uint16_t*>(dst), dst_ld, rows, cols,
-                              static_cast<cudaStream_t>(stream));
   VK_CATCH(return VK_OK, VK_RETURN_CODE)
 }
 

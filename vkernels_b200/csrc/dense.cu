@@ -25,39 +25,74 @@ void check_common(DenseType type, int T, int n_in, int n_out, bool gated, int ac
     expects(act >= kActNone && act <= kActGeluTanh, "fused_linear: activation must be 0 (none), 1 (silu), 2 (gelu) or 3 (gelu_tanh)");
   }
 }
-void check_operand(const void* p, int64_t ld, int cols, const char* null_msg, const char* align_msg) {
-  expects(p != nullptr, null_msg);
-  expects(ld >= cols, "dense: a row pitch is smaller than its row");
-  expects(tma_ready(p, ld), align_msg);
-}
-void check_result(const void* p, int64_t ld, int cols) {
+void check_matrix(const void* p, int64_t ld, int cols) {
   expects(p != nullptr && even(p), "dense: null or odd pointer");
   expects(ld >= cols, "dense: a row pitch is smaller than its row");
+}
+void check_preact(const float* p, int64_t ld, int cols) {
+  expects((reinterpret_cast<uintptr_t>(p) & 3u) == 0, "dense: preact must be aligned to its fp32 values");
+  expects(ld >= cols, "dense: a row pitch is smaller than its row");
+}
+
+size_t copy_bytes(const void* p, int64_t ld, int rows, int cols) {
+  return p == nullptr || tma_ready(p, ld) ? 0 : round_up((size_t)rows * round_up((size_t)cols, 8) * 2, 256);
+}
+
+// x and w as a tensor map takes them: as they are, or copied to rows on 16 bytes at the start of the workspace. Returns the
+// bytes used; a null operand is left alone.
+size_t bring_operands(const uint16_t*& x, int64_t& ldx, int T, const uint16_t*& w, int64_t& ldw, int w_rows, int cols, void* workspace,
+                      size_t workspace_bytes, cudaStream_t stream) {
+  const size_t bx = copy_bytes(x, ldx, T, cols), bw = copy_bytes(w, ldw, w_rows, cols);
+  if (bx + bw == 0) return 0;
+  expects(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "dense: workspace must start on 16 bytes");
+  expects(workspace_bytes >= bx + bw, "dense: workspace smaller than the copies of x and w that their alignment calls for");
+  char* base = static_cast<char*>(workspace);
+  const uint16_t* src[2] = {x, w};
+  const int64_t lds[2] = {ldx, ldw};
+  uint16_t* dst[2] = {bx ? reinterpret_cast<uint16_t*>(base) : nullptr, bw ? reinterpret_cast<uint16_t*>(base + bx) : nullptr};
+  const int rows[2] = {T, w_rows};
+  launch_dense_copy_rows(src, lds, dst, rows, cols, stream);
+  const int64_t pitch = (int64_t)round_up((size_t)cols, 8);
+  if (bx) x = dst[0], ldx = pitch;
+  if (bw) w = dst[1], ldw = pitch;
+  return bx + bw;
 }
 float effective_limit(bool gated, int act, float limit) { return gated && act == 0 && limit > 0.0f ? limit : INFINITY; }
 
 }  // namespace
 
+// Small batches go to the kernel that cuts k over clusters, the others to the CTA pairs: whichever takes less by the sizes. The
+// line lies near 64 tokens for short reductions of many features, at 256 for long ones of few (128 tokens: 2048 -> 7168 13.1 us
+// and 11.2, 2880 -> 2880 9.8 and 12, 7168 -> 2 x 2048 gated 16.4 and 24; 256 tokens 18.8 and 11.2, 12.9 and 12.1, 19.7 and 24.6).
 void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream) {
   if (g.M == 0 || g.N == 0) return;
   if (get_moe_impl() == MoeImpl::kSimt) launch_dense_simt(g, stream);
+  else if (!g.a.mn_major && g.M <= 256 && dense_narrow_us(g) < dense_wide_us(g)) launch_dense_narrow(g, stream);
   else launch_dense_wide(g, stream);
+}
+
+size_t dense_forward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int w_rows) {
+  expects(T >= 0 && n_in > 0 && w_rows > 0, "dense: T must not be negative, feature counts must be positive");
+  return T == 0 ? 0 : copy_bytes(x, ldx, T, n_in) + copy_bytes(w, ldw, w_rows, n_in);
 }
 
 void dense_forward(const DenseForward& f, cudaStream_t stream) {
   check_common(f.type, f.T, f.n_in, f.n_out, f.gated, f.act, f.limit, f.beta);
   if (f.T == 0) return;
   const int rows = f.gated ? 2 * f.n_out : f.n_out;
-  check_operand(f.x, f.ldx, f.n_in, "dense: x is null", "dense: x must start on 16 bytes, its row pitch must be a multiple of 8 elements");
-  check_operand(f.w, f.ldw, f.n_in, "dense: w is null", "dense: w must start on 16 bytes, its row pitch must be a multiple of 8 elements");
-  check_result(f.y, f.ldy, f.n_out);
+  check_matrix(f.x, f.ldx, f.n_in);
+  check_matrix(f.w, f.ldw, f.n_in);
+  check_matrix(f.y, f.ldy, f.n_out);
   expects(f.bias == nullptr || even(f.bias), "dense: odd bias pointer");
-  if (f.residual) check_result(f.residual, f.ldr, f.n_out);
-  if (f.preact) check_result(f.preact, f.ldp, rows);
+  if (f.residual) check_matrix(f.residual, f.ldr, f.n_out);
+  if (f.preact) check_preact(f.preact, f.ldp, rows);
+  const uint16_t *x = f.x, *w = f.w;
+  int64_t ldx = f.ldx, ldw = f.ldw;
+  bring_operands(x, ldx, f.T, w, ldw, rows, f.n_in, f.workspace, f.workspace_bytes, stream);
   DenseGemm g{};
   g.type = f.type;
-  g.a = {f.x, f.ldx, false};
-  g.b = {f.w, f.ldw, false};
+  g.a = {x, ldx, false};
+  g.b = {w, ldw, false};
   g.M = f.T;
   g.N = f.n_out;
   g.K = f.n_in;
@@ -76,50 +111,52 @@ void dense_forward(const DenseForward& f, cudaStream_t stream) {
   launch_dense_gemm(g, stream);
 }
 
-// Workspace of the backward pass: the gradient of the pre-activations at a pitch that a tensor map takes, then the chunks'
-// column sums.
-size_t dense_backward_workspace_bytes(int T, int n_out, bool gated) {
-  expects(T >= 0 && n_out > 0, "dense: T must not be negative, n_out must be positive");
+size_t dense_backward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int n_out, bool gated) {
+  expects(T >= 0 && n_in > 0 && n_out > 0, "dense: T must not be negative, feature counts must be positive");
   const size_t rows = (gated ? 2 : 1) * (size_t)n_out;
-  return round_up((size_t)T * round_up(rows, 8) * 2, 256) + (size_t)dense_sum_chunks(T) * rows * 4;
+  return copy_bytes(x, ldx, T, n_in) + copy_bytes(w, ldw, (int)rows, n_in) + round_up((size_t)T * round_up(rows, 8) * 2, 256) +
+         (size_t)dense_sum_chunks(T) * rows * 4;
 }
 
 void dense_backward(const DenseBackward& f, cudaStream_t stream) {
   check_common(f.type, f.T, f.n_in, f.n_out, f.gated, f.act, f.limit, f.beta);
   const int rows = f.gated ? 2 * f.n_out : f.n_out;
-  if (f.dw) check_result(f.dw, f.lddw, f.n_in);
+  if (f.dw) check_matrix(f.dw, f.lddw, f.n_in);
+  expects(f.db == nullptr || even(f.db), "dense: odd bias gradient pointer");
   if (f.T == 0) {   // no token: nothing flows back, and the sums over tokens are zero
     if (f.dw) VK_CUDA_CHECK(cudaMemset2DAsync(f.dw, (size_t)f.lddw * 2, 0, (size_t)f.n_in * 2, (size_t)rows, stream));
     if (f.db) VK_CUDA_CHECK(cudaMemsetAsync(f.db, 0, (size_t)rows * 2, stream));
     return;
   }
+  const bool products = f.dx || f.dw;
+  if (!products && !f.db) return;
   const bool has_act = f.gated || f.act != kActNone;
-  check_result(f.dy, f.lddy, f.n_out);
+  check_matrix(f.dy, f.lddy, f.n_out);
   if (has_act) {
     expects(f.preact != nullptr, "dense backward: the pre-activations of the forward pass are needed");
-    check_result(f.preact, f.ldp, rows);
+    check_preact(f.preact, f.ldp, rows);
   }
   if (f.dx) {
-    check_operand(f.w, f.ldw, f.n_in, "dense: w is null", "dense: w must start on 16 bytes, its row pitch must be a multiple of 8 elements");
-    check_result(f.dx, f.lddx, f.n_in);
+    check_matrix(f.w, f.ldw, f.n_in);
+    check_matrix(f.dx, f.lddx, f.n_in);
   }
-  if (f.dw)
-    check_operand(f.x, f.ldx, f.n_in, "dense: x is null", "dense: x must start on 16 bytes, its row pitch must be a multiple of 8 elements");
-  expects(f.db == nullptr || even(f.db), "dense: odd bias gradient pointer");
+  if (f.dw) check_matrix(f.x, f.ldx, f.n_in);
   // dy itself is the operand where there is no activation and a tensor map takes it
-  const bool products = f.dx || f.dw;
   const bool need_dz = products && (has_act || !tma_ready(f.dy, f.lddy));
-  if (!products && !f.db) return;
-  const int64_t ldz = (int64_t)round_up(rows, 8);
-  uint16_t* dz = nullptr;
-  float* partial = nullptr;
+  const uint16_t *x = f.dw ? f.x : nullptr, *w = f.dx ? f.w : nullptr;
+  int64_t ldx = f.ldx, ldw = f.ldw;
+  const int64_t ldz = (int64_t)round_up((size_t)rows, 8);
+  const size_t dz_bytes = need_dz ? round_up((size_t)f.T * ldz * 2, 256) : 0;
+  const size_t sums_bytes = f.db ? (size_t)dense_sum_chunks(f.T) * rows * 4 : 0;
+  const size_t copies = copy_bytes(x, ldx, f.T, f.n_in) + copy_bytes(w, ldw, rows, f.n_in);
+  if (copies + dz_bytes + sums_bytes > 0) {
+    expects(f.workspace != nullptr && (reinterpret_cast<uintptr_t>(f.workspace) & 15u) == 0, "dense: workspace must start on 16 bytes");
+    expects(f.workspace_bytes >= copies + dz_bytes + sums_bytes, "dense: workspace smaller than vk_cuda_dense_backward_workspace_bytes");
+  }
+  bring_operands(x, ldx, f.T, w, ldw, rows, f.n_in, f.workspace, f.workspace_bytes, stream);
+  uint16_t* dz = need_dz ? reinterpret_cast<uint16_t*>(static_cast<char*>(f.workspace) + copies) : nullptr;
   if (need_dz || f.db) {
-    expects(f.workspace != nullptr && (reinterpret_cast<uintptr_t>(f.workspace) & 15u) == 0, "dense backward: workspace must start on 16 bytes");
-    expects(f.workspace_bytes >= dense_backward_workspace_bytes(f.T, f.n_out, f.gated),
-            "dense backward: workspace smaller than vk_cuda_dense_backward_workspace_bytes");
-    char* base = static_cast<char*>(f.workspace);
-    if (need_dz) dz = reinterpret_cast<uint16_t*>(base);
-    if (f.db) partial = reinterpret_cast<float*>(base + round_up((size_t)f.T * ldz * 2, 256));
+    float* partial = f.db ? reinterpret_cast<float*>(static_cast<char*>(f.workspace) + copies + dz_bytes) : nullptr;
     DenseGrad g{};
     g.type = f.type;
     g.dy = f.dy;
@@ -146,7 +183,7 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
   g.limit = INFINITY;
   if (f.dx) {   // dx[t, i] = sum_n dz[t, n] w[n, i]
     g.a = {z, ldzz, false};
-    g.b = {f.w, f.ldw, true};
+    g.b = {w, ldw, true};
     g.M = f.T;
     g.N = f.n_in;
     g.K = rows;
@@ -156,7 +193,7 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
   }
   if (f.dw) {   // dw[n, i] = sum_t dz[t, n] x[t, i]
     g.a = {z, ldzz, true};
-    g.b = {f.x, f.ldx, true};
+    g.b = {x, ldx, true};
     g.M = rows;
     g.N = f.n_in;
     g.K = f.T;

@@ -22,8 +22,7 @@ struct DenseOperand {
 };
 
 // out[m, n] = act(sum_k A[m, k] B[n, k] + bias[n]) + residual[m, n], or the gated form: B has 2 N rows (gate rows, then up
-// rows), bias 2 N entries, out[m, n] = gate(z[m, n]) * up(z[m, N + n]). preact (optional) receives z, [M, N] or [M, 2 N],
-// rounded to the type without changing side of the clamp's limit.
+// rows), bias 2 N entries, out[m, n] = gate(z[m, n]) * up(z[m, N + n]). preact (optional) receives z in fp32, [M, N] or [M, 2 N].
 struct DenseGemm {
   DenseType type;
   DenseOperand a, b;
@@ -36,7 +35,7 @@ struct DenseGemm {
   int64_t ldr;
   uint16_t* out;
   int64_t ldo;
-  uint16_t* preact;           // or null
+  float* preact;              // or null
   int64_t ldp;
 };
 
@@ -47,7 +46,7 @@ struct DenseGrad {
   DenseType type;
   const uint16_t* dy;
   int64_t lddy;
-  const uint16_t* preact;     // null: no activation
+  const float* preact;        // null: no activation
   int64_t ldp;
   uint16_t* dz;
   int64_t ldz;
@@ -61,28 +60,35 @@ struct DenseGrad {
 int dense_sum_chunks(int T);
 void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_wide(const DenseGemm& g, cudaStream_t stream);   // dense_gemm.cu
+void launch_dense_narrow(const DenseGemm& g, cudaStream_t stream);  // dense_narrow.cu
+float dense_wide_us(const DenseGemm& g);      // the time that either is expected to take
+float dense_narrow_us(const DenseGemm& g);
 void launch_dense_simt(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_grad(const DenseGrad& g, cudaStream_t stream);
 // db[n] = sum over the chunks of partial[chunk, n], in order.
 void launch_dense_sum(DenseType type, const float* partial, int chunks, int cols, uint16_t* db, cudaStream_t stream);
-// dst[r, c] = src[r, c] at another pitch.
-void launch_dense_copy_rows(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t ldd, int rows, int cols, cudaStream_t stream);
+// dst[i][r, c] = src[i][r, c] for up to two matrices (dst[i] not null), rows of dst one after the other, each on 16 bytes.
+void launch_dense_copy_rows(const uint16_t* const* src, const int64_t* lds, uint16_t* const* dst, const int* rows, int cols, cudaStream_t stream);
 
 // ---- the operators ----
 struct DenseForward {
   DenseType type;
   const uint16_t *x, *w, *bias, *residual;
   int64_t ldx, ldw, ldr;
-  uint16_t *y, *preact;
+  uint16_t* y;
+  float* preact;
   int64_t ldy, ldp;
   int T, n_in, n_out;
   bool gated;
   int act;
   float limit, beta, linear_beta;
+  void* workspace;
+  size_t workspace_bytes;
 };
 struct DenseBackward {
   DenseType type;
-  const uint16_t *dy, *x, *w, *preact;
+  const uint16_t *dy, *x, *w;
+  const float* preact;
   int64_t lddy, ldx, ldw, ldp;
   uint16_t *dx, *dw, *db;     // each may be null
   int64_t lddx, lddw;
@@ -95,6 +101,9 @@ struct DenseBackward {
 };
 void dense_forward(const DenseForward& f, cudaStream_t stream);
 void dense_backward(const DenseBackward& f, cudaStream_t stream);
-size_t dense_backward_workspace_bytes(int T, int n_out, bool gated);
+// Workspace: copies of x and w where a tensor map does not take them as they are; of the backward pass also the gradient of the
+// pre-activations and the chunks' column sums.
+size_t dense_forward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int w_rows);
+size_t dense_backward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int n_out, bool gated);
 
 }  // namespace vkernels::kernels::cuda

@@ -11,21 +11,15 @@
 // (staged by its peer): an epilogue thread finds a feature's gate and up sums 128 columns apart in its own lane.
 #include <atomic>
 
-#include "dense.hpp"
-#include "dense_math.cuh"
-#include "sm100.cuh"
+#include "dense_tc.cuh"
 
 namespace vkernels::kernels::cuda {
-
-CUtensorMap sm100_make_map_bf16(const void* ptr, uint64_t inner, uint64_t outer, uint64_t pitch_bytes, uint32_t box_outer);
-int* sm100_status_address();
 
 namespace {
 
 constexpr int kStages = 6, kStageBytes = 32768;        // 128 rows of A and of B, 64 k each
 constexpr int kEpiWarps = 8, kThreads = 32 * (kEpiWarps + 2);
 constexpr int kStagingBytes = 4096;                    // of one epilogue warp: 32 rows x 64 values
-constexpr int kBn = 256;
 constexpr int kGroupM = 8;
 
 struct WideBars {
@@ -39,13 +33,15 @@ constexpr int kWideSmem = kStages * kStageBytes + kEpiWarps * kStagingBytes + (i
 struct WideParams {
   int M, N, K;                // N: columns of the result (gated: features)
   int a_mn, b_mn;
+  int bn;                     // rows of B a tile: 64, 128, 192 or 256
+  int stage_bytes;            // of one CTA: what the copies of a stage bring
   int tiles_m, tiles_n, n_tiles, k_blocks;
   int act;
   float limit, beta, linear_beta;
   const uint16_t* bias;
   const uint16_t* residual;
   uint16_t* out;
-  uint16_t* preact;
+  float* preact;
   int64_t ldr, ldo, ldp;
   int vec_r, vec_o, vec_p, vec_p2;   // 16-byte accesses possible (vec_p2: the up half of preact)
   int* status;
@@ -68,18 +64,6 @@ __device__ __forceinline__ void tc_mma_ss_pair(uint32_t d_tmem, uint64_t a_desc,
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Descriptor of a staged operand. Contiguous along k: rows of 64 k, groups of 8 rows 1024 bytes apart. Contiguous along the
-// other index: chunks of 64 indexes x 64 k, 8192 bytes apart, groups of 8 k 1024 bytes apart. 128-byte swizzle either way.
-__device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr, int mn_major) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)(mn_major ? 8192 >> 4 : 1) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
-
 // The staging buffer of a warp holds 32 rows x 64 values, eight units of 16 bytes a row, unit u of row r at u ^ (r % 8): a
 // thread that owns a row writes its units, eight threads at a time move a row to or from memory, both without bank conflicts.
 __device__ __forceinline__ uint32_t staging_at(uint32_t base, int row, int unit) { return base + row * 128 + ((unit ^ (row & 7)) << 4); }
@@ -91,42 +75,171 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
-// rows x cols (at most 32 x 64) of a row-major matrix, from and to the staging buffer.
-__device__ __forceinline__ void staging_out(uint32_t base, uint16_t* p, int64_t ld, int rows, int cols, int vec, int lane) {
+// rows x cols (at most 32 x 64) of a row-major matrix: a lane holds unit lane % 8 of rows lane / 8, 4 + lane / 8, ... The
+// common case - whole units on 16 bytes - is straight code, all eight accesses in flight at once (with a test at each the
+// loads wait for one another: 10 us instead of 2 for the last tile of a launch with a residual).
+struct Piece {
+  uint4 v[8];
+};
+__device__ __forceinline__ void piece_load(Piece& d, const uint16_t* p, int64_t ld, int rows, int cols, int vec, int lane) {
+  const int r0 = lane >> 3, u = lane & 7;
+  const uint16_t* q = p + (int64_t)r0 * ld + u * 8;
+  if (vec && (cols & 7) == 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      d.v[i] = i * 4 + r0 < rows && u * 8 < cols ? *reinterpret_cast<const uint4*>(q + (int64_t)(i * 4) * ld) : make_uint4(0, 0, 0, 0);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 3), u = lane & 7;
-    if (r >= rows) continue;
-    const uint4 v = lds128(staging_at(base, r, u));
-    uint16_t* q = p + (int64_t)r * ld + u * 8;
-    if (vec && u * 8 + 8 <= cols) {
-      *reinterpret_cast<uint4*>(q) = v;
-    } else {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (i * 4 + r0 < rows) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (u * 8 + j < cols) q[j] = (uint16_t)(w[j >> 1] >> ((j & 1) * 16));
+        if (u * 8 + j < cols) w[j >> 1] |= (uint32_t)q[(int64_t)(i * 4) * ld + j] << ((j & 1) * 16);
+    }
+    d.v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+__device__ __forceinline__ void piece_to_staging(const Piece& d, uint32_t base, int lane) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sts128(staging_at(base, i * 4 + (lane >> 3), lane & 7), d.v[i]);
+}
+__device__ __forceinline__ void staging_out(uint32_t base, uint16_t* p, int64_t ld, int rows, int cols, int vec, int lane) {
+  const int r0 = lane >> 3, u = lane & 7;
+  uint16_t* q = p + (int64_t)r0 * ld + u * 8;
+  if (vec && (cols & 7) == 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 v = lds128(staging_at(base, i * 4 + r0, u));
+      if (i * 4 + r0 < rows && u * 8 < cols) *reinterpret_cast<uint4*>(q + (int64_t)(i * 4) * ld) = v;
+    }
+    return;
+  }
+  // rows that start anywhere: a row at a time, a value a lane
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    uint16_t* row = p + (int64_t)r * ld;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = h * 32 + lane;
+      uint16_t v;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(staging_at(base, r, c >> 3) + (c & 7) * 2) : "memory");
+      if (c < cols) row[c] = v;
     }
   }
 }
-__device__ __forceinline__ void staging_in(uint32_t base, const uint16_t* p, int64_t ld, int rows, int cols, int vec, int lane) {
+
+// The epilogue's arithmetic: 64 columns of this thread's row, 16 at a time, into its row of the staging buffer. Rolled loops on
+// purpose, and one activation to a copy of the code: unrolled over the columns with the choice of activation inside, the last
+// tile of a launch waited 7 us for instructions instead of working 2.
+template <int TYPE>
+__device__ __forceinline__ void load_bias(float (&b)[2], const uint16_t* p, int cols, int lane) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 3), u = lane & 7;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < rows) {
-      const uint16_t* q = p + (int64_t)r * ld + u * 8;
-      if (vec && u * 8 + 8 <= cols) {
-        v = *reinterpret_cast<const uint4*>(q);
+  for (int i = 0; i < 2; ++i) b[i] = i * 32 + lane < cols ? dense_to_f32<TYPE>(p[i * 32 + lane]) : 0.0f;
+}
+__device__ __forceinline__ void add_bias(float (&z)[16], const float (&b)[2], int block) {
+  const float mine = block < 2 ? b[0] : b[1];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) z[j] += __shfl_sync(0xFFFFFFFFu, mine, (block & 1) * 16 + j);
+}
+__device__ __forceinline__ void load_columns(float (&z)[16], uint32_t taddr) {
+  uint32_t v[16];
+  tc_ld16(taddr, v);
+  tc_wait_ld();
+#pragma unroll
+  for (int j = 0; j < 16; ++j) z[j] = __uint_as_float(v[j]);
+}
+// The 64 pre-activations of this thread's row to memory in fp32, 32 at a time through the staging buffer.
+__device__ __forceinline__ void preact_columns(uint32_t tz, uint32_t staging, const float (&bias)[2], bool has_bias, float* p, int64_t ld,
+                                               int rows, int cols, int vec, int lane) {
+  const int r0 = lane >> 3, u = lane & 7;
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {
+#pragma unroll 1
+    for (int block = 0; block < 2; ++block) {
+      float z[16];
+      load_columns(z, tz + part * 32 + block * 16);
+      if (has_bias) add_bias(z, bias, part * 2 + block);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        sts128(staging_at(staging, lane, block * 4 + j), make_uint4(__float_as_uint(z[j * 4]), __float_as_uint(z[j * 4 + 1]),
+                                                                    __float_as_uint(z[j * 4 + 2]), __float_as_uint(z[j * 4 + 3])));
+    }
+    __syncwarp();
+    float* q = p + r0 * ld + part * 32 + u * 4;
+    const int left = cols - part * 32 - u * 4;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 v = lds128(staging_at(staging, i * 4 + r0, u));
+      if (i * 4 + r0 >= rows) continue;
+      float* at = q + (int64_t)(i * 4) * ld;
+      if (vec && left >= 4) {
+        *reinterpret_cast<uint4*>(at) = v;
       } else {
-        uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (u * 8 + j < cols) w[j >> 1] |= (uint32_t)q[j] << ((j & 1) * 16);
-        v = make_uint4(w[0], w[1], w[2], w[3]);
+        if (left > 0) at[0] = __uint_as_float(v.x);
+        if (left > 1) at[1] = __uint_as_float(v.y);
+        if (left > 2) at[2] = __uint_as_float(v.z);
+        if (left > 3) at[3] = __uint_as_float(v.w);
       }
     }
-    sts128(staging_at(base, r, u), v);
+    __syncwarp();
+  }
+}
+template <int TYPE, int ACT>
+__device__ __forceinline__ void linear_columns(uint32_t tz, uint32_t staging, const float (&bias)[2], bool has_bias, bool residual, int lane) {
+#pragma unroll 1
+  for (int block = 0; block < 4; ++block) {
+    float z[16];
+    load_columns(z, tz + block * 16);
+    if (has_bias) add_bias(z, bias, block);
+    if (ACT != kActNone) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) z[j] = dense_act(ACT, z[j]);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t at = staging_at(staging, lane, block * 2 + u);
+      if (residual) {
+        const uint4 q = lds128(at);
+        const uint32_t r[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 v = dense_unpack<TYPE>(r[j]);
+          z[u * 8 + j * 2] += v.x;
+          z[u * 8 + j * 2 + 1] += v.y;
+        }
+      }
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = dense_pack<TYPE>(z[u * 8 + j * 2], z[u * 8 + j * 2 + 1]);
+      sts128(at, make_uint4(w[0], w[1], w[2], w[3]));
+    }
+  }
+}
+template <int TYPE, int ACT>
+__device__ __forceinline__ void gated_columns(uint32_t tg, uint32_t tu, uint32_t staging, const float (&bias_g)[2], const float (&bias_u)[2],
+                                              bool has_bias, const WideParams& p, int lane) {
+#pragma unroll 1
+  for (int block = 0; block < 4; ++block) {
+    float g[16], u[16];
+    load_columns(g, tg + block * 16);
+    load_columns(u, tu + block * 16);
+    if (has_bias) {
+      add_bias(g, bias_g, block);
+      add_bias(u, bias_u, block);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = h * 8 + j * 2;
+        w[j] = dense_pack<TYPE>(dense_gated(ACT, g[c], u[c], p.limit, p.beta, p.linear_beta),
+                                dense_gated(ACT, g[c + 1], u[c + 1], p.limit, p.beta, p.linear_beta));
+      }
+      sts128(staging_at(staging, lane, block * 2 + h), make_uint4(w[0], w[1], w[2], w[3]));
+    }
   }
 }
 
@@ -163,6 +276,7 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   cluster_sync_all();   // the peer's barriers exist before anything arrives on them
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
+  wait_for_earlier_kernels();
   const int unit = blockIdx.x >> 1, n_units = gridDim.x >> 1;
   const int per_group = kGroupM * p.tiles_n;
   const auto place = [&](int t, int& tm, int& tn) {
@@ -181,14 +295,14 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         int tm, tn;
         place(t, tm, tn);
         const int m0 = tm * 256 + (int)rank * 128;
-        const int n0 = GATED ? tn * 128 + (int)rank * p.N : tn * kBn + (int)rank * 128;
+        const int n0 = GATED ? tn * (p.bn / 2) + (int)rank * p.N : tn * p.bn + (int)rank * (p.bn / 2);
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           const uint32_t full = smem_u32(&bars->full[s.slot]), dst = ring + s.slot * kStageBytes;
           if (!mbar_wait(smem_u32(&bars->empty[s.slot]), s.phase ^ 1u, abort_flag, 51)) {
             go = false;
             break;
           }
-          if (rank == 0) mbar_expect_tx(full, 2 * kStageBytes);
+          if (rank == 0) mbar_expect_tx(full, 2 * p.stage_bytes);
           if (p.a_mn) {
             tma_load_2d_pair(dst, &map_a, m0, kb * 64, full);
             tma_load_2d_pair(dst + 8192, &map_a, m0 + 64, kb * 64, full);
@@ -197,7 +311,7 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           }
           if (p.b_mn) {
             tma_load_2d_pair(dst + 16384, &map_b, n0, kb * 64, full);
-            tma_load_2d_pair(dst + 24576, &map_b, n0 + 64, kb * 64, full);
+            if (p.bn > 128) tma_load_2d_pair(dst + 24576, &map_b, n0 + 64, kb * 64, full);
           } else {
             tma_load_2d_pair(dst + 16384, &map_b, kb * 64, n0, full);
           }
@@ -216,8 +330,7 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   } else if (warp == kEpiWarps + 1) {
     // -------------------------------- MMAs ----------------------------------
     if (rank == 0 && elect_one()) {
-      const uint32_t idesc = (1u << 4) | (TYPE == kDenseBf16 ? (1u << 7) | (1u << 10) : 0u) | (p.a_mn ? 1u << 15 : 0u) |
-                             (p.b_mn ? 1u << 16 : 0u) | ((uint32_t)(kBn >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+      const uint32_t idesc = operand_idesc<TYPE>(256, p.bn, p.a_mn, p.b_mn);
       const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;   // 16 k on
       Ring s;
       int it = 0;
@@ -253,177 +366,84 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       int tm, tn;
       place(t, tm, tn);
       const int buf = it & 1;
+      const int64_t row0 = (int64_t)tm * 256 + rank * 128 + quad * 32;
+      const int rows = (int)min((int64_t)32, (int64_t)p.M - row0);
+      Piece ahead;   // the residual of the coming 64 columns, on its way while the MMAs run
+      // 64 columns at a time: the even ones of a tile's chunks are the first four warps', the odd ones the others'
+      const int chunks = ((GATED ? p.bn / 2 : p.bn) + 63) / 64, tile_col = tn * (GATED ? p.bn / 2 : p.bn);
+      if (!GATED && p.residual && rows > 0 && half < chunks && tile_col + half * 64 < p.N)
+        piece_load(ahead, p.residual + row0 * p.ldr + tile_col + half * 64, p.ldr, rows, min(64, p.N - tile_col - half * 64), p.vec_r, lane);
       const bool ready = mbar_wait(smem_u32(&bars->acc_full[buf]), (it >> 1) & 1, abort_flag, 54, 32);
       if (!__all_sync(0xFFFFFFFFu, ready)) break;
       tc_fence_after();
       const uint32_t lanes = tmem_base + buf * 256 + ((uint32_t)(quad * 32) << 16);
-      const int64_t row0 = (int64_t)tm * 256 + rank * 128 + quad * 32;
-      const int rows = (int)min((int64_t)32, (int64_t)p.M - row0);
       if constexpr (GATED) {
-        // 64 features of this warp: gate sums at columns half * 64, up sums 128 on
-        const int col0 = tn * 128 + half * 64, cols = min(64, p.N - col0);
-        const uint32_t tg = lanes + half * 64, tu = tg + 128;
+        // up to 64 features of this warp: gate sums at columns half * 64, up sums half a tile on
+        const int col0 = tile_col + half * 64, cols = min(min(64, p.bn / 2 - half * 64), p.N - col0);
+        const uint32_t tg = lanes + half * 64, tu = tg + p.bn / 2;
+        const bool any = rows > 0 && cols > 0;
+        const bool has_bias = p.bias != nullptr && any;
         float bias_g[2] = {}, bias_u[2] = {};
-        if (p.bias) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (i * 32 + lane < cols) {
-              bias_g[i] = dense_to_f32<TYPE>(p.bias[col0 + i * 32 + lane]);
-              bias_u[i] = dense_to_f32<TYPE>(p.bias[p.N + col0 + i * 32 + lane]);
-            }
+        if (has_bias) {
+          load_bias<TYPE>(bias_g, p.bias + col0, cols, lane);
+          load_bias<TYPE>(bias_u, p.bias + p.N + col0, cols, lane);
         }
-        if (p.preact && rows > 0 && cols > 0) {
-#pragma unroll
+        if (p.preact && any) {
+#pragma unroll 1
           for (int part = 0; part < 2; ++part) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t v[32];
-              tc_ld32((part ? tu : tg) + i * 32, v);
-              tc_wait_ld();
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const int c = u * 8 + j * 2;
-                  float z0 = __uint_as_float(v[c]), z1 = __uint_as_float(v[c + 1]);
-                  if (p.bias) {
-                    z0 += __shfl_sync(0xFFFFFFFFu, part ? bias_u[i] : bias_g[i], c);
-                    z1 += __shfl_sync(0xFFFFFFFFu, part ? bias_u[i] : bias_g[i], c + 1);
-                  }
-                  w[j] = dense_round_preact<TYPE>(z0, p.limit) | ((uint32_t)dense_round_preact<TYPE>(z1, p.limit) << 16);
-                }
-                sts128(staging_at(staging, lane, i * 4 + u), make_uint4(w[0], w[1], w[2], w[3]));
-              }
-            }
-            __syncwarp();
-            staging_out(staging, p.preact + row0 * p.ldp + (part ? p.N : 0) + col0, p.ldp, rows, cols, part ? p.vec_p2 : p.vec_p, lane);
-            __syncwarp();
+            const float b[2] = {part ? bias_u[0] : bias_g[0], part ? bias_u[1] : bias_g[1]};
+            preact_columns(part ? tu : tg, staging, b, has_bias, p.preact + row0 * p.ldp + (part ? p.N : 0) + col0, p.ldp, rows, cols,
+                           part ? p.vec_p2 : p.vec_p, lane);
           }
         }
-        if (rows > 0 && cols > 0) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t g[32], uu[32];
-            tc_ld32(tg + i * 32, g);
-            tc_ld32(tu + i * 32, uu);
-            tc_wait_ld();
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              uint32_t w[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                float h[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int c = u * 8 + j * 2 + e;
-                  float zg = __uint_as_float(g[c]), zu = __uint_as_float(uu[c]);
-                  if (p.bias) {
-                    zg += __shfl_sync(0xFFFFFFFFu, bias_g[i], c);
-                    zu += __shfl_sync(0xFFFFFFFFu, bias_u[i], c);
-                  }
-                  h[e] = dense_gated(p.act, zg, zu, p.limit, p.beta, p.linear_beta);
-                }
-                w[j] = dense_pack<TYPE>(h[0], h[1]);
-              }
-              sts128(staging_at(staging, lane, i * 4 + u), make_uint4(w[0], w[1], w[2], w[3]));
-            }
-          }
+        if (any) {
+          if (p.act == 1) gated_columns<TYPE, 1>(tg, tu, staging, bias_g, bias_u, has_bias, p, lane);
+          else gated_columns<TYPE, 0>(tg, tu, staging, bias_g, bias_u, has_bias, p, lane);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cta(smem_u32(&bars->acc_empty[buf]), 0);
-        if (rows > 0 && cols > 0) {
+        if (any) {
           staging_out(staging, p.out + row0 * p.ldo + col0, p.ldo, rows, cols, p.vec_o, lane);
           __syncwarp();
         }
       } else {
 #pragma unroll 1
-        for (int chunk = 0; chunk < 2; ++chunk) {
-          const int col0 = tn * kBn + half * 128 + chunk * 64, cols = min(64, p.N - col0);
-          const uint32_t tz = lanes + half * 128 + chunk * 64;
+        for (int chunk = half; chunk < chunks; chunk += 2) {
+          const int col0 = tile_col + chunk * 64, cols = min(64, p.N - col0);
+          const uint32_t tz = lanes + chunk * 64;
           const bool any = rows > 0 && cols > 0;
+          const bool has_bias = p.bias != nullptr && any;
           float bias[2] = {};
-          if (p.bias && any) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (i * 32 + lane < cols) bias[i] = dense_to_f32<TYPE>(p.bias[col0 + i * 32 + lane]);
-          }
+          if (has_bias) load_bias<TYPE>(bias, p.bias + col0, cols, lane);
           if (p.preact && any) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t v[32];
-              tc_ld32(tz + i * 32, v);
-              tc_wait_ld();
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const int c = u * 8 + j * 2;
-                  float z0 = __uint_as_float(v[c]), z1 = __uint_as_float(v[c + 1]);
-                  if (p.bias) {
-                    z0 += __shfl_sync(0xFFFFFFFFu, bias[i], c);
-                    z1 += __shfl_sync(0xFFFFFFFFu, bias[i], c + 1);
-                  }
-                  w[j] = dense_round_preact<TYPE>(z0, p.limit) | ((uint32_t)dense_round_preact<TYPE>(z1, p.limit) << 16);
-                }
-                sts128(staging_at(staging, lane, i * 4 + u), make_uint4(w[0], w[1], w[2], w[3]));
-              }
-            }
-            __syncwarp();
-            staging_out(staging, p.preact + row0 * p.ldp + col0, p.ldp, rows, cols, p.vec_p, lane);
-            __syncwarp();
+            preact_columns(tz, staging, bias, has_bias, p.preact + row0 * p.ldp + col0, p.ldp, rows, cols, p.vec_p, lane);
           }
           if (p.residual && any) {
-            staging_in(staging, p.residual + row0 * p.ldr + col0, p.ldr, rows, cols, p.vec_r, lane);
+            piece_to_staging(ahead, staging, lane);
             __syncwarp();
+            if (chunk + 2 < chunks && col0 + 128 < p.N)
+              piece_load(ahead, p.residual + row0 * p.ldr + col0 + 128, p.ldr, rows, min(64, p.N - col0 - 128), p.vec_r, lane);
           }
           if (any) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t v[32];
-              tc_ld32(tz + i * 32, v);
-              tc_wait_ld();
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                const uint32_t at = staging_at(staging, lane, i * 4 + u);
-                uint32_t r[4] = {0, 0, 0, 0}, w[4];
-                if (p.residual) {
-                  const uint4 q = lds128(at);
-                  r[0] = q.x, r[1] = q.y, r[2] = q.z, r[3] = q.w;
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const int c = u * 8 + j * 2;
-                  float z0 = __uint_as_float(v[c]), z1 = __uint_as_float(v[c + 1]);
-                  if (p.bias) {
-                    z0 += __shfl_sync(0xFFFFFFFFu, bias[i], c);
-                    z1 += __shfl_sync(0xFFFFFFFFu, bias[i], c + 1);
-                  }
-                  if (p.act != kActNone) {
-                    z0 = dense_act(p.act, z0);
-                    z1 = dense_act(p.act, z1);
-                  }
-                  if (p.residual) {
-                    const float2 q = dense_unpack<TYPE>(r[j]);
-                    z0 += q.x;
-                    z1 += q.y;
-                  }
-                  w[j] = dense_pack<TYPE>(z0, z1);
-                }
-                sts128(at, make_uint4(w[0], w[1], w[2], w[3]));
-              }
+            const bool res = p.residual != nullptr;
+            switch (p.act) {
+              case kActSilu: linear_columns<TYPE, kActSilu>(tz, staging, bias, has_bias, res, lane); break;
+              case kActGelu: linear_columns<TYPE, kActGelu>(tz, staging, bias, has_bias, res, lane); break;
+              case kActGeluTanh: linear_columns<TYPE, kActGeluTanh>(tz, staging, bias, has_bias, res, lane); break;
+              default: linear_columns<TYPE, kActNone>(tz, staging, bias, has_bias, res, lane);
             }
           }
-          if (chunk == 1) tc_fence_before();
+          const bool last = chunk + 2 >= chunks;
+          if (last) tc_fence_before();
           __syncwarp();
-          if (chunk == 1 && lane == 0) mbar_arrive_cta(smem_u32(&bars->acc_empty[buf]), 0);
+          if (last && lane == 0) mbar_arrive_cta(smem_u32(&bars->acc_empty[buf]), 0);
           if (any) {
             staging_out(staging, p.out + row0 * p.ldo + col0, p.ldo, rows, cols, p.vec_o, lane);
             __syncwarp();
           }
         }
+        if (half >= chunks && lane == 0) mbar_arrive_cta(smem_u32(&bars->acc_empty[buf]), 0);   // nothing here for this warp
       }
     }
   }
@@ -439,22 +459,35 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   if (tid == 0 && bars->abort_flag != 0) atomicExch(p.status, 100 + bars->abort_flag);
 }
 
-bool aligned16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
-
-int* status_address() {
-  static std::atomic<int*> known[64];
-  int dev = 0;
-  VK_CUDA_CHECK(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64) return sm100_status_address();
-  int* p = known[dev].load();
-  if (p == nullptr) known[dev].store(p = sm100_status_address());
-  return p;
+// A tensor map of one operand: boxes of 64 values along the contiguous index by `box` (k contiguous) or 64 rows.
+CUtensorMap operand_map(const DenseOperand& o, int64_t rows, int K, int box) {
+  return o.mn_major ? sm100_make_map_bf16(o.p, (uint64_t)rows, (uint64_t)K, (uint64_t)o.ld * 2, 64)
+                    : sm100_make_map_bf16(o.p, (uint64_t)K, (uint64_t)rows, (uint64_t)o.ld * 2, (uint32_t)box);
 }
 
-// A tensor map of one operand: boxes of 64 values along the contiguous index by 128 (k contiguous) or 64 rows.
-CUtensorMap operand_map(const DenseOperand& o, int64_t rows, int K) {
-  return o.mn_major ? sm100_make_map_bf16(o.p, (uint64_t)rows, (uint64_t)K, (uint64_t)o.ld * 2, 64)
-                    : sm100_make_map_bf16(o.p, (uint64_t)K, (uint64_t)rows, (uint64_t)o.ld * 2, 128);
+// How a launch is cut, and how long it takes by that (us): the width of a tile that makes waves x time of a wave smallest. A
+// tile's time is its k blocks' (0.28, 0.216, 0.152 and 0.148 us each for 256, 192, 128 and 64 rows of B: below 192 a stage is
+// bound by bringing A) and what comes before and after them. Measured on 2880 -> 2880: 512 tokens 20.1, 17.6, 13.4 and 19.1 us,
+// 1024 tokens 22.3, 18.4, 21.2 and 27.0, 2047 tokens 35.2, 29.3, 30.4 and 43.3; with many waves the widest is best or within
+// 4 % of it (8192 tokens 101.5, 97.9, 108.5, 161.1; 8192 x 7168 -> 2048 170, 175, 193, 296).
+struct WidePlan {
+  int bn;
+  float us;
+};
+WidePlan plan_wide(int64_t M, int64_t N, int64_t K, bool gated) {
+  constexpr int kWidths[4] = {256, 192, 128, 64};
+  constexpr float kBlockUs[4] = {0.28f, 0.216f, 0.152f, 0.148f}, kEndsUs[4] = {7.2f, 6.3f, 5.3f, 5.4f};
+  const int64_t pairs = sm_count() / 2, tiles_m = (M + 255) / 256, blocks = (K + 63) / 64;
+  WidePlan best{256, 1e30f};
+  for (int i = 0; i < 4; ++i) {
+    const int64_t tile_n = gated ? kWidths[i] / 2 : kWidths[i], tiles = tiles_m * ((N + tile_n - 1) / tile_n);
+    const float waves = (float)((tiles + pairs - 1) / pairs);
+    // the more pairs are at work, the slower the narrower tiles, which bring more bytes for a product
+    const float load = waves > 1.0f || i == 0 ? 1.0f + 0.06f * i : 1.0f + 0.06f * i * (float)tiles / (float)pairs;
+    const float us = kEndsUs[i] + waves * ((float)blocks * kBlockUs[i] * load) + (waves - 1.0f) * 1.0f;
+    if (us < best.us) best = {kWidths[i], us};
+  }
+  return best;
 }
 
 template <int TYPE, bool GATED>
@@ -472,7 +505,9 @@ void launch_wide(const DenseGemm& g, cudaStream_t stream) {
   p.K = g.K;
   p.a_mn = g.a.mn_major;
   p.b_mn = g.b.mn_major;
-  const int tile_n = GATED ? 128 : kBn;
+  p.bn = plan_wide(g.M, g.N, g.K, GATED).bn;
+  p.stage_bytes = 16384 + (g.b.mn_major ? (p.bn > 128 ? 16384 : 8192) : p.bn * 64);
+  const int tile_n = GATED ? p.bn / 2 : p.bn;
   p.tiles_m = (g.M + 255) / 256;
   p.tiles_n = (g.N + tile_n - 1) / tile_n;
   expects((int64_t)p.tiles_m * p.tiles_n < (1ll << 30), "dense product: more than 2^30 tiles");
@@ -491,16 +526,26 @@ void launch_wide(const DenseGemm& g, cudaStream_t stream) {
   p.ldp = g.ldp;
   p.vec_r = g.residual != nullptr && aligned16(g.residual, g.ldr);
   p.vec_o = aligned16(g.out, g.ldo);
-  p.vec_p = g.preact != nullptr && aligned16(g.preact, g.ldp);
-  p.vec_p2 = p.vec_p && g.N % 8 == 0;
+  p.vec_p = (reinterpret_cast<uintptr_t>(g.preact) & 15u) == 0 && g.ldp % 4 == 0;
+  p.vec_p2 = p.vec_p && g.N % 4 == 0;
   p.status = status_address();
-  const CUtensorMap a = operand_map(g.a, g.M, g.K), b = operand_map(g.b, GATED ? 2 * (int64_t)g.N : g.N, g.K);
+  const CUtensorMap a = operand_map(g.a, g.M, g.K, 128), b = operand_map(g.b, GATED ? 2 * (int64_t)g.N : g.N, g.K, p.bn / 2);
   const int units = min(p.n_tiles, sm_count() / 2);
-  dense_wide_kernel<TYPE, GATED><<<2 * units, kThreads, kWideSmem, stream>>>(a, b, p);
-  VK_CUDA_CHECK(cudaGetLastError());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(2 * units));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kWideSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  overlap_launch(attr[0]);
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  VK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, dense_wide_kernel<TYPE, GATED>, a, b, p));
 }
 
 }  // namespace
+
+float dense_wide_us(const DenseGemm& g) { return plan_wide(g.M, g.N, g.K, g.gated).us; }
 
 void launch_dense_wide(const DenseGemm& g, cudaStream_t stream) {
   if (g.type == kDenseBf16) {

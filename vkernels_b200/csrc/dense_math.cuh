@@ -32,22 +32,6 @@ __device__ __forceinline__ float2 dense_unpack(uint32_t v) {
   return make_float2(dense_to_f32<TYPE>((uint16_t)(v & 0xFFFFu)), dense_to_f32<TYPE>((uint16_t)(v >> 16)));
 }
 
-// A pre-activation kept for the backward pass: the nearest 16-bit value on the same side of the clamp's limit, so that the
-// slope of a clamped input is 0 exactly where the forward pass clamped it (limit = inf: no clamp). A finite value beyond
-// fp16's range becomes the largest finite one: the slopes there are those of the limit, where inf would give inf - inf.
-template <int TYPE>
-__device__ __forceinline__ uint16_t dense_round_preact(float v, float limit) {
-  uint16_t r = dense_from_f32<TYPE>(v);
-  if (TYPE == kDenseFp16 && (r & 0x7FFFu) == 0x7C00u && fabsf(v) <= 3.402823466e38f) r -= 1;
-  const float m = fabsf(dense_to_f32<TYPE>(r));
-  if (fabsf(v) > limit) {
-    if (!(m > limit)) r += 1;
-  } else if (m > limit) {
-    r -= 1;
-  }
-  return r;
-}
-
 // 1 / (1 + exp(-v)) by the hardware's exp2 and reciprocal (relative error about 1e-6, a bf16 half step is 4e-3, an fp16 one
 // 5e-4); 1 at +inf, 0 at -inf, NaN stays.
 __device__ __forceinline__ float dense_sigmoid(float v) {
@@ -57,7 +41,25 @@ __device__ __forceinline__ float dense_sigmoid(float v) {
   return r;
 }
 
-constexpr float kSqrtHalf = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f;
+// tanh: beyond 1/4 through the same two instructions, 1 - 2 / (1 + exp(2 y)); below, where that would lose digits, by its
+// Taylor series to y^9 (the first term left out is 9e-9 of the value at 1/4).
+__device__ __forceinline__ float dense_tanh(float y) {
+  const float q = y * y;
+  const float near = y * (1.0f + q * (-0.33333333f + q * (0.13333333f + q * (-0.053968254f + q * 0.021869489f))));
+  const float far = 1.0f - 2.0f * dense_sigmoid(-2.0f * y);
+  return fabsf(y) < 0.25f ? near : far;
+}
+// The normal distribution up to z and e = exp(-z^2 / 2): erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x)
+// (Abramowitz and Stegun 7.1.26, off by at most 1.5e-7), x = |z| / sqrt(2); nothing cancels on either side of 0.
+__device__ __forceinline__ float dense_normal_cdf(float z, float& e) {
+  float t;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * z * -0.72134752f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.0f)));
+  const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  return z < 0.0f ? q : 1.0f - q;
+}
+
+constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 // 0.5 (1 + tanh(y)) = sigmoid(2 y), y = sqrt(2 / pi) (z + 0.044715 z^3)
 constexpr float kGeluC = 1.5957691216057308f, kGeluA = 0.044715f;
 
@@ -65,7 +67,10 @@ constexpr float kGeluC = 1.5957691216057308f, kGeluA = 0.044715f;
 __device__ __forceinline__ float dense_act(int act, float z) {
   switch (act) {
     case kActSilu: return z * dense_sigmoid(z);
-    case kActGelu: return 0.5f * z * (1.0f + erff(z * kSqrtHalf));
+    case kActGelu: {
+      float e;
+      return z * dense_normal_cdf(z, e);
+    }
     case kActGeluTanh: return z * dense_sigmoid(kGeluC * (z + kGeluA * z * z * z));
     default: return z;
   }
@@ -77,7 +82,11 @@ __device__ __forceinline__ float dense_act_slope(int act, float z) {
       const float p = dense_sigmoid(z);
       return p + z * p * (1.0f - p);
     }
-    case kActGelu: return 0.5f * (1.0f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * __expf(-0.5f * z * z);
+    case kActGelu: {
+      float e;
+      const float cdf = dense_normal_cdf(z, e);
+      return cdf + z * kInvSqrt2Pi * e;
+    }
     case kActGeluTanh: {
       const float p = dense_sigmoid(kGeluC * (z + kGeluA * z * z * z));
       return p + z * p * (1.0f - p) * kGeluC * (1.0f + 3.0f * kGeluA * fminf(z * z, 1e8f));
@@ -89,8 +98,8 @@ __device__ __forceinline__ float dense_act_slope(int act, float z) {
 // The gated product of one feature; `limit` = inf for no clamp. min.NaN / max.NaN: a NaN stays NaN.
 __device__ __forceinline__ float dense_gated(int act, float g, float u, float limit, float beta, float linear_beta) {
   if (act == 1) {
-    const float up = linear_beta > 0.0f ? linear_beta * tanhf(u / linear_beta) : u;
-    return beta * tanhf(g / beta) * dense_sigmoid(g) * up;
+    const float up = linear_beta > 0.0f ? linear_beta * dense_tanh(u / linear_beta) : u;
+    return beta * dense_tanh(g / beta) * dense_sigmoid(g) * up;
   }
   float lo = -limit;
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(g) : "f"(limit));
@@ -102,8 +111,8 @@ __device__ __forceinline__ float dense_gated(int act, float g, float u, float li
 __device__ __forceinline__ void dense_gated_grad(int act, float dh, float g, float u, float limit, float beta, float linear_beta,
                                                  float& dg, float& du) {
   if (act == 1) {
-    const float p = dense_sigmoid(g), a = tanhf(g / beta);
-    const float b = linear_beta > 0.0f ? tanhf(u / linear_beta) : 0.0f;
+    const float p = dense_sigmoid(g), a = dense_tanh(g / beta);
+    const float b = linear_beta > 0.0f ? dense_tanh(u / linear_beta) : 0.0f;
     const float up = linear_beta > 0.0f ? linear_beta * b : u;
     dg = dh * up * ((1.0f - a * a) * p + beta * a * p * (1.0f - p));
     du = dh * (beta * a * p) * (1.0f - b * b);

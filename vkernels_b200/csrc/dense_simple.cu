@@ -65,8 +65,8 @@ __global__ void __launch_bounds__(256) dense_simt_kernel(DenseGemm g) {
           zu += dense_to_f32<TYPE>(g.bias[g.N + n]);
         }
         if (g.preact) {
-          g.preact[(int64_t)m * g.ldp + n] = dense_round_preact<TYPE>(zg, g.limit);
-          g.preact[(int64_t)m * g.ldp + g.N + n] = dense_round_preact<TYPE>(zu, g.limit);
+          g.preact[(int64_t)m * g.ldp + n] = zg;
+          g.preact[(int64_t)m * g.ldp + g.N + n] = zu;
         }
         g.out[(int64_t)m * g.ldo + n] = dense_from_f32<TYPE>(dense_gated(g.act, zg, zu, g.limit, g.beta, g.linear_beta));
       }
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(256) dense_simt_kernel(DenseGemm g) {
         const int n = n0 + tx * 4 + j;
         if (n >= g.N) continue;
         float z = acc[i][j] + (g.bias ? dense_to_f32<TYPE>(g.bias[n]) : 0.0f);
-        if (g.preact) g.preact[(int64_t)m * g.ldp + n] = dense_round_preact<TYPE>(z, g.limit);
+        if (g.preact) g.preact[(int64_t)m * g.ldp + n] = z;
         z = dense_act(g.act, z);
         if (g.residual) z += dense_to_f32<TYPE>(g.residual[(int64_t)m * g.ldr + n]);
         g.out[(int64_t)m * g.ldo + n] = dense_from_f32<TYPE>(z);
@@ -109,6 +109,16 @@ __device__ __forceinline__ void store_eight(uint16_t* p, const Eight& e, int n, 
   }
 }
 
+__device__ __forceinline__ void load_eight_f32(float (&v)[8], const float* p, int n, bool vec) {
+  if (vec && n >= 8) {
+    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
+    *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(p + 4);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : 0.0f;
+  }
+}
+
 constexpr int kGradCols = 256, kGradThreads = 256;   // 32 threads across the columns, eight each; 8 rows at a time
 
 // dz = dy * act'(z) and the column sums of a chunk of rows, in one pass: one CTA per 256 columns of dy and chunk. A column's
@@ -125,14 +135,14 @@ __global__ void __launch_bounds__(kGradThreads) dense_grad_kernel(DenseGrad g, i
     for (int r = blockIdx.y * rows_per_chunk + sub; r < r_end; r += 8) {
       const Eight dy = load_eight(g.dy + (int64_t)r * g.lddy + c0, left, vec);
       if constexpr (GATED) {
-        const Eight zg = load_eight(g.preact + (int64_t)r * g.ldp + c0, left, vec);
-        const Eight zu = load_eight(g.preact + (int64_t)r * g.ldp + g.N + c0, left, vec);
+        float zg[8], zu[8];
+        load_eight_f32(zg, g.preact + (int64_t)r * g.ldp + c0, left, vec);
+        load_eight_f32(zu, g.preact + (int64_t)r * g.ldp + g.N + c0, left, vec);
         Eight og, ou;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float dg, du;
-          dense_gated_grad(g.act, dense_to_f32<TYPE>(dy.v[j]), dense_to_f32<TYPE>(zg.v[j]), dense_to_f32<TYPE>(zu.v[j]), g.limit,
-                           g.beta, g.linear_beta, dg, du);
+          dense_gated_grad(g.act, dense_to_f32<TYPE>(dy.v[j]), zg[j], zu[j], g.limit, g.beta, g.linear_beta, dg, du);
           sg[j] += dg;
           su[j] += du;
           og.v[j] = dense_from_f32<TYPE>(dg);
@@ -143,12 +153,13 @@ __global__ void __launch_bounds__(kGradThreads) dense_grad_kernel(DenseGrad g, i
           store_eight(g.dz + (int64_t)r * g.ldz + g.N + c0, ou, left, vec);
         }
       } else {
-        Eight z = dy, o;
-        if (g.preact) z = load_eight(g.preact + (int64_t)r * g.ldp + c0, left, vec);
+        Eight o;
+        float z[8];
+        if (g.preact) load_eight_f32(z, g.preact + (int64_t)r * g.ldp + c0, left, vec);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float d = dense_to_f32<TYPE>(dy.v[j]);
-          if (g.preact) d *= dense_act_slope(g.act, dense_to_f32<TYPE>(z.v[j]));
+          if (g.preact) d *= dense_act_slope(g.act, z[j]);
           sg[j] += d;
           o.v[j] = dense_from_f32<TYPE>(d);
         }
@@ -184,17 +195,25 @@ __global__ void __launch_bounds__(128) dense_sum_kernel(const float* __restrict_
   db[c] = dense_from_f32<TYPE>(s);
 }
 
-__global__ void __launch_bounds__(256) dense_copy_rows_kernel(const uint16_t* __restrict__ src, int64_t lds, uint16_t* __restrict__ dst,
-                                                              int64_t ldd, int rows, int cols) {
-  for (int r = blockIdx.y; r < rows; r += gridDim.y)
-    for (int c = blockIdx.x * 256 + threadIdx.x; c < cols; c += gridDim.x * 256) dst[(int64_t)r * ldd + c] = src[(int64_t)r * lds + c];
+// dst[r, c] = src[r, c] for two matrices at once (grid z), rows of dst on 16 bytes, filled up with zeros to whole units of 8.
+struct RowCopies {
+  const uint16_t* src[2];
+  uint16_t* dst[2];
+  int64_t lds[2];
+  int rows[2];
+};
+__global__ void __launch_bounds__(256) dense_copy_rows_kernel(RowCopies c, int cols) {
+  const int z = blockIdx.z, units = (cols + 7) / 8;
+  for (int r = blockIdx.y; r < c.rows[z]; r += gridDim.y)
+    for (int u = blockIdx.x * 256 + threadIdx.x; u < units; u += gridDim.x * 256)
+      store_eight(c.dst[z] + ((int64_t)r * units + u) * 8, load_eight(c.src[z] + r * c.lds[z] + u * 8, cols - u * 8, false), 8, true);
 }
 
 bool aligned16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
 
 template <int TYPE>
 void grad_of_type(const DenseGrad& g, int chunks, cudaStream_t stream) {
-  bool vec = aligned16(g.dy, g.lddy) && (g.preact == nullptr || aligned16(g.preact, g.ldp)) && (g.dz == nullptr || aligned16(g.dz, g.ldz));
+  bool vec = aligned16(g.dy, g.lddy) && (g.preact == nullptr || ((reinterpret_cast<uintptr_t>(g.preact) & 15u) == 0 && g.ldp % 4 == 0)) && (g.dz == nullptr || aligned16(g.dz, g.ldz));
   if (g.gated) vec = vec && g.N % 8 == 0;
   const dim3 grid((g.N + kGradCols - 1) / kGradCols, chunks);
   const int rows = (g.T + chunks - 1) / chunks;
@@ -236,10 +255,18 @@ void launch_dense_sum(DenseType type, const float* partial, int chunks, int cols
   VK_CUDA_CHECK(cudaGetLastError());
 }
 
-void launch_dense_copy_rows(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t ldd, int rows, int cols, cudaStream_t stream) {
-  if (rows <= 0 || cols <= 0) return;
-  const dim3 grid((cols + 255) / 256 < 16 ? (cols + 255) / 256 : 16, rows < 16384 ? rows : 16384);
-  dense_copy_rows_kernel<<<grid, 256, 0, stream>>>(src, lds, dst, ldd, rows, cols);
+void launch_dense_copy_rows(const uint16_t* const* src, const int64_t* lds, uint16_t* const* dst, const int* rows, int cols, cudaStream_t stream) {
+  RowCopies c{};
+  int n = 0, most = 0;
+  for (int i = 0; i < 2; ++i)
+    if (dst[i] != nullptr) {
+      c.src[n] = src[i], c.lds[n] = lds[i], c.dst[n] = dst[i], c.rows[n] = rows[i];
+      most = rows[i] > most ? rows[i] : most;
+      ++n;
+    }
+  if (n == 0) return;
+  const int wide = (cols + 2047) / 2048;
+  dense_copy_rows_kernel<<<dim3(wide < 8 ? wide : 8, most < 16384 ? most : 16384, n), 256, 0, stream>>>(c, cols);
   VK_CUDA_CHECK(cudaGetLastError());
 }
 

@@ -90,14 +90,14 @@ _SIGNATURES = {
                                      [c_int, c_float, c_int, c_float, c_float, c_void_p, c_void_p,
                                       c_int, c_void_p]),
     "vk_cuda_gated_linear": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64] +
-                             [c_int] * 5 + [c_float] * 3 + [c_void_p]),
+                             [c_int] * 5 + [c_float] * 3 + [c_void_p, c_size_t, c_void_p]),
     "vk_cuda_fused_linear": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p] + [c_void_p, c_int64] * 3 + [c_int] * 5 +
-                             [c_void_p]),
-    "vk_cuda_dense_backward_workspace_bytes": (c_size_t, [c_int] * 3),
+                             [c_void_p, c_size_t, c_void_p]),
+    "vk_cuda_dense_forward_workspace_bytes": (c_size_t, [c_void_p, c_int64] * 2 + [c_int] * 3),
+    "vk_cuda_dense_backward_workspace_bytes": (c_size_t, [c_void_p, c_int64] * 2 + [c_int] * 4),
     "vk_cuda_gated_linear_backward": (c_int, [c_void_p, c_int64] * 6 + [c_void_p] + [c_int] * 5 + [c_float] * 3 +
                                       [c_void_p, c_size_t, c_void_p]),
     "vk_cuda_fused_linear_backward": (c_int, [c_void_p, c_int64] * 6 + [c_void_p] + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
-    "vk_cuda_dense_copy_rows": (c_int, [c_void_p, c_int64] * 2 + [c_int] * 2 + [c_void_p]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

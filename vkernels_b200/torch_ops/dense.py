@@ -6,11 +6,12 @@ always-on expert that the checkpoint keeps in bf16 or fp16), forward and backwar
 ``fused_linear``  a projection with bias, activation and residual in its epilogue
 
 Tensors are bf16 or fp16, one type per call, on one GPU; sums are fp32 and rounded once. Rows may have any pitch, the values of a
-row must be neighbours. An operand whose rows do not start on 16 bytes is first copied to rows that do. Calls run on the current
-stream, allocate through torch only, and may be captured.
+row must be neighbours; x and weights whose rows do not start on 16 bytes are copied to rows that do, within the call. Calls run
+on the current stream, allocate through torch only, and may be captured.
 
 Called with gradients enabled and an input that requires one, the two operators record themselves for ``backward()``; that
-form cannot be captured into a CUDA graph (capture ``*_backward`` instead, which record nothing).
+form cannot be captured into a CUDA graph (capture the forward call with ``return_preact=True`` and ``*_backward`` instead, which
+record nothing).
 """
 from __future__ import annotations
 
@@ -24,22 +25,41 @@ from .moe_fused_mxfp4 import SITU, SWIGLU
 
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1}
 _LINEAR_ACT = {None: 0, "none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
+# what the kernels index
+_MOST_TOKENS, _MOST_ROWS, _MOST_IN = 2 ** 30, 2 ** 30, 2 ** 30
+
+_entries = {}
 
 
-def _call(name, device, *args):
-    """The C entry on the current stream of `device`, which becomes the current device for the call."""
-    fn = getattr(nr.load_library(), name)
-    index = device.index
+def _entry(name):
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(nr.load_library(), name)
+    return fn
+
+
+# the handle alone: a Stream object around it costs a microsecond of a decode step's dozen
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(name, index, *args):
+    """The C entry on the current stream of device `index`, which becomes the current device for the call."""
     if index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        rc = _entry(name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+            rc = _entry(name)(*args, _raw_stream(index))
     if rc:
         nr.check(rc, name)
 
 
+def _plain(t, shape, dtype, index):
+    """Whether a tensor is just what the kernels read: contiguous, of this shape and type, on this device and on 16 bytes."""
+    return t.shape == shape and t.dtype is dtype and t.get_device() == index and t.is_contiguous() and not t.data_ptr() & 15
+
+
 def _check(name, t, dtype, device):
+    require(isinstance(t, torch.Tensor), f"{name} must be a tensor")
     require(t.dtype == dtype, f"{name} must be {dtype}, like the other tensors of the call, got {t.dtype}")
     require(t.device == device, f"{name} must be on {device}, got {t.device}")
 
@@ -52,18 +72,6 @@ def _pitch(name, t):
         return (n + 7) // 8 * 8
     require(t.stride(0) >= n, f"the rows of {name} must not overlap")
     return t.stride(0)
-
-
-def _operand(name, t):
-    """(tensor to keep, pointer, pitch) of a matrix that the products read: rows on 16 bytes, copied there if they are not."""
-    ld = _pitch(name, t)
-    p = t.data_ptr()
-    if (p & 15) == 0 and (ld & 7) == 0:
-        return t, p, ld
-    T, n = t.shape
-    wide = torch.empty((T, (n + 7) // 8 * 8), dtype=t.dtype, device=t.device)
-    _call("vk_cuda_dense_copy_rows", t.device, p, ld, wide.data_ptr(), wide.shape[1], T, n)
-    return wide, wide.data_ptr(), wide.shape[1]
 
 
 def _span(t):
@@ -93,15 +101,16 @@ def _rows2d(name, t, cols):
         require(False, f"{name} must be viewable as rows of {cols}")
 
 
-def _inputs(x, w, rows, what):
+def _inputs(x, w, gated, what):
     require(isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor), f"{what}: tensors expected")
     require(x.dtype in _DTYPE, f"x must be bfloat16 or float16, got {x.dtype}")
     _check("the weight", w, x.dtype, x.device)
     require(x.dim() >= 1 and w.dim() == 2 and w.shape[1] == x.shape[-1], f"{what}: x [..., n_in] and a weight [rows, n_in] expected")
     require(w.shape[1] > 0 and w.shape[0] > 0, f"{what}: feature counts must be positive")
-    require(rows != 2 or w.shape[0] % 2 == 0, "w13 must hold gate rows followed by up rows: an even row count")
+    require(not gated or w.shape[0] % 2 == 0, "w13 must hold gate rows followed by up rows: an even row count")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    require(x2.shape[0] < 2 ** 30 and w.shape[0] < 2 ** 30 and w.shape[1] <= 2 ** 30, f"{what}: more rows or features than the kernels index")
+    require(x2.shape[0] < _MOST_TOKENS and w.shape[0] < _MOST_ROWS and w.shape[1] <= _MOST_IN,
+            f"{what}: more rows or features than the kernels index")
     return x2
 
 
@@ -114,7 +123,11 @@ def _bias(bias, rows, x):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _no_capture():
@@ -146,6 +159,15 @@ def _result(out, out2, shape, x):
     return out, out2
 
 
+def _forward_work(x, ldx, w, ldw, T, n_in, rows):
+    """(tensor to keep, pointer, bytes) of the room for copies of x and w, where their alignment calls for them."""
+    if not (x.data_ptr() & 15 or w.data_ptr() & 15 or ldx & 7 or ldw & 7):
+        return None, None, 0
+    nbytes = _entry("vk_cuda_dense_forward_workspace_bytes")(x.data_ptr(), ldx, w.data_ptr(), ldw, T, n_in, rows)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    return work, work.data_ptr(), nbytes
+
+
 # ---------------------------------------------------------------------------
 # gated projection
 # ---------------------------------------------------------------------------
@@ -161,29 +183,45 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, b13: torch.Tensor | None = 
                  return_preact: bool = False):
     """``h [..., ispp] = act(x Wg^T + bg) * (x Wu^T + bu)`` for x ``[..., hidden]`` and w13 ``[2 * ispp, hidden]`` (gate rows, then
     up rows; b13 ``[2 * ispp]`` likewise). SwiGLU: gate * sigmoid(gate) * up, the gate clamped from above and up from both sides
-    at `swiglu_limit` if that is positive; SiTU: beta tanh(gate / beta) sigmoid(gate) * linear_beta tanh(up / linear_beta).
+    at `swiglu_limit` if that is positive; SiTU: beta tanh(gate / beta) sigmoid(gate) * linear_beta tanh(up / linear_beta) (up
+    itself if linear_beta is not positive).
 
-    ``return_preact``: also return what ``gated_linear_backward`` needs, the pre-activations ``[T, 2 * ispp]`` in the type of x
-    (T: all leading dimensions of x together)."""
-    x2 = _inputs(x, w13, 2, "gated_linear")
+    ``return_preact``: also return what ``gated_linear_backward`` needs, the pre-activations in fp32, ``[T, 2 * ispp]`` (T: all
+    leading dimensions of x together)."""
+    if out is None and type(x) is torch.Tensor and isinstance(w13, torch.Tensor):
+        # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
+        shape, index, dtype, wshape = x.shape, x.get_device(), x.dtype, w13.shape
+        if (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and wshape[1] == shape[1] > 0
+                and not shape[1] & 7 and 0 < wshape[0] < _MOST_ROWS and not wshape[0] & 1 and 0 < shape[0] < _MOST_TOKENS
+                and (activation == SWIGLU or activation == SITU and beta > 0) and swiglu_limit >= 0
+                and _plain(x, shape, dtype, index) and _plain(w13, wshape, dtype, index)
+                and (b13 is None or _plain(b13, wshape[:1], dtype, index)) and not _wants_grad(x, w13, b13)):
+            T, rows = shape[0], wshape[0]
+            h = x.new_empty((T, rows // 2))
+            preact = x.new_empty((T, rows), dtype=torch.float32) if return_preact else None
+            _call("vk_cuda_gated_linear", index, x.data_ptr(), shape[1], w13.data_ptr(), shape[1], None if b13 is None else b13.data_ptr(),
+                  h.data_ptr(), rows // 2, None if preact is None else preact.data_ptr(), rows, _DTYPE[dtype], T, shape[1], rows // 2,
+                  activation, swiglu_limit, beta, linear_beta, None, 0)
+            return (h, preact) if return_preact else h
+    x2 = _inputs(x, w13, True, "gated_linear")
     _gated_kind(activation, swiglu_limit, beta)
     rows, ispp = w13.shape[0], w13.shape[0] // 2
     b = _bias(b13, rows, x)
     T, hidden = x2.shape
     shape = (*x.shape[:-1], ispp)
+    ldx, ldw = _pitch("x", x2), _pitch("w13", w13)
     out2 = None if out is None else _given_out(out, shape, x, (("x", x), ("w13", w13), ("b13", b13)))
     _resident(x)
     if _wants_grad(x, w13, b13, out):
         require(out is None and not return_preact, "gated_linear: out and return_preact are for calls that record no gradient")
         return _GatedLinear.apply(x, w13, b13, activation, swiglu_limit, beta, linear_beta)
     h, h2 = _result(out, out2, shape, x)
-    preact = torch.empty((T, rows), dtype=x.dtype, device=x.device) if return_preact else None
+    preact = torch.empty((T, rows), dtype=torch.float32, device=x.device) if return_preact else None
     if T > 0:
-        xk, xp, ldx = _operand("x", x2)
-        wk, wp, ldw = _operand("w13", w13)
-        _call("vk_cuda_gated_linear", x.device, xp, ldx, wp, ldw, b, h2.data_ptr(), _pitch("out", h2),
+        work, wp, nbytes = _forward_work(x2, ldx, w13, ldw, T, hidden, rows)
+        _call("vk_cuda_gated_linear", x.get_device(), x2.data_ptr(), ldx, w13.data_ptr(), ldw, b, h2.data_ptr(), _pitch("out", h2),
               None if preact is None else preact.data_ptr(), rows, _DTYPE[x.dtype], T, hidden, ispp, activation, swiglu_limit, beta,
-              linear_beta)
+              linear_beta, wp, nbytes)
     return (h, preact) if return_preact else h
 
 
@@ -192,11 +230,9 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w13: torch.Tensor, 
                           x_grad: bool = True, w_grad: bool = True):
     """``(dx, dw13, db13)`` for the gradient dh of ``gated_linear``'s result; ``preact`` as that call returned it, the other
     arguments as it was given. What is not asked for is None."""
-    x2 = _inputs(x, w13, 2, "gated_linear_backward")
     _gated_kind(activation, swiglu_limit, beta)
-    ispp = w13.shape[0] // 2
     require(preact is not None, "gated_linear_backward needs the forward call's pre-activations")
-    return _backward("vk_cuda_gated_linear_backward", dh, x, x2, w13, preact, ispp, True, bias_grad, x_grad, w_grad,
+    return _backward("vk_cuda_gated_linear_backward", dh, x, w13, preact, True, bias_grad, x_grad, w_grad,
                      (activation, swiglu_limit, beta, linear_beta))
 
 
@@ -215,13 +251,30 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     """``y [..., n_out] = act(x w^T + bias) + residual`` for x ``[..., n_in]``, w ``[n_out, n_in]``; activation None, "silu",
     "gelu" (erf) or "gelu_tanh"; residual of y's shape (not broadcast). ``out`` may be the residual itself.
 
-    ``return_preact``: also return what ``fused_linear_backward`` needs: the pre-activations ``[T, n_out]``, or None where there
-    is no activation."""
-    x2 = _inputs(x, w, 1, "fused_linear")
+    ``return_preact``: also return what ``fused_linear_backward`` needs: the pre-activations in fp32, ``[T, n_out]``, or None
+    where there is no activation."""
     act = _linear_kind(activation)
+    if out is None and type(x) is torch.Tensor and isinstance(w, torch.Tensor):
+        # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
+        shape, index, dtype, wshape = x.shape, x.get_device(), x.dtype, w.shape
+        if (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and wshape[1] == shape[1] > 0
+                and not shape[1] & 7 and 0 < wshape[0] < _MOST_ROWS and 0 < shape[0] < _MOST_TOKENS
+                and _plain(x, shape, dtype, index) and _plain(w, wshape, dtype, index)
+                and (bias is None or _plain(bias, wshape[:1], dtype, index))
+                and (residual is None or _plain(residual, (shape[0], wshape[0]), dtype, index))
+                and not _wants_grad(x, w, bias, residual)):
+            T, n_in, n_out = shape[0], shape[1], wshape[0]
+            y = x.new_empty((T, n_out))
+            preact = x.new_empty((T, n_out), dtype=torch.float32) if return_preact and act else None
+            _call("vk_cuda_fused_linear", index, x.data_ptr(), n_in, w.data_ptr(), n_in, None if bias is None else bias.data_ptr(),
+                  None if residual is None else residual.data_ptr(), n_out, y.data_ptr(), n_out,
+                  None if preact is None else preact.data_ptr(), n_out, _DTYPE[dtype], T, n_in, n_out, act, None, 0)
+            return (y, preact) if return_preact else y
+    x2 = _inputs(x, w, False, "fused_linear")
     n_out = w.shape[0]
     b = _bias(bias, n_out, x)
     shape = (*x.shape[:-1], n_out)
+    ldx, ldw = _pitch("x", x2), _pitch("w", w)
     r2, ldr = None, 0
     if residual is not None:
         _check("the residual", residual, x.dtype, x.device)
@@ -238,12 +291,12 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
         return _FusedLinear.apply(x, w, bias, residual, activation)
     T, n_in = x2.shape
     y, y2 = _result(out, out2, shape, x)
-    preact = torch.empty((T, n_out), dtype=x.dtype, device=x.device) if return_preact and act else None
+    preact = torch.empty((T, n_out), dtype=torch.float32, device=x.device) if return_preact and act else None
     if T > 0:
-        xk, xp, ldx = _operand("x", x2)
-        wk, wp, ldw = _operand("w", w)
-        _call("vk_cuda_fused_linear", x.device, xp, ldx, wp, ldw, b, None if r2 is None else r2.data_ptr(), ldr, y2.data_ptr(), _pitch("out", y2),
-              None if preact is None else preact.data_ptr(), n_out, _DTYPE[x.dtype], T, n_in, n_out, act)
+        work, wp, nbytes = _forward_work(x2, ldx, w, ldw, T, n_in, n_out)
+        _call("vk_cuda_fused_linear", x.get_device(), x2.data_ptr(), ldx, w.data_ptr(), ldw, b, None if r2 is None else r2.data_ptr(), ldr,
+              y2.data_ptr(), _pitch("out", y2), None if preact is None else preact.data_ptr(), n_out, _DTYPE[x.dtype], T, n_in, n_out,
+              act, wp, nbytes)
     return (y, preact) if return_preact else y
 
 
@@ -251,34 +304,34 @@ def fused_linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pr
                           activation: str | None = None, bias_grad: bool = False, x_grad: bool = True, w_grad: bool = True):
     """``(dx, dw, dbias)`` for the gradient dy of ``fused_linear``'s result; ``preact`` as that call returned it (None without an
     activation). What is not asked for is None. The residual's gradient is dy."""
-    x2 = _inputs(x, w, 1, "fused_linear_backward")
     act = _linear_kind(activation)
     require(act == 0 or preact is not None, "fused_linear_backward needs the forward call's pre-activations")
-    return _backward("vk_cuda_fused_linear_backward", dy, x, x2, w, preact if act else None, w.shape[0], False, bias_grad, x_grad,
-                     w_grad, (act,))
+    return _backward("vk_cuda_fused_linear_backward", dy, x, w, preact if act else None, False, bias_grad, x_grad, w_grad, (act,))
 
 
-def _backward(entry, dy, x, x2, w, preact, n_out, gated, bias_grad, x_grad, w_grad, kind):
+def _backward(entry, dy, x, w, preact, gated, bias_grad, x_grad, w_grad, kind):
+    x2 = _inputs(x, w, gated, entry[8:])
     rows, (T, n_in) = w.shape[0], x2.shape
+    n_out = rows // 2 if gated else rows
     dtype, device = x.dtype, x.device
     _check("the result's gradient", dy, dtype, device)
     require(tuple(dy.shape) == (*x.shape[:-1], n_out), f"the result's gradient must be {(*x.shape[:-1], n_out)}, got {tuple(dy.shape)}")
     dy2 = dy if dy.dim() == 2 else dy.reshape(-1, n_out)
     if preact is not None:
-        _check("preact", preact, dtype, device)
+        _check("preact", preact, torch.float32, device)
         require(tuple(preact.shape) == (T, rows), f"preact must be {(T, rows)}, got {tuple(preact.shape)}")
-    ld_dy, ld_p = _pitch("the result's gradient", dy2), 0 if preact is None else _pitch("preact", preact)
+    ldx, ldw, ld_dy = _pitch("x", x2), _pitch("the weight", w), _pitch("the result's gradient", dy2)
+    ldp = 0 if preact is None else _pitch("preact", preact)
     _resident(x)
     dx = torch.empty(x.shape, dtype=dtype, device=device) if x_grad else None
     dw = torch.empty((rows, n_in), dtype=dtype, device=device) if w_grad else None
     db = torch.empty(rows, dtype=dtype, device=device) if bias_grad else None
     if dx is None and dw is None and db is None:
         return None, None, None
-    nbytes = nr.load_library().vk_cuda_dense_backward_workspace_bytes(T, n_out, int(gated))
+    xp, wp = x2.data_ptr(), w.data_ptr()
+    nbytes = _entry("vk_cuda_dense_backward_workspace_bytes")(xp, ldx, wp, ldw, T, n_in, n_out, gated)
     work = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    xk, xp, ldx = _operand("x", x2) if w_grad and T > 0 else (x2, None, 0)
-    wk, wp, ldw = _operand("the weight", w) if x_grad and T > 0 else (w, None, 0)
-    _call(entry, device, dy2.data_ptr(), ld_dy, xp, ldx, wp, ldw, None if preact is None else preact.data_ptr(), ld_p,
+    _call(entry, x.get_device(), dy2.data_ptr(), ld_dy, xp, ldx, wp, ldw, None if preact is None else preact.data_ptr(), ldp,
           None if dx is None else dx.data_ptr(), n_in, None if dw is None else dw.data_ptr(), n_in, None if db is None else db.data_ptr(),
           _DTYPE[dtype], T, n_in, n_out, *kind, work.data_ptr(), nbytes)
     return dx, dw, db
@@ -288,7 +341,7 @@ def _backward(entry, dy, x, x2, w, preact, n_out, gated, bias_grad, x_grad, w_gr
 # recording for backward()
 # ---------------------------------------------------------------------------
 
-def _plain_rows(t):
+def _neighbours(t):
     """A gradient as autograd hands it over (it may be an expanded number), with rows that the kernels take."""
     return t if t.stride(-1) == 1 and (t.dim() < 2 or t.stride(-2) >= t.shape[-1]) else t.contiguous()
 
@@ -298,8 +351,7 @@ class _GatedLinear(torch.autograd.Function):
     def forward(ctx, x, w13, b13, activation, swiglu_limit, beta, linear_beta):
         _no_capture()
         ctx.kw = dict(activation=activation, swiglu_limit=swiglu_limit, beta=beta, linear_beta=linear_beta)
-        with torch.no_grad():
-            h, preact = gated_linear(x, w13, b13, return_preact=True, **ctx.kw)
+        h, preact = gated_linear(x, w13, b13, return_preact=True, **ctx.kw)
         ctx.save_for_backward(x, w13, preact)
         return h
 
@@ -309,7 +361,7 @@ class _GatedLinear(torch.autograd.Function):
         _no_capture()
         x, w13, preact = ctx.saved_tensors
         nx, nw, nb = ctx.needs_input_grad[:3]
-        dx, dw, db = gated_linear_backward(_plain_rows(dh), x, w13, preact, x_grad=nx, w_grad=nw, bias_grad=nb, **ctx.kw)
+        dx, dw, db = gated_linear_backward(_neighbours(dh), x, w13, preact, x_grad=nx, w_grad=nw, bias_grad=nb, **ctx.kw)
         return dx, dw, db, None, None, None, None
 
 
@@ -318,8 +370,7 @@ class _FusedLinear(torch.autograd.Function):
     def forward(ctx, x, w, bias, residual, activation):
         _no_capture()
         ctx.activation = activation
-        with torch.no_grad():
-            y, preact = fused_linear(x, w, bias, activation=activation, residual=residual, return_preact=True)
+        y, preact = fused_linear(x, w, bias, activation=activation, residual=residual, return_preact=True)
         ctx.save_for_backward(x, w, preact)
         return y
 
@@ -328,7 +379,9 @@ class _FusedLinear(torch.autograd.Function):
     def backward(ctx, dy):
         _no_capture()
         x, w, preact = ctx.saved_tensors
-        nx, nw, nb, nr_, _ = ctx.needs_input_grad
-        dx, dw, db = fused_linear_backward(_plain_rows(dy), x, w, preact, activation=ctx.activation, x_grad=nx, w_grad=nw,
-                                           bias_grad=nb)
-        return dx, dw, db, dy if nr_ else None, None
+        nx, nw, nb, n_residual, _ = ctx.needs_input_grad
+        dx = dw = db = None
+        if nx or nw or nb:
+            dx, dw, db = fused_linear_backward(_neighbours(dy), x, w, preact, activation=ctx.activation, x_grad=nx, w_grad=nw,
+                                               bias_grad=nb)
+        return dx, dw, db, dy if n_residual else None, None
