@@ -180,3 +180,20 @@ def test_linear_slopes_against_differences(act):
         named = {"silu": torch.nn.functional.silu(z), "gelu": torch.nn.functional.gelu(z),
                  "gelu_tanh": torch.nn.functional.gelu(z, approximate="tanh")}[act]
         assert torch.allclose(value, named, rtol=1e-12, atol=1e-15)
+
+
+def test_feed_forward_checks_its_weights():
+    from vkernels_b200.dist import CudaBackend
+    from vkernels_b200.feedforward import DenseFeedForward
+
+    DenseFeedForward(t(32, 8), t(8, 16), b13=t(32), b2=t(8))
+    for bad in ((t(32, 8), t(8, 15)), (t(32, 8), t(9, 16)), (t(31, 8), t(8, 16)), (t(32, 8), t(8, 16, dtype=torch.float16))):
+        with pytest.raises(ops.OpNotEligible):
+            DenseFeedForward(*bad)
+    with pytest.raises(ops.OpNotEligible, match="b2"):
+        DenseFeedForward(t(32, 8), t(8, 16), b2=t(8, dtype=torch.float32))
+
+    class Layer:
+        shared_ffn = DenseFeedForward(t(32, 8), t(8, 16))
+    with pytest.raises(ValueError, match="routed experts only"):
+        CudaBackend(Layer(), "cpu")

@@ -115,7 +115,7 @@ size_t dense_backward_workspace_bytes(const void* x, int64_t ldx, const void* w,
   expects(T >= 0 && n_in > 0 && n_out > 0, "dense: T must not be negative, feature counts must be positive");
   const size_t rows = (gated ? 2 : 1) * (size_t)n_out;
   return copy_bytes(x, ldx, T, n_in) + copy_bytes(w, ldw, (int)rows, n_in) + round_up((size_t)T * round_up(rows, 8) * 2, 256) +
-         (size_t)dense_sum_chunks(T) * rows * 4;
+         (size_t)dense_sum_chunks(T, n_out) * rows * 4;
 }
 
 void dense_backward(const DenseBackward& f, cudaStream_t stream) {
@@ -147,7 +147,7 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
   int64_t ldx = f.ldx, ldw = f.ldw;
   const int64_t ldz = (int64_t)round_up((size_t)rows, 8);
   const size_t dz_bytes = need_dz ? round_up((size_t)f.T * ldz * 2, 256) : 0;
-  const size_t sums_bytes = f.db ? (size_t)dense_sum_chunks(f.T) * rows * 4 : 0;
+  const size_t sums_bytes = f.db ? (size_t)dense_sum_chunks(f.T, f.n_out) * rows * 4 : 0;
   const size_t copies = copy_bytes(x, ldx, f.T, f.n_in) + copy_bytes(w, ldw, rows, f.n_in);
   if (copies + dz_bytes + sums_bytes > 0) {
     expects(f.workspace != nullptr && (reinterpret_cast<uintptr_t>(f.workspace) & 15u) == 0, "dense: workspace must start on 16 bytes");
@@ -174,7 +174,7 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
     g.beta = f.beta;
     g.linear_beta = f.linear_beta;
     launch_dense_grad(g, stream);
-    if (f.db) launch_dense_sum(f.type, partial, dense_sum_chunks(f.T), rows, f.db, stream);
+    if (f.db) launch_dense_sum(f.type, partial, dense_sum_chunks(f.T, f.n_out), rows, f.db, stream);
   }
   const uint16_t* z = need_dz ? dz : f.dy;
   const int64_t ldzz = need_dz ? ldz : f.lddy;

@@ -41,7 +41,7 @@ struct DenseGemm {
 
 // Gradient of the pre-activations: dz = dy * act'(z), [T, rows] (linear) or [T, 2 ispp] (gated) at pitch ldz; with no
 // activation a copy of dy. dz may be null (only the column sums are wanted). partial (optional) receives the column sums of
-// each chunk of rows in fp32, [dense_sum_chunks(T), rows].
+// each chunk of rows in fp32, [dense_sum_chunks(T, N), rows].
 struct DenseGrad {
   DenseType type;
   const uint16_t* dy;
@@ -57,7 +57,7 @@ struct DenseGrad {
   float limit, beta, linear_beta;
 };
 
-int dense_sum_chunks(int T);
+int dense_sum_chunks(int T, int n_out);
 void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_wide(const DenseGemm& g, cudaStream_t stream);   // dense_gemm.cu
 void launch_dense_narrow(const DenseGemm& g, cudaStream_t stream);  // dense_narrow.cu

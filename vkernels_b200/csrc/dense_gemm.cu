@@ -75,35 +75,39 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void sts16(uint32_t addr, uint16_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory"); }
 // rows x cols (at most 32 x 64) of a row-major matrix: a lane holds unit lane % 8 of rows lane / 8, 4 + lane / 8, ... The
 // common case - whole units on 16 bytes - is straight code, all eight accesses in flight at once (with a test at each the
 // loads wait for one another: 10 us instead of 2 for the last tile of a launch with a residual).
 struct Piece {
   uint4 v[8];
 };
-__device__ __forceinline__ void piece_load(Piece& d, const uint16_t* p, int64_t ld, int rows, int cols, int vec, int lane) {
+__device__ __forceinline__ void piece_load(Piece& d, const uint16_t* p, int64_t ld, int rows, int cols, int lane) {
   const int r0 = lane >> 3, u = lane & 7;
   const uint16_t* q = p + (int64_t)r0 * ld + u * 8;
-  if (vec && (cols & 7) == 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      d.v[i] = i * 4 + r0 < rows && u * 8 < cols ? *reinterpret_cast<const uint4*>(q + (int64_t)(i * 4) * ld) : make_uint4(0, 0, 0, 0);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (i * 4 + r0 < rows) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (u * 8 + j < cols) w[j >> 1] |= (uint32_t)q[(int64_t)(i * 4) * ld + j] << ((j & 1) * 16);
-    }
-    d.v[i] = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+  for (int i = 0; i < 8; ++i)
+    d.v[i] = i * 4 + r0 < rows && u * 8 + 8 <= cols ? *reinterpret_cast<const uint4*>(q + (int64_t)(i * 4) * ld) : make_uint4(0, 0, 0, 0);
 }
-__device__ __forceinline__ void piece_to_staging(const Piece& d, uint32_t base, int lane) {
+// ... with the columns behind the last whole unit fetched one by one.
+__device__ __forceinline__ void piece_to_staging(const Piece& d, uint32_t base, const uint16_t* p, int64_t ld, int rows, int cols, int lane) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) sts128(staging_at(base, i * 4 + (lane >> 3), lane & 7), d.v[i]);
+  if ((cols & 7) == 0) return;
+  __syncwarp();
+  for (int c = cols & ~7; c < cols; ++c)
+    if (lane < rows) sts16(staging_at(base, lane, c >> 3) + (c & 7) * 2, p[(int64_t)lane * ld + c]);
+}
+// Rows that start anywhere: a row at a time, a value a lane.
+__device__ __forceinline__ void values_in(uint32_t base, const uint16_t* p, int64_t ld, int rows, int cols, int lane) {
+#pragma unroll 16
+  for (int r = 0; r < 32; ++r) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = h * 32 + lane;
+      sts16(staging_at(base, r, c >> 3) + (c & 7) * 2, r < rows && c < cols ? p[(int64_t)r * ld + c] : (uint16_t)0);
+    }
+  }
 }
 __device__ __forceinline__ void staging_out(uint32_t base, uint16_t* p, int64_t ld, int rows, int cols, int vec, int lane) {
   const int r0 = lane >> 3, u = lane & 7;
@@ -116,8 +120,7 @@ __device__ __forceinline__ void staging_out(uint32_t base, uint16_t* p, int64_t 
     }
     return;
   }
-  // rows that start anywhere: a row at a time, a value a lane
-#pragma unroll 4
+#pragma unroll 8
   for (int r = 0; r < rows; ++r) {
     uint16_t* row = p + (int64_t)r * ld;
 #pragma unroll
@@ -130,7 +133,7 @@ __device__ __forceinline__ void staging_out(uint32_t base, uint16_t* p, int64_t 
   }
 }
 
-// The epilogue's arithmetic: 64 columns of this thread's row, 16 at a time, into its row of the staging buffer. Rolled loops on
+// The epilogue's arithmetic: up to 64 columns of this thread's row, 16 at a time, into its row of the staging buffer. Rolled loops on
 // purpose, and one activation to a copy of the code: unrolled over the columns with the choice of activation inside, the last
 // tile of a launch waited 7 us for instructions instead of working 2.
 template <int TYPE>
@@ -151,13 +154,13 @@ __device__ __forceinline__ void load_columns(float (&z)[16], uint32_t taddr) {
   for (int j = 0; j < 16; ++j) z[j] = __uint_as_float(v[j]);
 }
 // The 64 pre-activations of this thread's row to memory in fp32, 32 at a time through the staging buffer.
-__device__ __forceinline__ void preact_columns(uint32_t tz, uint32_t staging, const float (&bias)[2], bool has_bias, float* p, int64_t ld,
+__device__ __forceinline__ void preact_columns(uint32_t tz, int width, uint32_t staging, const float (&bias)[2], bool has_bias, float* p, int64_t ld,
                                                int rows, int cols, int vec, int lane) {
   const int r0 = lane >> 3, u = lane & 7;
 #pragma unroll 1
-  for (int part = 0; part < 2; ++part) {
+  for (int part = 0; part * 32 < width; ++part) {
 #pragma unroll 1
-    for (int block = 0; block < 2; ++block) {
+    for (int block = 0; block < 2 && part * 32 + block * 16 < width; ++block) {
       float z[16];
       load_columns(z, tz + part * 32 + block * 16);
       if (has_bias) add_bias(z, bias, part * 2 + block);
@@ -187,9 +190,9 @@ __device__ __forceinline__ void preact_columns(uint32_t tz, uint32_t staging, co
   }
 }
 template <int TYPE, int ACT>
-__device__ __forceinline__ void linear_columns(uint32_t tz, uint32_t staging, const float (&bias)[2], bool has_bias, bool residual, int lane) {
+__device__ __forceinline__ void linear_columns(uint32_t tz, int width, uint32_t staging, const float (&bias)[2], bool has_bias, bool residual, int lane) {
 #pragma unroll 1
-  for (int block = 0; block < 4; ++block) {
+  for (int block = 0; block * 16 < width; ++block) {
     float z[16];
     load_columns(z, tz + block * 16);
     if (has_bias) add_bias(z, bias, block);
@@ -218,10 +221,10 @@ __device__ __forceinline__ void linear_columns(uint32_t tz, uint32_t staging, co
   }
 }
 template <int TYPE, int ACT>
-__device__ __forceinline__ void gated_columns(uint32_t tg, uint32_t tu, uint32_t staging, const float (&bias_g)[2], const float (&bias_u)[2],
+__device__ __forceinline__ void gated_columns(uint32_t tg, uint32_t tu, int width, uint32_t staging, const float (&bias_g)[2], const float (&bias_u)[2],
                                               bool has_bias, const WideParams& p, int lane) {
 #pragma unroll 1
-  for (int block = 0; block < 4; ++block) {
+  for (int block = 0; block * 16 < width; ++block) {
     float g[16], u[16];
     load_columns(g, tg + block * 16);
     load_columns(u, tu + block * 16);
@@ -369,18 +372,18 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       const int64_t row0 = (int64_t)tm * 256 + rank * 128 + quad * 32;
       const int rows = (int)min((int64_t)32, (int64_t)p.M - row0);
       Piece ahead;   // the residual of the coming 64 columns, on its way while the MMAs run
-      // 64 columns at a time: the even ones of a tile's chunks are the first four warps', the odd ones the others'
-      const int chunks = ((GATED ? p.bn / 2 : p.bn) + 63) / 64, tile_col = tn * (GATED ? p.bn / 2 : p.bn);
-      if (!GATED && p.residual && rows > 0 && half < chunks && tile_col + half * 64 < p.N)
-        piece_load(ahead, p.residual + row0 * p.ldr + tile_col + half * 64, p.ldr, rows, min(64, p.N - tile_col - half * 64), p.vec_r, lane);
+      // the first four warps take the first half of a tile's columns (gated: features), the others the second, up to 64 at a time
+      const int tile_cols = GATED ? p.bn / 2 : p.bn, mine = tile_cols / 2, col_first = tn * tile_cols + half * mine;
+      if (!GATED && p.residual && p.vec_r && rows > 0 && col_first < p.N)
+        piece_load(ahead, p.residual + row0 * p.ldr + col_first, p.ldr, rows, min(min(64, mine), p.N - col_first), lane);
       const bool ready = mbar_wait(smem_u32(&bars->acc_full[buf]), (it >> 1) & 1, abort_flag, 54, 32);
       if (!__all_sync(0xFFFFFFFFu, ready)) break;
       tc_fence_after();
       const uint32_t lanes = tmem_base + buf * 256 + ((uint32_t)(quad * 32) << 16);
       if constexpr (GATED) {
-        // up to 64 features of this warp: gate sums at columns half * 64, up sums half a tile on
-        const int col0 = tile_col + half * 64, cols = min(min(64, p.bn / 2 - half * 64), p.N - col0);
-        const uint32_t tg = lanes + half * 64, tu = tg + p.bn / 2;
+        // gate sums at columns half * mine of the accumulator, up sums half a tile on
+        const int col0 = col_first, cols = min(mine, p.N - col0);
+        const uint32_t tg = lanes + half * mine, tu = tg + tile_cols;
         const bool any = rows > 0 && cols > 0;
         const bool has_bias = p.bias != nullptr && any;
         float bias_g[2] = {}, bias_u[2] = {};
@@ -392,13 +395,13 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 #pragma unroll 1
           for (int part = 0; part < 2; ++part) {
             const float b[2] = {part ? bias_u[0] : bias_g[0], part ? bias_u[1] : bias_g[1]};
-            preact_columns(part ? tu : tg, staging, b, has_bias, p.preact + row0 * p.ldp + (part ? p.N : 0) + col0, p.ldp, rows, cols,
+            preact_columns(part ? tu : tg, mine, staging, b, has_bias, p.preact + row0 * p.ldp + (part ? p.N : 0) + col0, p.ldp, rows, cols,
                            part ? p.vec_p2 : p.vec_p, lane);
           }
         }
         if (any) {
-          if (p.act == 1) gated_columns<TYPE, 1>(tg, tu, staging, bias_g, bias_u, has_bias, p, lane);
-          else gated_columns<TYPE, 0>(tg, tu, staging, bias_g, bias_u, has_bias, p, lane);
+          if (p.act == 1) gated_columns<TYPE, 1>(tg, tu, mine, staging, bias_g, bias_u, has_bias, p, lane);
+          else gated_columns<TYPE, 0>(tg, tu, mine, staging, bias_g, bias_u, has_bias, p, lane);
         }
         tc_fence_before();
         __syncwarp();
@@ -409,32 +412,33 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         }
       } else {
 #pragma unroll 1
-        for (int chunk = half; chunk < chunks; chunk += 2) {
-          const int col0 = tile_col + chunk * 64, cols = min(64, p.N - col0);
-          const uint32_t tz = lanes + chunk * 64;
-          const bool any = rows > 0 && cols > 0;
+        for (int at = 0; at < mine; at += 64) {
+          const int width = min(64, mine - at), col0 = col_first + at, cols = min(width, p.N - col0);
+          const uint32_t tz = lanes + half * mine + at;
+          const bool any = rows > 0 && cols > 0, last = at + 64 >= mine;
           const bool has_bias = p.bias != nullptr && any;
           float bias[2] = {};
           if (has_bias) load_bias<TYPE>(bias, p.bias + col0, cols, lane);
-          if (p.preact && any) {
-            preact_columns(tz, staging, bias, has_bias, p.preact + row0 * p.ldp + col0, p.ldp, rows, cols, p.vec_p, lane);
-          }
+          if (p.preact && any) preact_columns(tz, width, staging, bias, has_bias, p.preact + row0 * p.ldp + col0, p.ldp, rows, cols, p.vec_p, lane);
           if (p.residual && any) {
-            piece_to_staging(ahead, staging, lane);
+            if (p.vec_r) {
+              piece_to_staging(ahead, staging, p.residual + row0 * p.ldr + col0, p.ldr, rows, cols, lane);
+              if (!last && col0 + 64 < p.N)
+                piece_load(ahead, p.residual + row0 * p.ldr + col0 + 64, p.ldr, rows, min(min(64, mine - at - 64), p.N - col0 - 64), lane);
+            } else {
+              values_in(staging, p.residual + row0 * p.ldr + col0, p.ldr, rows, cols, lane);
+            }
             __syncwarp();
-            if (chunk + 2 < chunks && col0 + 128 < p.N)
-              piece_load(ahead, p.residual + row0 * p.ldr + col0 + 128, p.ldr, rows, min(64, p.N - col0 - 128), p.vec_r, lane);
           }
           if (any) {
             const bool res = p.residual != nullptr;
             switch (p.act) {
-              case kActSilu: linear_columns<TYPE, kActSilu>(tz, staging, bias, has_bias, res, lane); break;
-              case kActGelu: linear_columns<TYPE, kActGelu>(tz, staging, bias, has_bias, res, lane); break;
-              case kActGeluTanh: linear_columns<TYPE, kActGeluTanh>(tz, staging, bias, has_bias, res, lane); break;
-              default: linear_columns<TYPE, kActNone>(tz, staging, bias, has_bias, res, lane);
+              case kActSilu: linear_columns<TYPE, kActSilu>(tz, width, staging, bias, has_bias, res, lane); break;
+              case kActGelu: linear_columns<TYPE, kActGelu>(tz, width, staging, bias, has_bias, res, lane); break;
+              case kActGeluTanh: linear_columns<TYPE, kActGeluTanh>(tz, width, staging, bias, has_bias, res, lane); break;
+              default: linear_columns<TYPE, kActNone>(tz, width, staging, bias, has_bias, res, lane);
             }
           }
-          const bool last = chunk + 2 >= chunks;
           if (last) tc_fence_before();
           __syncwarp();
           if (last && lane == 0) mbar_arrive_cta(smem_u32(&bars->acc_empty[buf]), 0);
@@ -443,7 +447,6 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             __syncwarp();
           }
         }
-        if (half >= chunks && lane == 0) mbar_arrive_cta(smem_u32(&bars->acc_empty[buf]), 0);   // nothing here for this warp
       }
     }
   }

@@ -98,8 +98,8 @@ __device__ __forceinline__ float dense_act_slope(int act, float z) {
 // The gated product of one feature; `limit` = inf for no clamp. min.NaN / max.NaN: a NaN stays NaN.
 __device__ __forceinline__ float dense_gated(int act, float g, float u, float limit, float beta, float linear_beta) {
   if (act == 1) {
-    const float up = linear_beta > 0.0f ? linear_beta * dense_tanh(u / linear_beta) : u;
-    return beta * dense_tanh(g / beta) * dense_sigmoid(g) * up;
+    const float up = linear_beta > 0.0f ? linear_beta * dense_tanh(__fdividef(u, linear_beta)) : u;
+    return beta * dense_tanh(__fdividef(g, beta)) * dense_sigmoid(g) * up;
   }
   float lo = -limit;
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(g) : "f"(limit));
@@ -111,8 +111,8 @@ __device__ __forceinline__ float dense_gated(int act, float g, float u, float li
 __device__ __forceinline__ void dense_gated_grad(int act, float dh, float g, float u, float limit, float beta, float linear_beta,
                                                  float& dg, float& du) {
   if (act == 1) {
-    const float p = dense_sigmoid(g), a = dense_tanh(g / beta);
-    const float b = linear_beta > 0.0f ? dense_tanh(u / linear_beta) : 0.0f;
+    const float p = dense_sigmoid(g), a = dense_tanh(__fdividef(g, beta));
+    const float b = linear_beta > 0.0f ? dense_tanh(__fdividef(u, linear_beta)) : 0.0f;
     const float up = linear_beta > 0.0f ? linear_beta * b : u;
     dg = dh * up * ((1.0f - a * a) * p + beta * a * p * (1.0f - p));
     du = dh * (beta * a * p) * (1.0f - b * b);

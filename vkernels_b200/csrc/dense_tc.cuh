@@ -4,6 +4,7 @@
 #include <atomic>
 
 #include "dense.hpp"
+#include "dense_launch.cuh"
 #include "dense_math.cuh"
 #include "sm100.cuh"
 
@@ -42,18 +43,6 @@ __device__ __forceinline__ uint32_t operand_idesc(int m, int n, int a_mn, int b_
 }
 
 bool aligned16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
-
-// A kernel of these may be scheduled while the kernels before it on its stream still run (programmatic launch): its barriers
-// and tensor memory are set up meanwhile. Nothing in memory is touched before this, which returns once all of them are done
-// and their writes visible.
-__device__ __forceinline__ void wait_for_earlier_kernels() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-void overlap_launch(cudaLaunchAttribute& a) {
-  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  a.val.programmaticStreamSerializationAllowed = 1;
-}
 
 int* status_address() {
   static std::atomic<int*> known[64];

@@ -159,6 +159,9 @@ class CudaBackend:
     """Device steps of the EP layer on the CUDA library."""
 
     def __init__(self, layer, device):
+        if getattr(layer, "shared_ffn", None) is not None:
+            raise ValueError("the expert-parallel layer runs the routed experts only: build it without shared_ffn and call "
+                             "shared_ffn(x, y, out=y) on each rank's tokens and result")
         self.layer = layer          # vkernels_b200.experts.FusedMoEMxfp4 holding the LOCAL experts
         self.device = torch.device(device)
 

@@ -86,8 +86,11 @@ class FusedMoEMxfp4:
                  scaling: float = 1.0, n_group: int = 1, topk_group: int = 1, n_shared: int = 0,
                  swiglu_limit: float = 0.0, activation: int = ops.moe_fused_mxfp4.SWIGLU,
                  beta: float = 4.0, linear_beta: float = 25.0, b13=None, b2=None,
-                 max_tokens: int = DEFAULT_TOKEN_BUDGET, block_size: int = 16, prepack: bool = False):
-        """``prepack``: also keep the weights in the prepacked form (``ops.prepack_weights``; about as
+                 max_tokens: int = DEFAULT_TOKEN_BUDGET, block_size: int = 16, prepack: bool = False, shared_ffn=None):
+        """``shared_ffn`` (``feedforward.DenseFeedForward``): an always-on expert in bf16, for checkpoints that do not hold it
+        among the MXFP4 experts (those take ``n_shared``); ``forward`` adds its result to the routed experts'.
+
+        ``prepack``: also keep the weights in the prepacked form (``ops.prepack_weights``; about as
         large as the checkpoint form again) and run decode-size batches from it - their kernels
         then expand nothing and run at the memory rate. Off by default because of the memory; a
         weight set with codes the form cannot express (inf / NaN) silently stays on the
@@ -112,6 +115,10 @@ class FusedMoEMxfp4:
         # layer holds only a slice of them
         self.n_router = self.n_routed if router_weight is None else router_weight.shape[0]
         self.block_size = block_size
+        ops.require(shared_ffn is None or (shared_ffn.hidden == self.hidden and shared_ffn.w13.dtype == torch.bfloat16
+                                           and shared_ffn.w13.device == self.device),
+                    f"shared_ffn must be bf16, with hidden = {self.hidden}, on {self.device}")
+        self.shared_ffn = shared_ffn
         self.max_tokens = int(max_tokens or DEFAULT_TOKEN_BUDGET)
         self.capture_stream = None
         self.prepacked = None
@@ -153,6 +160,7 @@ class FusedMoEMxfp4:
             "out": (torch.float32, T * self.hidden),
             "x": (torch.bfloat16, T * self.hidden),
             "y": (torch.bfloat16, T * self.hidden),
+            "shared": (torch.bfloat16, T * (0 if self.shared_ffn is None else self.shared_ffn.ispp)),
         }, self.device)
 
     def _buffers(self, T: int):
@@ -248,7 +256,7 @@ class FusedMoEMxfp4:
                                       store_slots=store_slots)
 
     def forward(self, x: torch.Tensor, *, logits: torch.Tensor | None = None, out_bf16=None):
-        """route -> align -> gate/up -> down+combine, all on the current stream."""
+        """route -> align -> gate/up -> down+combine (+ shared_ffn), all on the current stream."""
         ops.require(x.dim() == 2 and x.shape[1] == self.hidden, "x must be [T, hidden]")
         bufs = self._buffers(x.shape[0])
         T = x.shape[0]
@@ -263,10 +271,18 @@ class FusedMoEMxfp4:
                     renorm=self.renorm, scaling=self.scaling, n_shared=self.n_shared, max_EM=self._em_bound(T),
                     out=(bufs["ids"].view(T, self.slots), bufs["w"].view(T, self.slots), bufs["sids"], bufs["eids"],
                          bufs["out_em"]))
-            return self.experts(x, ids, w, bufs, out_bf16=out_bf16, aligned=(sids, eids))
+            return self._add_shared(x, self.experts(x, ids, w, bufs, out_bf16=out_bf16, aligned=(sids, eids)))
         with _region("moe:apply.route"):
             ids, w = self.route(x, bufs, logits=logits)
-        return self.experts(x, ids, w, bufs, out_bf16=out_bf16)
+        return self._add_shared(x, self.experts(x, ids, w, bufs, out_bf16=out_bf16))
+
+    def _add_shared(self, x, y):
+        """y, with the always-on expert's result added in place (the routed result is its residual)."""
+        if self.shared_ffn is None:
+            return y
+        T = x.shape[0]
+        with _region("moe:apply.shared"):
+            return self.shared_ffn(x, y, out=y, product=self.arena.take("shared", T * self.shared_ffn.ispp).view(T, -1))
 
     __call__ = forward
 
@@ -355,11 +371,13 @@ class HostPipeline:
         self.d2h.synchronize()
 
 
-def layer_from_config(cfg, weights: dict, router: dict | None, *, max_tokens: int | None = None, prepack: bool = False):
+def layer_from_config(cfg, weights: dict, router: dict | None, *, max_tokens: int | None = None, prepack: bool = False,
+                      shared_ffn=None):
     """Build the layer for a ``synthetic.MoEConfig`` from generated tensors."""
     return FusedMoEMxfp4(
         weights["w13"], weights["w13_scale"], weights["w2"], weights["w2_scale"], top_k=cfg.top_k,
         router_weight=None if router is None else router["wr"],
         router_bias=None if router is None else router["bias"], routing=cfg.routing,
         renorm=cfg.renorm, scaling=cfg.scaling, n_group=cfg.n_group, topk_group=cfg.topk_group,
-        n_shared=cfg.shared_experts, swiglu_limit=cfg.swiglu_limit, max_tokens=max_tokens, prepack=prepack)
+        n_shared=cfg.shared_experts, swiglu_limit=cfg.swiglu_limit, max_tokens=max_tokens, prepack=prepack,
+        shared_ffn=shared_ffn)

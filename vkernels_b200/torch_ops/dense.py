@@ -20,7 +20,7 @@ from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
 from .. import native_runtime as nr
-from ._dispatch import require
+from ._dispatch import OpNotEligible
 from .moe_fused_mxfp4 import SITU, SWIGLU
 
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1}
@@ -59,18 +59,23 @@ def _plain(t, shape, dtype, index):
 
 
 def _check(name, t, dtype, device):
-    require(isinstance(t, torch.Tensor), f"{name} must be a tensor")
-    require(t.dtype == dtype, f"{name} must be {dtype}, like the other tensors of the call, got {t.dtype}")
-    require(t.device == device, f"{name} must be on {device}, got {t.device}")
+    if not isinstance(t, torch.Tensor):
+        raise OpNotEligible(f"{name} must be a tensor")
+    if t.dtype != dtype:
+        raise OpNotEligible(f"{name} must be {dtype}, like the other tensors of the call, got {t.dtype}")
+    if t.device != device:
+        raise OpNotEligible(f"{name} must be on {device}, got {t.device}")
 
 
 def _pitch(name, t):
     """Elements from one row of a 2-D tensor to the next."""
     T, n = t.shape
-    require(n <= 1 or t.stride(1) == 1, f"the values of a row of {name} must be neighbours in memory")
+    if n > 1 and t.stride(1) != 1:
+        raise OpNotEligible(f"the values of a row of {name} must be neighbours in memory")
     if T <= 1:
         return (n + 7) // 8 * 8
-    require(t.stride(0) >= n, f"the rows of {name} must not overlap")
+    if t.stride(0) < n:
+        raise OpNotEligible(f"the rows of {name} must not overlap")
     return t.stride(0)
 
 
@@ -87,30 +92,37 @@ def _apart(name, out, others):
     for other_name, t in others:
         if t is not None:
             c, d = _span(t)
-            require(b <= c or d <= a, f"{name} must not overlap {other_name}")
+            if a < d and c < b:
+                raise OpNotEligible(f"{name} must not overlap {other_name}")
 
 
 def _rows2d(name, t, cols):
     """A result tensor of the caller, or a tensor that goes with the result, as [T, cols] without a copy."""
-    require(t.dim() >= 1 and t.shape[-1] == cols, f"{name} must have {cols} columns")
+    if t.dim() < 1 or t.shape[-1] != cols:
+        raise OpNotEligible(f"{name} must have {cols} columns")
     if t.dim() == 2:
         return t
     try:
         return t.view(-1, cols)
     except RuntimeError:
-        require(False, f"{name} must be viewable as rows of {cols}")
+        raise OpNotEligible(f"{name} must be viewable as rows of {cols}")
 
 
 def _inputs(x, w, gated, what):
-    require(isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor), f"{what}: tensors expected")
-    require(x.dtype in _DTYPE, f"x must be bfloat16 or float16, got {x.dtype}")
+    if not (isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor)):
+        raise OpNotEligible(f"{what}: tensors expected")
+    if x.dtype not in _DTYPE:
+        raise OpNotEligible(f"x must be bfloat16 or float16, got {x.dtype}")
     _check("the weight", w, x.dtype, x.device)
-    require(x.dim() >= 1 and w.dim() == 2 and w.shape[1] == x.shape[-1], f"{what}: x [..., n_in] and a weight [rows, n_in] expected")
-    require(w.shape[1] > 0 and w.shape[0] > 0, f"{what}: feature counts must be positive")
-    require(not gated or w.shape[0] % 2 == 0, "w13 must hold gate rows followed by up rows: an even row count")
+    if not (x.dim() >= 1 and w.dim() == 2 and w.shape[1] == x.shape[-1]):
+        raise OpNotEligible(f"{what}: x [..., n_in] and a weight [rows, n_in] expected")
+    if not (w.shape[1] > 0 and w.shape[0] > 0):
+        raise OpNotEligible(f"{what}: feature counts must be positive")
+    if gated and w.shape[0] % 2:
+        raise OpNotEligible("w13 must hold gate rows followed by up rows: an even row count")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    require(x2.shape[0] < _MOST_TOKENS and w.shape[0] < _MOST_ROWS and w.shape[1] <= _MOST_IN,
-            f"{what}: more rows or features than the kernels index")
+    if not (x2.shape[0] < _MOST_TOKENS and w.shape[0] < _MOST_ROWS and w.shape[1] <= _MOST_IN):
+        raise OpNotEligible(f"{what}: more rows or features than the kernels index")
     return x2
 
 
@@ -118,7 +130,8 @@ def _bias(bias, rows, x):
     if bias is None:
         return None
     _check("the bias", bias, x.dtype, x.device)
-    require(bias.shape == (rows,) and (rows == 1 or bias.stride(0) == 1), f"the bias must be contiguous [{rows}]")
+    if not (bias.shape == (rows,) and (rows == 1 or bias.stride(0) == 1)):
+        raise OpNotEligible(f"the bias must be contiguous [{rows}]")
     return bias.data_ptr()
 
 
@@ -131,19 +144,21 @@ def _wants_grad(*tensors):
 
 
 def _no_capture():
-    require(not torch.cuda.is_current_stream_capturing(),
-            "recording for backward() cannot be captured into a CUDA graph: capture the forward call with return_preact=True "
-            "on detached tensors and its *_backward")
+    if torch.cuda.is_current_stream_capturing():
+        raise OpNotEligible("recording for backward() cannot be captured into a CUDA graph: capture the forward call with "
+                            "return_preact=True on detached tensors and its *_backward")
 
 
 def _resident(x):
-    require(x.is_cuda, "inputs must be CUDA-resident (there is no CPU path)")
+    if not x.is_cuda:
+        raise OpNotEligible("inputs must be CUDA-resident (there is no CPU path)")
 
 
 def _given_out(out, shape, x, others):
     """A result tensor of the caller, as rows."""
     _check("out", out, x.dtype, x.device)
-    require(tuple(out.shape) == tuple(shape), f"out must be {tuple(shape)}, got {tuple(out.shape)}")
+    if tuple(out.shape) != tuple(shape):
+        raise OpNotEligible(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
     _apart("out", out, others)
     out2 = _rows2d("out", out, shape[-1])
     _pitch("out", out2)
@@ -173,9 +188,12 @@ def _forward_work(x, ldx, w, ldw, T, n_in, rows):
 # ---------------------------------------------------------------------------
 
 def _gated_kind(activation, swiglu_limit, beta):
-    require(activation in (SWIGLU, SITU), "activation must be SWIGLU or SITU")
-    require(swiglu_limit >= 0, "swiglu_limit must not be negative (0 for none)")
-    require(activation == SWIGLU or beta > 0, "SiTU needs a positive beta")
+    if activation not in (SWIGLU, SITU):
+        raise OpNotEligible("activation must be SWIGLU or SITU")
+    if not swiglu_limit >= 0:
+        raise OpNotEligible("swiglu_limit must not be negative (0 for none)")
+    if activation == SITU and not beta > 0:
+        raise OpNotEligible("SiTU needs a positive beta")
 
 
 def gated_linear(x: torch.Tensor, w13: torch.Tensor, b13: torch.Tensor | None = None, *, activation: int = SWIGLU,
@@ -213,7 +231,8 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, b13: torch.Tensor | None = 
     out2 = None if out is None else _given_out(out, shape, x, (("x", x), ("w13", w13), ("b13", b13)))
     _resident(x)
     if _wants_grad(x, w13, b13, out):
-        require(out is None and not return_preact, "gated_linear: out and return_preact are for calls that record no gradient")
+        if out is not None or return_preact:
+            raise OpNotEligible("gated_linear: out and return_preact are for calls that record no gradient")
         return _GatedLinear.apply(x, w13, b13, activation, swiglu_limit, beta, linear_beta)
     h, h2 = _result(out, out2, shape, x)
     preact = torch.empty((T, rows), dtype=torch.float32, device=x.device) if return_preact else None
@@ -231,7 +250,8 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w13: torch.Tensor, 
     """``(dx, dw13, db13)`` for the gradient dh of ``gated_linear``'s result; ``preact`` as that call returned it, the other
     arguments as it was given. What is not asked for is None."""
     _gated_kind(activation, swiglu_limit, beta)
-    require(preact is not None, "gated_linear_backward needs the forward call's pre-activations")
+    if preact is None:
+        raise OpNotEligible("gated_linear_backward needs the forward call's pre-activations")
     return _backward("vk_cuda_gated_linear_backward", dh, x, w13, preact, True, bias_grad, x_grad, w_grad,
                      (activation, swiglu_limit, beta, linear_beta))
 
@@ -242,7 +262,8 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w13: torch.Tensor, 
 
 def _linear_kind(activation):
     kind = _LINEAR_ACT.get(activation) if activation is None or isinstance(activation, str) else None
-    require(kind is not None, f"activation must be None, 'silu', 'gelu' or 'gelu_tanh', got {activation!r}")
+    if kind is None:
+        raise OpNotEligible(f"activation must be None, 'silu', 'gelu' or 'gelu_tanh', got {activation!r}")
     return kind
 
 
@@ -278,7 +299,8 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     r2, ldr = None, 0
     if residual is not None:
         _check("the residual", residual, x.dtype, x.device)
-        require(tuple(residual.shape) == shape, f"the residual must be {shape}, got {tuple(residual.shape)}")
+        if tuple(residual.shape) != shape:
+            raise OpNotEligible(f"the residual must be {shape}, got {tuple(residual.shape)}")
         r2 = _rows2d("the residual", residual, n_out)
         ldr = _pitch("the residual", r2)
     out2 = None
@@ -287,7 +309,8 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
         out2 = _given_out(out, shape, x, (("x", x), ("w", w), ("the bias", bias), ("the residual", None if in_place else residual)))
     _resident(x)
     if _wants_grad(x, w, bias, residual, out):
-        require(out is None and not return_preact, "fused_linear: out and return_preact are for calls that record no gradient")
+        if out is not None or return_preact:
+            raise OpNotEligible("fused_linear: out and return_preact are for calls that record no gradient")
         return _FusedLinear.apply(x, w, bias, residual, activation)
     T, n_in = x2.shape
     y, y2 = _result(out, out2, shape, x)
@@ -305,33 +328,53 @@ def fused_linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pr
     """``(dx, dw, dbias)`` for the gradient dy of ``fused_linear``'s result; ``preact`` as that call returned it (None without an
     activation). What is not asked for is None. The residual's gradient is dy."""
     act = _linear_kind(activation)
-    require(act == 0 or preact is not None, "fused_linear_backward needs the forward call's pre-activations")
+    if act and preact is None:
+        raise OpNotEligible("fused_linear_backward needs the forward call's pre-activations")
     return _backward("vk_cuda_fused_linear_backward", dy, x, w, preact if act else None, False, bias_grad, x_grad, w_grad, (act,))
 
 
 def _backward(entry, dy, x, w, preact, gated, bias_grad, x_grad, w_grad, kind):
-    x2 = _inputs(x, w, gated, entry[8:])
-    rows, (T, n_in) = w.shape[0], x2.shape
-    n_out = rows // 2 if gated else rows
-    dtype, device = x.dtype, x.device
-    _check("the result's gradient", dy, dtype, device)
-    require(tuple(dy.shape) == (*x.shape[:-1], n_out), f"the result's gradient must be {(*x.shape[:-1], n_out)}, got {tuple(dy.shape)}")
-    dy2 = dy if dy.dim() == 2 else dy.reshape(-1, n_out)
-    if preact is not None:
-        _check("preact", preact, torch.float32, device)
-        require(tuple(preact.shape) == (T, rows), f"preact must be {(T, rows)}, got {tuple(preact.shape)}")
-    ldx, ldw, ld_dy = _pitch("x", x2), _pitch("the weight", w), _pitch("the result's gradient", dy2)
-    ldp = 0 if preact is None else _pitch("preact", preact)
-    _resident(x)
-    dx = torch.empty(x.shape, dtype=dtype, device=device) if x_grad else None
-    dw = torch.empty((rows, n_in), dtype=dtype, device=device) if w_grad else None
-    db = torch.empty(rows, dtype=dtype, device=device) if bias_grad else None
+    ordinary = False
+    if type(x) is torch.Tensor and isinstance(w, torch.Tensor) and isinstance(dy, torch.Tensor):
+        # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
+        shape, index, dtype, wshape = x.shape, x.get_device(), x.dtype, w.shape
+        ordinary = (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and wshape[1] == shape[1] > 0
+                    and not shape[1] & 7 and 0 < wshape[0] < _MOST_ROWS and not (gated and wshape[0] & 1) and 0 < shape[0] < _MOST_TOKENS
+                    and _plain(x, shape, dtype, index) and _plain(w, wshape, dtype, index)
+                    and _plain(dy, (shape[0], wshape[0] >> gated), dtype, index)
+                    and (preact is None or _plain(preact, (shape[0], wshape[0]), torch.float32, index)))
+    if ordinary:
+        (T, n_in), rows = shape, wshape[0]
+        n_out = ld_dy = rows >> gated
+        ldx = ldw = n_in
+        ldp = rows
+        dy2, x2 = dy, x
+    else:
+        x2 = _inputs(x, w, gated, entry[8:])
+        rows, (T, n_in) = w.shape[0], x2.shape
+        n_out = rows // 2 if gated else rows
+        dtype = x.dtype
+        _check("the result's gradient", dy, dtype, x.device)
+        if tuple(dy.shape) != (*x.shape[:-1], n_out):
+            raise OpNotEligible(f"the result's gradient must be {(*x.shape[:-1], n_out)}, got {tuple(dy.shape)}")
+        dy2 = dy if dy.dim() == 2 else dy.reshape(-1, n_out)
+        if preact is not None:
+            _check("preact", preact, torch.float32, x.device)
+            if tuple(preact.shape) != (T, rows):
+                raise OpNotEligible(f"preact must be {(T, rows)}, got {tuple(preact.shape)}")
+        ldx, ldw, ld_dy = _pitch("x", x2), _pitch("the weight", w), _pitch("the result's gradient", dy2)
+        ldp = 0 if preact is None else _pitch("preact", preact)
+        _resident(x)
+        index = x.get_device()
+    dx = x.new_empty(x.shape) if x_grad else None
+    dw = x.new_empty((rows, n_in)) if w_grad else None
+    db = x.new_empty((rows,)) if bias_grad else None
     if dx is None and dw is None and db is None:
         return None, None, None
     xp, wp = x2.data_ptr(), w.data_ptr()
     nbytes = _entry("vk_cuda_dense_backward_workspace_bytes")(xp, ldx, wp, ldw, T, n_in, n_out, gated)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _call(entry, x.get_device(), dy2.data_ptr(), ld_dy, xp, ldx, wp, ldw, None if preact is None else preact.data_ptr(), ldp,
+    work = x.new_empty((nbytes,), dtype=torch.uint8)
+    _call(entry, index, dy2.data_ptr(), ld_dy, xp, ldx, wp, ldw, None if preact is None else preact.data_ptr(), ldp,
           None if dx is None else dx.data_ptr(), n_in, None if dw is None else dw.data_ptr(), n_in, None if db is None else db.data_ptr(),
           _DTYPE[dtype], T, n_in, n_out, *kind, work.data_ptr(), nbytes)
     return dx, dw, db
