@@ -33,7 +33,7 @@ constexpr int kWideSmem = kStages * kStageBytes + kEpiWarps * kStagingBytes + (i
 struct WideParams {
   int M, N, K;                // N: columns of the result (gated: features)
   int a_mn, b_mn;
-  int bn;                     // rows of B a tile: 64, 128, 192 or 256
+  int bn;                     // rows of B a tile: a multiple of 32 from 64 to 256
   int stage_bytes;            // of one CTA: what the copies of a stage bring
   int tiles_m, tiles_n, n_tiles, k_blocks;
   int act;
@@ -98,15 +98,19 @@ __device__ __forceinline__ void piece_to_staging(const Piece& d, uint32_t base, 
   for (int c = cols & ~7; c < cols; ++c)
     if (lane < rows) sts16(staging_at(base, lane, c >> 3) + (c & 7) * 2, p[(int64_t)lane * ld + c]);
 }
-// Rows that start anywhere: a row at a time, a value a lane.
+// Rows that start anywhere: a row at a time, a value a lane; sixteen rows on their way before the first is put down.
 __device__ __forceinline__ void values_in(uint32_t base, const uint16_t* p, int64_t ld, int rows, int cols, int lane) {
-#pragma unroll 16
-  for (int r = 0; r < 32; ++r) {
+#pragma unroll 1
+  for (int first = 0; first < 32; first += 16) {
+    uint16_t v[16][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = h * 32 + lane;
-      sts16(staging_at(base, r, c >> 3) + (c & 7) * 2, r < rows && c < cols ? p[(int64_t)r * ld + c] : (uint16_t)0);
-    }
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) v[i][h] = first + i < rows && h * 32 + lane < cols ? p[(int64_t)(first + i) * ld + h * 32 + lane] : (uint16_t)0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) sts16(staging_at(base, first + i, (h * 32 + lane) >> 3) + (lane & 7) * 2, v[i][h]);
   }
 }
 __device__ __forceinline__ void staging_out(uint32_t base, uint16_t* p, int64_t ld, int rows, int cols, int vec, int lane) {
@@ -170,20 +174,20 @@ __device__ __forceinline__ void preact_columns(uint32_t tz, int width, uint32_t 
                                                                     __float_as_uint(z[j * 4 + 2]), __float_as_uint(z[j * 4 + 3])));
     }
     __syncwarp();
-    float* q = p + r0 * ld + part * 32 + u * 4;
-    const int left = cols - part * 32 - u * 4;
+    const int left = min(32, cols - part * 32);
+    float* q = p + part * 32;
+    if (vec && (left & 3) == 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint4 v = lds128(staging_at(staging, i * 4 + r0, u));
-      if (i * 4 + r0 >= rows) continue;
-      float* at = q + (int64_t)(i * 4) * ld;
-      if (vec && left >= 4) {
-        *reinterpret_cast<uint4*>(at) = v;
-      } else {
-        if (left > 0) at[0] = __uint_as_float(v.x);
-        if (left > 1) at[1] = __uint_as_float(v.y);
-        if (left > 2) at[2] = __uint_as_float(v.z);
-        if (left > 3) at[3] = __uint_as_float(v.w);
+      for (int i = 0; i < 8; ++i) {
+        const uint4 v = lds128(staging_at(staging, i * 4 + r0, u));
+        if (i * 4 + r0 < rows && u * 4 < left) *reinterpret_cast<uint4*>(q + (int64_t)(i * 4 + r0) * ld + u * 4) = v;
+      }
+    } else {   // rows that start anywhere: a row at a time, a value a lane
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r) {
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(staging_at(staging, r, lane >> 2) + (lane & 3) * 4) : "memory");
+        if (lane < left) q[(int64_t)r * ld + lane] = v;
       }
     }
     __syncwarp();
@@ -469,26 +473,26 @@ CUtensorMap operand_map(const DenseOperand& o, int64_t rows, int K, int box) {
 }
 
 // How a launch is cut, and how long it takes by that (us): the width of a tile that makes waves x time of a wave smallest. A
-// tile's time is its k blocks' (0.28, 0.216, 0.152 and 0.148 us each for 256, 192, 128 and 64 rows of B: below 192 a stage is
-// bound by bringing A) and what comes before and after them. Measured on 2880 -> 2880: 512 tokens 20.1, 17.6, 13.4 and 19.1 us,
-// 1024 tokens 22.3, 18.4, 21.2 and 27.0, 2047 tokens 35.2, 29.3, 30.4 and 43.3; with many waves the widest is best or within
-// 4 % of it (8192 tokens 101.5, 97.9, 108.5, 161.1; 8192 x 7168 -> 2048 170, 175, 193, 296).
+// tile's time is its k blocks' (0.152 us each for 128 rows of B, 0.28 for 256, straight between; below 128 a stage is bound by
+// bringing A) and what comes before and after them. Measured on 2880 -> 2880, widths 256, 192, 128 and 64: 512 tokens 20.1, 17.6,
+// 13.4 and 19.1 us, 1024 tokens 22.3, 18.4, 21.2 and 27.0, 2047 tokens 35.2, 29.3, 30.4 and 43.3; with many waves the widest is
+// best or within 4 % of it (8192 tokens 101.5, 97.9, 108.5, 161.1; 8192 x 7168 -> 2048 170, 175, 193, 296).
 struct WidePlan {
   int bn;
   float us;
 };
 WidePlan plan_wide(int64_t M, int64_t N, int64_t K, bool gated) {
-  constexpr int kWidths[4] = {256, 192, 128, 64};
-  constexpr float kBlockUs[4] = {0.28f, 0.216f, 0.152f, 0.148f}, kEndsUs[4] = {7.2f, 6.3f, 5.3f, 5.4f};
   const int64_t pairs = sm_count() / 2, tiles_m = (M + 255) / 256, blocks = (K + 63) / 64;
   WidePlan best{256, 1e30f};
-  for (int i = 0; i < 4; ++i) {
-    const int64_t tile_n = gated ? kWidths[i] / 2 : kWidths[i], tiles = tiles_m * ((N + tile_n - 1) / tile_n);
-    const float waves = (float)((tiles + pairs - 1) / pairs);
+  for (int bn = 256; bn >= 64; bn -= 32) {
+    const int64_t tile_n = gated ? bn / 2 : bn, tiles = tiles_m * ((N + tile_n - 1) / tile_n);
+    const float waves = (float)((tiles + pairs - 1) / pairs), narrower = (float)(256 - bn) / 64.0f;
+    const float block_us = bn >= 128 ? 0.024f + 0.001f * (float)bn : 0.144f + 0.0001f * (float)bn;
+    const float ends_us = bn >= 128 ? 3.4f + 0.0148f * (float)bn : 5.4f;
     // the more pairs are at work, the slower the narrower tiles, which bring more bytes for a product
-    const float load = waves > 1.0f || i == 0 ? 1.0f + 0.06f * i : 1.0f + 0.06f * i * (float)tiles / (float)pairs;
-    const float us = kEndsUs[i] + waves * ((float)blocks * kBlockUs[i] * load) + (waves - 1.0f) * 1.0f;
-    if (us < best.us) best = {kWidths[i], us};
+    const float load = 1.0f + 0.06f * narrower * (waves > 1.0f ? 1.0f : (float)tiles / (float)pairs);
+    const float us = ends_us + waves * ((float)blocks * block_us * load) + (waves - 1.0f) * 1.0f;
+    if (us < best.us) best = {bn, us};
   }
   return best;
 }

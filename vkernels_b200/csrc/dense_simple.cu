@@ -102,95 +102,88 @@ __device__ __forceinline__ Eight load_eight(const uint16_t* p, int n, bool vec) 
   }
   return e;
 }
-__device__ __forceinline__ void store_eight(uint16_t* p, const Eight& e, int n, bool vec) {
-  if (vec && n >= 8) {
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e.v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = e.v[j];
-  }
-}
 
-__device__ __forceinline__ void load_eight_f32(float (&v)[8], const float* p, int n, bool vec) {
-  if (vec && n >= 8) {
-    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
-    *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(p + 4);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : 0.0f;
-  }
-}
-
-constexpr int kGradCols = 256, kGradThreads = 256;   // 32 threads across the columns, eight each; 8 rows at a time
+constexpr int kGradCols = 256, kGradThreads = 256;   // 64 threads across the columns, four each; four rows at a time
+constexpr int kGradRows = 4, kGradStep = 4 * kGradRows;   // rows a thread has on their way, rows a CTA takes at once
 
 // dz = dy * act'(z) and the column sums of a chunk of rows, in one pass: one CTA per 256 columns of dy and chunk. A column's
-// sum is added by one thread per eighth row in fp32, the eighths in order, the chunks by dense_sum_kernel: no atomics, the
-// same result every time. The sums are of the unrounded gradients. Bound by memory: dy and z in, dz out. VEC: a thread's eight
-// columns are neighbours, in 16-byte accesses; else 32 apart, so that a warp still reads whole lines of rows that start anywhere
-// (1001 x 1027 gated: 14.6 us with neighbours).
+// sum is added by one thread per fourth row in fp32, the fourths in order, the chunks by dense_sum_kernel: no atomics, the same
+// result every time. The sums are of the unrounded gradients. Bound by memory (dy and z in, dz out), as long as enough of it is
+// on its way: four rows a thread before the first is worked on, the whole launch resident at once (4096 x 2880 gated: eight
+// columns a thread, one row at a time and three times as many CTAs took 41 us). VEC: a thread's four columns are neighbours, in
+// whole accesses; else 64 apart, so that a warp still reads whole lines of rows that start anywhere.
 template <int TYPE, bool GATED, bool VEC>
-__global__ void __launch_bounds__(kGradThreads) dense_grad_kernel(DenseGrad g, int rows_per_chunk) {
-  __shared__ float sums[GATED ? 2 : 1][8][kGradCols];
+__global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g, int rows_per_chunk) {
+  __shared__ float sums[GATED ? 2 : 1][4][kGradCols];
   wait_for_earlier_kernels();
-  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5, first = blockIdx.x * kGradCols;
+  const int across = threadIdx.x & 63, sub = threadIdx.x >> 6, first = blockIdx.x * kGradCols;
   const int r_end = min(g.T, (int)(blockIdx.y + 1) * rows_per_chunk);
-  const auto column = [&](int j) { return VEC ? lane * 8 + j : lane + j * 32; };
+  const auto column = [&](int j) { return VEC ? across * 4 + j : across + j * 64; };
   const int c0 = first + column(0);
-  float sg[8] = {}, su[8] = {};
+  float sg[4] = {}, su[4] = {};
   if (c0 < g.N) {
-#pragma unroll 2
-    for (int r = blockIdx.y * rows_per_chunk + sub; r < r_end; r += 8) {
-      const uint16_t* py = g.dy + (int64_t)r * g.lddy + c0;
-      const float* pz = g.preact + (int64_t)r * g.ldp + c0;
-      uint16_t* pd = g.dz + (int64_t)r * g.ldz + c0;
-      Eight dy, og, ou;
-      float zg[8] = {}, zu[8] = {};
-      if constexpr (VEC) {
-        dy = load_eight(py, g.N - c0, true);
-        if (g.preact) load_eight_f32(zg, pz, g.N - c0, true);
-        if constexpr (GATED) load_eight_f32(zu, pz + g.N, g.N - c0, true);
-      } else {
+    for (int r0 = blockIdx.y * rows_per_chunk + sub; r0 < r_end; r0 += kGradStep) {
+      uint2 dy[kGradRows];
+      float zg[kGradRows][4] = {}, zu[kGradRows][4] = {};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool in = c0 + j * 32 < g.N;
-          dy.v[j] = in ? py[j * 32] : (uint16_t)0;
-          if (g.preact) zg[j] = in ? pz[j * 32] : 0.0f;
-          if constexpr (GATED) zu[j] = in ? pz[g.N + j * 32] : 0.0f;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float d = dense_to_f32<TYPE>(dy.v[j]);
-        if constexpr (GATED) {
-          float du;
-          dense_gated_grad(g.act, d, zg[j], zu[j], g.limit, g.beta, g.linear_beta, d, du);
-          su[j] += du;
-          ou.v[j] = dense_from_f32<TYPE>(du);
-        } else {
-          if (g.preact) d *= dense_act_slope(g.act, zg[j]);
-        }
-        sg[j] += d;
-        og.v[j] = dense_from_f32<TYPE>(d);
-      }
-      if (g.dz) {
+      for (int i = 0; i < kGradRows; ++i) {
+        const int64_t r = r0 + i * 4;
+        dy[i] = make_uint2(0, 0);
+        if (r >= r_end) continue;
+        const uint16_t* py = g.dy + r * g.lddy + c0;
+        const float* pz = g.preact + r * g.ldp + c0;
         if constexpr (VEC) {
-          store_eight(pd, og, g.N - c0, true);
-          if constexpr (GATED) store_eight(pd + g.N, ou, g.N - c0, true);
+          dy[i] = *reinterpret_cast<const uint2*>(py);
+          if (GATED || g.preact) *reinterpret_cast<float4*>(zg[i]) = *reinterpret_cast<const float4*>(pz);
+          if constexpr (GATED) *reinterpret_cast<float4*>(zu[i]) = *reinterpret_cast<const float4*>(pz + g.N);
         } else {
+          uint16_t v[4];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (c0 + j * 32 < g.N) {
-              pd[j * 32] = og.v[j];
-              if constexpr (GATED) pd[g.N + j * 32] = ou.v[j];
-            }
+          for (int j = 0; j < 4; ++j) {
+            const bool in = c0 + j * 64 < g.N;
+            v[j] = in ? py[j * 64] : (uint16_t)0;
+            if (GATED || g.preact) zg[i][j] = in ? pz[j * 64] : 0.0f;
+            if constexpr (GATED) zu[i][j] = in ? pz[g.N + j * 64] : 0.0f;
+          }
+          dy[i] = make_uint2(v[0] | ((uint32_t)v[1] << 16), v[2] | ((uint32_t)v[3] << 16));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kGradRows; ++i) {
+        const int64_t r = r0 + i * 4;
+        if (r >= r_end) break;
+        const float2 lo = dense_unpack<TYPE>(dy[i].x), hi = dense_unpack<TYPE>(dy[i].y);
+        float d[4] = {lo.x, lo.y, hi.x, hi.y}, du[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (GATED) {
+            dense_gated_grad(g.act, d[j], zg[i][j], zu[i][j], g.limit, g.beta, g.linear_beta, d[j], du[j]);
+            su[j] += du[j];
+          } else {
+            if (g.preact) d[j] *= dense_act_slope(g.act, zg[i][j]);
+          }
+          sg[j] += d[j];
+        }
+        if (g.dz) {
+          uint16_t* pd = g.dz + r * g.ldz + c0;
+          if constexpr (VEC) {
+            *reinterpret_cast<uint2*>(pd) = make_uint2(dense_pack<TYPE>(d[0], d[1]), dense_pack<TYPE>(d[2], d[3]));
+            if constexpr (GATED) *reinterpret_cast<uint2*>(pd + g.N) = make_uint2(dense_pack<TYPE>(du[0], du[1]), dense_pack<TYPE>(du[2], du[3]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (c0 + j * 64 < g.N) {
+                pd[j * 64] = dense_from_f32<TYPE>(d[j]);
+                if constexpr (GATED) pd[g.N + j * 64] = dense_from_f32<TYPE>(du[j]);
+              }
+          }
         }
       }
     }
   }
   if (g.partial == nullptr) return;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 4; ++j) {
     sums[0][sub][column(j)] = sg[j];
     if constexpr (GATED) sums[GATED ? 1 : 0][sub][column(j)] = su[j];
   }
@@ -202,7 +195,7 @@ __global__ void __launch_bounds__(kGradThreads) dense_grad_kernel(DenseGrad g, i
   for (int h = 0; h < (GATED ? 2 : 1); ++h) {
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += sums[h][i][threadIdx.x];
+    for (int i = 0; i < 4; ++i) s += sums[h][i][threadIdx.x];
     g.partial[(int64_t)blockIdx.y * rows + h * g.N + col] = s;
   }
 }
@@ -253,11 +246,10 @@ __global__ void __launch_bounds__(256) dense_copy_rows_kernel(RowCopies c, int c
 #pragma unroll 2
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
     const int r = (int)(i / units), u = (int)(i - (int64_t)r * units);
-    store_eight(c.dst[z] + i * 8, load_eight_words(c.src[z] + r * c.lds[z] + u * 8, cols - u * 8), 8, true);
+    const Eight e = load_eight_words(c.src[z] + r * c.lds[z] + u * 8, cols - u * 8);
+    *reinterpret_cast<uint4*>(c.dst[z] + i * 8) = *reinterpret_cast<const uint4*>(e.v);
   }
 }
-
-bool aligned16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
 
 template <class... P, class... A>
 void launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t stream, A... args) {
@@ -274,8 +266,8 @@ void launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, cudaStream_
 
 template <int TYPE, bool GATED>
 void grad_of_type(const DenseGrad& g, int chunks, cudaStream_t stream) {
-  bool vec = aligned16(g.dy, g.lddy) && (g.preact == nullptr || ((reinterpret_cast<uintptr_t>(g.preact) & 15u) == 0 && g.ldp % 4 == 0)) && (g.dz == nullptr || aligned16(g.dz, g.ldz));
-  if (GATED) vec = vec && g.N % 8 == 0;
+  const auto aligned = [](const void* p, int bytes, int64_t ld) { return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0 && ld % 4 == 0); };
+  const bool vec = g.N % 4 == 0 && aligned(g.dy, 8, g.lddy) && aligned(g.preact, 16, g.ldp) && aligned(g.dz, 8, g.ldz);
   const dim3 grid((g.N + kGradCols - 1) / kGradCols, chunks);
   const int rows = (g.T + chunks - 1) / chunks;
   if (vec) launch_overlapped(dense_grad_kernel<TYPE, GATED, true>, grid, kGradThreads, stream, g, rows);
@@ -284,10 +276,10 @@ void grad_of_type(const DenseGrad& g, int chunks, cudaStream_t stream) {
 
 }  // namespace
 
-// Chunks of rows: enough for eight CTAs an SM over 256 columns each, of at least 16 rows.
+// Chunks of rows: as many as make the launch three CTAs an SM over 256 columns each, of at least 16 rows.
 int dense_sum_chunks(int T, int n_out) {
   const int across = (n_out + kGradCols - 1) / kGradCols;
-  return std::max(1, std::min((8 * 148 + across - 1) / across, std::min((T + 15) / 16, 128)));
+  return std::max(1, std::min(std::max(1, 3 * 148 / across), (T + kGradStep - 1) / kGradStep));
 }
 
 void launch_dense_simt(const DenseGemm& g, cudaStream_t stream) {
