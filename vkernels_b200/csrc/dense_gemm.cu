@@ -43,7 +43,8 @@ struct WideParams {
   uint16_t* out;
   float* preact;
   int64_t ldr, ldo, ldp;
-  int vec_r, vec_o, vec_p, vec_p2;   // 16-byte accesses possible (vec_p2: the up half of preact)
+  int direct;                 // rows of result and residual start on 16 bytes, those of preact on 32
+  int wide_o;                 // ... and the result's on 32
   int* status;
 };
 
@@ -76,9 +77,65 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   return v;
 }
 __device__ __forceinline__ void sts16(uint32_t addr, uint16_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory"); }
-// rows x cols (at most 32 x 64) of a row-major matrix: a lane holds unit lane % 8 of rows lane / 8, 4 + lane / 8, ... The
-// common case - whole units on 16 bytes - is straight code, all eight accesses in flight at once (with a test at each the
-// loads wait for one another: 10 us instead of 2 for the last tile of a launch with a residual).
+// Rows that start anywhere go through the staging buffer: rows x cols (at most 32 x 64), a row at a time, a value a lane; on the
+// way in, sixteen rows are fetched before the first is put down.
+__device__ __forceinline__ void values_in(uint32_t base, const uint16_t* p, int64_t ld, int rows, int cols, int lane) {
+#pragma unroll 1
+  for (int first = 0; first < 32; first += 16) {
+    uint16_t v[16][2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) v[i][h] = first + i < rows && h * 32 + lane < cols ? p[(int64_t)(first + i) * ld + h * 32 + lane] : (uint16_t)0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) sts16(staging_at(base, first + i, (h * 32 + lane) >> 3) + (lane & 7) * 2, v[i][h]);
+  }
+}
+__device__ __forceinline__ void values_out(uint32_t base, uint16_t* p, int64_t ld, int rows, int cols, int lane) {
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r) {
+    uint16_t* row = p + (int64_t)r * ld;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = h * 32 + lane;
+      uint16_t v;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(staging_at(base, r, c >> 3) + (c & 7) * 2) : "memory");
+      if (c < cols) row[c] = v;
+    }
+  }
+}
+
+// Rows that start on 16 bytes are written from registers: a thread owns a row and takes 16 of its values at a time, 32 bytes, in
+// one access where the row starts on 32 - whole sectors, although neighbouring threads are a row apart. (Through the staging
+// buffer the same bytes cross shared memory twice, which the MMAs need for their operands: 8192 x 7168 -> 2 x 2048 gated 309 us
+// instead of 299, the gradient of the weight of 8192 x 2048 -> 7168 193 instead of 181.)
+__device__ __forceinline__ void stg32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+// n (of 16) 16-bit values.
+__device__ __forceinline__ void row_store(uint16_t* p, const uint32_t (&w)[8], int n, int wide) {
+  if (wide && n >= 16) {
+    stg32(p, w);
+    return;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (n >= h * 8 + 8) {
+      *reinterpret_cast<uint4*>(p + h * 8) = make_uint4(w[h * 4], w[h * 4 + 1], w[h * 4 + 2], w[h * 4 + 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (h * 8 + j < n) p[h * 8 + j] = (uint16_t)(w[h * 4 + (j >> 1)] >> ((j & 1) * 16));
+    }
+  }
+}
+// A residual on 16 bytes is fetched in whole lines, eight threads a row, 64 columns ahead of their use (a lane holds unit lane % 8
+// of rows lane / 8, 4 + lane / 8, ...), and handed to the rows' owners through the staging buffer. (Each owner fetching its own 32
+// bytes a block ahead: 8192 x 7168 -> 2048 173 us instead of 168.)
 struct Piece {
   uint4 v[8];
 };
@@ -98,47 +155,21 @@ __device__ __forceinline__ void piece_to_staging(const Piece& d, uint32_t base, 
   for (int c = cols & ~7; c < cols; ++c)
     if (lane < rows) sts16(staging_at(base, lane, c >> 3) + (c & 7) * 2, p[(int64_t)lane * ld + c]);
 }
-// Rows that start anywhere: a row at a time, a value a lane; sixteen rows on their way before the first is put down.
-__device__ __forceinline__ void values_in(uint32_t base, const uint16_t* p, int64_t ld, int rows, int cols, int lane) {
-#pragma unroll 1
-  for (int first = 0; first < 32; first += 16) {
-    uint16_t v[16][2];
+// n (of 16) fp32 values, p on 32 bytes.
+__device__ __forceinline__ void row_store_f32(float* p, const float (&z)[16], int n) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+  for (int h = 0; h < 2; ++h) {
+    if (n >= h * 8 + 8) {
+      stg32(p + h * 8, reinterpret_cast<const uint32_t*>(&z[h * 8]));
+    } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) v[i][h] = first + i < rows && h * 32 + lane < cols ? p[(int64_t)(first + i) * ld + h * 32 + lane] : (uint16_t)0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) sts16(staging_at(base, first + i, (h * 32 + lane) >> 3) + (lane & 7) * 2, v[i][h]);
-  }
-}
-__device__ __forceinline__ void staging_out(uint32_t base, uint16_t* p, int64_t ld, int rows, int cols, int vec, int lane) {
-  const int r0 = lane >> 3, u = lane & 7;
-  uint16_t* q = p + (int64_t)r0 * ld + u * 8;
-  if (vec && (cols & 7) == 0) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint4 v = lds128(staging_at(base, i * 4 + r0, u));
-      if (i * 4 + r0 < rows && u * 8 < cols) *reinterpret_cast<uint4*>(q + (int64_t)(i * 4) * ld) = v;
-    }
-    return;
-  }
-#pragma unroll 8
-  for (int r = 0; r < rows; ++r) {
-    uint16_t* row = p + (int64_t)r * ld;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = h * 32 + lane;
-      uint16_t v;
-      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(staging_at(base, r, c >> 3) + (c & 7) * 2) : "memory");
-      if (c < cols) row[c] = v;
+      for (int j = 0; j < 8; ++j)
+        if (h * 8 + j < n) p[h * 8 + j] = z[h * 8 + j];
     }
   }
 }
 
-// The epilogue's arithmetic: up to 64 columns of this thread's row, 16 at a time, into its row of the staging buffer. Rolled loops on
-// purpose, and one activation to a copy of the code: unrolled over the columns with the choice of activation inside, the last
+// The epilogue's arithmetic: columns of this thread's row, 16 at a time. Rolled loops on purpose, and one activation to a copy of the code: unrolled over the columns with the choice of activation inside, the last
 // tile of a launch waited 7 us for instructions instead of working 2.
 template <int TYPE>
 __device__ __forceinline__ void load_bias(float (&b)[2], const uint16_t* p, int cols, int lane) {
@@ -157,10 +188,9 @@ __device__ __forceinline__ void load_columns(float (&z)[16], uint32_t taddr) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) z[j] = __uint_as_float(v[j]);
 }
-// The 64 pre-activations of this thread's row to memory in fp32, 32 at a time through the staging buffer.
-__device__ __forceinline__ void preact_columns(uint32_t tz, int width, uint32_t staging, const float (&bias)[2], bool has_bias, float* p, int64_t ld,
-                                               int rows, int cols, int vec, int lane) {
-  const int r0 = lane >> 3, u = lane & 7;
+// Up to 64 pre-activations of this thread's row to rows of memory that start anywhere, 32 at a time through the staging buffer.
+__device__ __forceinline__ void preact_anywhere(uint32_t tz, int width, uint32_t staging, const float (&bias)[2], bool has_bias, float* p,
+                                                int64_t ld, int rows, int cols, int lane) {
 #pragma unroll 1
   for (int part = 0; part * 32 < width; ++part) {
 #pragma unroll 1
@@ -175,40 +205,40 @@ __device__ __forceinline__ void preact_columns(uint32_t tz, int width, uint32_t 
     }
     __syncwarp();
     const int left = min(32, cols - part * 32);
-    float* q = p + part * 32;
-    if (vec && (left & 3) == 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint4 v = lds128(staging_at(staging, i * 4 + r0, u));
-        if (i * 4 + r0 < rows && u * 4 < left) *reinterpret_cast<uint4*>(q + (int64_t)(i * 4 + r0) * ld + u * 4) = v;
-      }
-    } else {   // rows that start anywhere: a row at a time, a value a lane
 #pragma unroll 8
-      for (int r = 0; r < rows; ++r) {
-        float v;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(staging_at(staging, r, lane >> 2) + (lane & 3) * 4) : "memory");
-        if (lane < left) q[(int64_t)r * ld + lane] = v;
-      }
+    for (int r = 0; r < rows; ++r) {
+      float v;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(staging_at(staging, r, lane >> 2) + (lane & 3) * 4) : "memory");
+      if (lane < left) p[(int64_t)r * ld + part * 32 + lane] = v;
     }
     __syncwarp();
   }
 }
-template <int TYPE, int ACT>
-__device__ __forceinline__ void linear_columns(uint32_t tz, int width, uint32_t staging, const float (&bias)[2], bool has_bias, bool residual, int lane) {
+// Where a thread's row starts in the result and the pre-activations (null: not there, or a row behind the last), and how many of
+// the columns exist.
+struct RowPlace {
+  uint16_t* out;
+  float *preact, *preact_up;
+  int cols;
+};
+template <int TYPE, int ACT, bool DIRECT>
+__device__ __forceinline__ void linear_columns(uint32_t tz, int width, uint32_t staging, const float (&bias)[2], bool has_bias, bool residual,
+                                               const RowPlace& at, const WideParams& p, int lane) {
 #pragma unroll 1
   for (int block = 0; block * 16 < width; ++block) {
+    const int n = at.cols - block * 16;
     float z[16];
     load_columns(z, tz + block * 16);
     if (has_bias) add_bias(z, bias, block);
+    if (DIRECT && at.preact) row_store_f32(at.preact + block * 16, z, n);
     if (ACT != kActNone) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) z[j] = dense_act(ACT, z[j]);
     }
+    if (residual) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint32_t at = staging_at(staging, lane, block * 2 + u);
-      if (residual) {
-        const uint4 q = lds128(at);
+      for (int u = 0; u < 2; ++u) {
+        const uint4 q = lds128(staging_at(staging, lane, block * 2 + u));
         const uint32_t r[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -217,18 +247,24 @@ __device__ __forceinline__ void linear_columns(uint32_t tz, int width, uint32_t 
           z[u * 8 + j * 2 + 1] += v.y;
         }
       }
-      uint32_t w[4];
+    }
+    uint32_t w[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = dense_pack<TYPE>(z[u * 8 + j * 2], z[u * 8 + j * 2 + 1]);
-      sts128(at, make_uint4(w[0], w[1], w[2], w[3]));
+    for (int j = 0; j < 8; ++j) w[j] = dense_pack<TYPE>(z[j * 2], z[j * 2 + 1]);
+    if (DIRECT) {
+      if (at.out && n > 0) row_store(at.out + block * 16, w, n, p.wide_o);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) sts128(staging_at(staging, lane, block * 2 + u), make_uint4(w[u * 4], w[u * 4 + 1], w[u * 4 + 2], w[u * 4 + 3]));
     }
   }
 }
-template <int TYPE, int ACT>
+template <int TYPE, int ACT, bool DIRECT>
 __device__ __forceinline__ void gated_columns(uint32_t tg, uint32_t tu, int width, uint32_t staging, const float (&bias_g)[2], const float (&bias_u)[2],
-                                              bool has_bias, const WideParams& p, int lane) {
+                                              bool has_bias, const RowPlace& at, const WideParams& p, int lane) {
 #pragma unroll 1
   for (int block = 0; block * 16 < width; ++block) {
+    const int n = at.cols - block * 16;
     float g[16], u[16];
     load_columns(g, tg + block * 16);
     load_columns(u, tu + block * 16);
@@ -236,17 +272,31 @@ __device__ __forceinline__ void gated_columns(uint32_t tg, uint32_t tu, int widt
       add_bias(g, bias_g, block);
       add_bias(u, bias_u, block);
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = h * 8 + j * 2;
-        w[j] = dense_pack<TYPE>(dense_gated(ACT, g[c], u[c], p.limit, p.beta, p.linear_beta),
-                                dense_gated(ACT, g[c + 1], u[c + 1], p.limit, p.beta, p.linear_beta));
-      }
-      sts128(staging_at(staging, lane, block * 2 + h), make_uint4(w[0], w[1], w[2], w[3]));
+    if (DIRECT && at.preact) {
+      row_store_f32(at.preact + block * 16, g, n);
+      row_store_f32(at.preact_up + block * 16, u, n);
     }
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      w[j] = dense_pack<TYPE>(dense_gated(ACT, g[j * 2], u[j * 2], p.limit, p.beta, p.linear_beta),
+                              dense_gated(ACT, g[j * 2 + 1], u[j * 2 + 1], p.limit, p.beta, p.linear_beta));
+    if (DIRECT) {
+      if (at.out && n > 0) row_store(at.out + block * 16, w, n, p.wide_o);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) sts128(staging_at(staging, lane, block * 2 + h), make_uint4(w[h * 4], w[h * 4 + 1], w[h * 4 + 2], w[h * 4 + 3]));
+    }
+  }
+}
+template <int TYPE, bool DIRECT>
+__device__ __forceinline__ void linear_columns(uint32_t tz, int width, uint32_t staging, const float (&bias)[2], bool has_bias, bool residual,
+                                               const RowPlace& at, const WideParams& p, int lane) {
+  switch (p.act) {
+    case kActSilu: linear_columns<TYPE, kActSilu, DIRECT>(tz, width, staging, bias, has_bias, residual, at, p, lane); break;
+    case kActGelu: linear_columns<TYPE, kActGelu, DIRECT>(tz, width, staging, bias, has_bias, residual, at, p, lane); break;
+    case kActGeluTanh: linear_columns<TYPE, kActGeluTanh, DIRECT>(tz, width, staging, bias, has_bias, residual, at, p, lane); break;
+    default: linear_columns<TYPE, kActNone, DIRECT>(tz, width, staging, bias, has_bias, residual, at, p, lane);
   }
 }
 
@@ -375,82 +425,72 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       const int buf = it & 1;
       const int64_t row0 = (int64_t)tm * 256 + rank * 128 + quad * 32;
       const int rows = (int)min((int64_t)32, (int64_t)p.M - row0);
-      Piece ahead;   // the residual of the coming 64 columns, on its way while the MMAs run
       // the first four warps take the first half of a tile's columns (gated: features), the others the second, up to 64 at a time
       const int tile_cols = GATED ? p.bn / 2 : p.bn, mine = tile_cols / 2, col_first = tn * tile_cols + half * mine;
-      if (!GATED && p.residual && p.vec_r && rows > 0 && col_first < p.N)
+      const int64_t row = row0 + lane;
+      const bool row_ok = lane < rows;
+      Piece ahead;   // the residual of the coming columns, on its way while the MMAs run
+      if (!GATED && p.residual && p.direct && rows > 0 && col_first < p.N)
         piece_load(ahead, p.residual + row0 * p.ldr + col_first, p.ldr, rows, min(min(64, mine), p.N - col_first), lane);
       const bool ready = mbar_wait(smem_u32(&bars->acc_full[buf]), (it >> 1) & 1, abort_flag, 54, 32);
       if (!__all_sync(0xFFFFFFFFu, ready)) break;
       tc_fence_after();
       const uint32_t lanes = tmem_base + buf * 256 + ((uint32_t)(quad * 32) << 16);
-      if constexpr (GATED) {
-        // gate sums at columns half * mine of the accumulator, up sums half a tile on
-        const int col0 = col_first, cols = min(mine, p.N - col0);
-        const uint32_t tg = lanes + half * mine, tu = tg + tile_cols;
-        const bool any = rows > 0 && cols > 0;
-        const bool has_bias = p.bias != nullptr && any;
-        float bias_g[2] = {}, bias_u[2] = {};
+#pragma unroll 1
+      for (int first = 0; first < mine; first += 64) {
+        const int width = min(64, mine - first), col0 = col_first + first, cols = min(width, p.N - col0);
+        const bool any = rows > 0 && cols > 0, last = first + 64 >= mine, has_bias = p.bias != nullptr && any;
+        const uint32_t tz = lanes + half * mine + first, tu = tz + tile_cols;   // gated: gate sums, up sums half a tile on
+        float bias[2] = {}, bias_u[2] = {};
         if (has_bias) {
-          load_bias<TYPE>(bias_g, p.bias + col0, cols, lane);
-          load_bias<TYPE>(bias_u, p.bias + p.N + col0, cols, lane);
-        }
-        if (p.preact && any) {
-#pragma unroll 1
-          for (int part = 0; part < 2; ++part) {
-            const float b[2] = {part ? bias_u[0] : bias_g[0], part ? bias_u[1] : bias_g[1]};
-            preact_columns(part ? tu : tg, mine, staging, b, has_bias, p.preact + row0 * p.ldp + (part ? p.N : 0) + col0, p.ldp, rows, cols,
-                           part ? p.vec_p2 : p.vec_p, lane);
-          }
+          load_bias<TYPE>(bias, p.bias + col0, cols, lane);
+          if (GATED) load_bias<TYPE>(bias_u, p.bias + p.N + col0, cols, lane);
         }
         if (any) {
-          if (p.act == 1) gated_columns<TYPE, 1>(tg, tu, mine, staging, bias_g, bias_u, has_bias, p, lane);
-          else gated_columns<TYPE, 0>(tg, tu, mine, staging, bias_g, bias_u, has_bias, p, lane);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cta(smem_u32(&bars->acc_empty[buf]), 0);
-        if (any) {
-          staging_out(staging, p.out + row0 * p.ldo + col0, p.ldo, rows, cols, p.vec_o, lane);
-          __syncwarp();
-        }
-      } else {
-#pragma unroll 1
-        for (int at = 0; at < mine; at += 64) {
-          const int width = min(64, mine - at), col0 = col_first + at, cols = min(width, p.N - col0);
-          const uint32_t tz = lanes + half * mine + at;
-          const bool any = rows > 0 && cols > 0, last = at + 64 >= mine;
-          const bool has_bias = p.bias != nullptr && any;
-          float bias[2] = {};
-          if (has_bias) load_bias<TYPE>(bias, p.bias + col0, cols, lane);
-          if (p.preact && any) preact_columns(tz, width, staging, bias, has_bias, p.preact + row0 * p.ldp + col0, p.ldp, rows, cols, p.vec_p, lane);
-          if (p.residual && any) {
-            if (p.vec_r) {
-              piece_to_staging(ahead, staging, p.residual + row0 * p.ldr + col0, p.ldr, rows, cols, lane);
-              if (!last && col0 + 64 < p.N)
-                piece_load(ahead, p.residual + row0 * p.ldr + col0 + 64, p.ldr, rows, min(min(64, mine - at - 64), p.N - col0 - 64), lane);
+          RowPlace at{};
+          at.cols = cols;
+          if (p.direct) {
+            if (row_ok) {
+              at.out = p.out + row * p.ldo + col0;
+              if (p.preact) {
+                at.preact = p.preact + row * p.ldp + col0;
+                at.preact_up = at.preact + p.N;
+              }
+            }
+            if constexpr (GATED) {
+              if (p.act == 1) gated_columns<TYPE, 1, true>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
+              else gated_columns<TYPE, 0, true>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
             } else {
+              if (p.residual) {
+                piece_to_staging(ahead, staging, p.residual + row0 * p.ldr + col0, p.ldr, rows, cols, lane);
+                if (!last && col0 + 64 < p.N)
+                  piece_load(ahead, p.residual + row0 * p.ldr + col0 + 64, p.ldr, rows, min(min(64, mine - first - 64), p.N - col0 - 64), lane);
+                __syncwarp();
+              }
+              linear_columns<TYPE, true>(tz, width, staging, bias, has_bias, p.residual != nullptr, at, p, lane);
+            }
+          } else {
+            if (p.preact) {
+              preact_anywhere(tz, width, staging, bias, has_bias, p.preact + row0 * p.ldp + col0, p.ldp, rows, cols, lane);
+              if (GATED) preact_anywhere(tu, width, staging, bias_u, has_bias, p.preact + row0 * p.ldp + p.N + col0, p.ldp, rows, cols, lane);
+            }
+            if (!GATED && p.residual) {
               values_in(staging, p.residual + row0 * p.ldr + col0, p.ldr, rows, cols, lane);
+              __syncwarp();
+            }
+            if constexpr (GATED) {
+              if (p.act == 1) gated_columns<TYPE, 1, false>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
+              else gated_columns<TYPE, 0, false>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
+            } else {
+              linear_columns<TYPE, false>(tz, width, staging, bias, has_bias, p.residual != nullptr, at, p, lane);
             }
             __syncwarp();
-          }
-          if (any) {
-            const bool res = p.residual != nullptr;
-            switch (p.act) {
-              case kActSilu: linear_columns<TYPE, kActSilu>(tz, width, staging, bias, has_bias, res, lane); break;
-              case kActGelu: linear_columns<TYPE, kActGelu>(tz, width, staging, bias, has_bias, res, lane); break;
-              case kActGeluTanh: linear_columns<TYPE, kActGeluTanh>(tz, width, staging, bias, has_bias, res, lane); break;
-              default: linear_columns<TYPE, kActNone>(tz, width, staging, bias, has_bias, res, lane);
-            }
-          }
-          if (last) tc_fence_before();
-          __syncwarp();
-          if (last && lane == 0) mbar_arrive_cta(smem_u32(&bars->acc_empty[buf]), 0);
-          if (any) {
-            staging_out(staging, p.out + row0 * p.ldo + col0, p.ldo, rows, cols, p.vec_o, lane);
-            __syncwarp();
+            values_out(staging, p.out + row0 * p.ldo + col0, p.ldo, rows, cols, lane);
           }
         }
+        if (last) tc_fence_before();
+        __syncwarp();
+        if (last && lane == 0) mbar_arrive_cta(smem_u32(&bars->acc_empty[buf]), 0);
       }
     }
   }
@@ -481,16 +521,19 @@ struct WidePlan {
   int bn;
   float us;
 };
-WidePlan plan_wide(int64_t M, int64_t N, int64_t K, bool gated) {
+WidePlan plan_wide(int64_t M, int64_t N, int64_t K, bool gated, bool b_mn) {
   const int64_t pairs = sm_count() / 2, tiles_m = (M + 255) / 256, blocks = (K + 63) / 64;
   WidePlan best{256, 1e30f};
   for (int bn = 256; bn >= 64; bn -= 32) {
     const int64_t tile_n = gated ? bn / 2 : bn, tiles = tiles_m * ((N + tile_n - 1) / tile_n);
-    const float waves = (float)((tiles + pairs - 1) / pairs), narrower = (float)(256 - bn) / 64.0f;
+    // the last wave of many: half of what its idle pairs leave undone comes back as clock and bandwidth for the others
+    const float full = (float)tiles / (float)pairs, waves = full <= 1.0f ? 1.0f : 0.5f * (full + (float)((tiles + pairs - 1) / pairs));
+    const float narrower = (float)(256 - bn) / 64.0f;
     const float block_us = bn >= 128 ? 0.024f + 0.001f * (float)bn : 0.144f + 0.0001f * (float)bn;
     const float ends_us = bn >= 128 ? 3.4f + 0.0148f * (float)bn : 5.4f;
     // the more pairs are at work, the slower the narrower tiles, which bring more bytes for a product
-    const float load = 1.0f + 0.06f * narrower * (waves > 1.0f ? 1.0f : (float)tiles / (float)pairs);
+    float load = 1.0f + 0.06f * narrower * (full > 1.0f ? 1.0f : full);
+    if (b_mn && bn % 128 != 0) load *= 1.05f;   // B comes in boxes of 64 columns a CTA, some of them for nothing
     const float us = ends_us + waves * ((float)blocks * block_us * load) + (waves - 1.0f) * 1.0f;
     if (us < best.us) best = {bn, us};
   }
@@ -512,7 +555,7 @@ void launch_wide(const DenseGemm& g, cudaStream_t stream) {
   p.K = g.K;
   p.a_mn = g.a.mn_major;
   p.b_mn = g.b.mn_major;
-  p.bn = plan_wide(g.M, g.N, g.K, GATED).bn;
+  p.bn = plan_wide(g.M, g.N, g.K, GATED, g.b.mn_major).bn;
   p.stage_bytes = 16384 + (g.b.mn_major ? (p.bn > 128 ? 16384 : 8192) : p.bn * 64);
   const int tile_n = GATED ? p.bn / 2 : p.bn;
   p.tiles_m = (g.M + 255) / 256;
@@ -531,10 +574,11 @@ void launch_wide(const DenseGemm& g, cudaStream_t stream) {
   p.ldr = g.ldr;
   p.ldo = g.ldo;
   p.ldp = g.ldp;
-  p.vec_r = g.residual != nullptr && aligned16(g.residual, g.ldr);
-  p.vec_o = aligned16(g.out, g.ldo);
-  p.vec_p = (reinterpret_cast<uintptr_t>(g.preact) & 15u) == 0 && g.ldp % 4 == 0;
-  p.vec_p2 = p.vec_p && g.N % 4 == 0;
+  const auto on = [](const void* q, int64_t ld_bytes, int bytes) { return ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)ld_bytes) & (uintptr_t)(bytes - 1)) == 0; };
+  p.direct = on(g.out, g.ldo * 2, 16) && (g.residual == nullptr || on(g.residual, g.ldr * 2, 16)) &&
+             (g.preact == nullptr || (on(g.preact, g.ldp * 4, 32) && (!GATED || g.N % 8 == 0)));
+  const bool whole = (GATED ? p.bn / 4 : p.bn / 2) % 16 == 0;   // every warp's columns start on 32 bytes of a row that does
+  p.wide_o = whole && on(g.out, g.ldo * 2, 32);
   p.status = status_address();
   const CUtensorMap a = operand_map(g.a, g.M, g.K, 128), b = operand_map(g.b, GATED ? 2 * (int64_t)g.N : g.N, g.K, p.bn / 2);
   const int units = min(p.n_tiles, sm_count() / 2);
@@ -552,7 +596,7 @@ void launch_wide(const DenseGemm& g, cudaStream_t stream) {
 
 }  // namespace
 
-float dense_wide_us(const DenseGemm& g) { return plan_wide(g.M, g.N, g.K, g.gated).us; }
+float dense_wide_us(const DenseGemm& g) { return plan_wide(g.M, g.N, g.K, g.gated, g.b.mn_major).us; }
 
 void launch_dense_wide(const DenseGemm& g, cudaStream_t stream) {
   if (g.type == kDenseBf16) {

@@ -42,8 +42,6 @@ __device__ __forceinline__ uint32_t operand_idesc(int m, int n, int a_mn, int b_
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-bool aligned16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
-
 int* status_address() {
   static std::atomic<int*> known[64];
   int dev = 0;
