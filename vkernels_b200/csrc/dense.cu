@@ -165,7 +165,9 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
     g.ldp = f.ldp;
     g.dz = dz;
     g.ldz = ldz;
-    g.partial = partial;
+    const int chunks = dense_sum_chunks(f.T, f.n_out);
+    g.partial = chunks > 1 ? partial : nullptr;
+    g.db = chunks > 1 ? nullptr : f.db;
     g.T = f.T;
     g.N = f.n_out;
     g.gated = f.gated;
@@ -174,33 +176,38 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
     g.beta = f.beta;
     g.linear_beta = f.linear_beta;
     launch_dense_grad(g, stream);
-    if (f.db) launch_dense_sum(f.type, partial, dense_sum_chunks(f.T, f.n_out), rows, f.db, stream);
+    if (f.db && chunks > 1) launch_dense_sum(f.type, partial, chunks, rows, f.db, stream);
   }
   const uint16_t* z = need_dz ? dz : f.dy;
   const int64_t ldzz = need_dz ? ldz : f.lddy;
-  DenseGemm g{};
-  g.type = f.type;
-  g.limit = INFINITY;
+  DenseGemm gx{}, gw{};
+  gx.type = gw.type = f.type;
+  gx.limit = gw.limit = INFINITY;
   if (f.dx) {   // dx[t, i] = sum_n dz[t, n] w[n, i]
-    g.a = {z, ldzz, false};
-    g.b = {w, ldw, true};
-    g.M = f.T;
-    g.N = f.n_in;
-    g.K = rows;
-    g.out = f.dx;
-    g.ldo = f.lddx;
-    launch_dense_gemm(g, stream);
+    gx.a = {z, ldzz, false};
+    gx.b = {w, ldw, true};
+    gx.M = f.T;
+    gx.N = f.n_in;
+    gx.K = rows;
+    gx.out = f.dx;
+    gx.ldo = f.lddx;
   }
   if (f.dw) {   // dw[n, i] = sum_t dz[t, n] x[t, i]
-    g.a = {z, ldzz, true};
-    g.b = {x, ldx, true};
-    g.M = rows;
-    g.N = f.n_in;
-    g.K = f.T;
-    g.out = f.dw;
-    g.ldo = f.lddw;
-    launch_dense_gemm(g, stream);
+    gw.a = {z, ldzz, true};
+    gw.b = {x, ldx, true};
+    gw.M = rows;
+    gw.N = f.n_in;
+    gw.K = f.T;
+    gw.out = f.dw;
+    gw.ldo = f.lddw;
   }
+  // both in one launch: the tiles of one fill what the other leaves idle (1001 tokens, 1504 -> 2 x 1024: 21.3 us as two)
+  if (f.dx && f.dw && get_moe_impl() != MoeImpl::kSimt) {
+    launch_dense_wide_two(gx, gw, stream);
+    return;
+  }
+  if (f.dx) launch_dense_gemm(gx, stream);
+  if (f.dw) launch_dense_gemm(gw, stream);
 }
 
 }  // namespace vkernels::kernels::cuda

@@ -41,7 +41,7 @@ struct DenseGemm {
 
 // Gradient of the pre-activations: dz = dy * act'(z), [T, rows] (linear) or [T, 2 ispp] (gated) at pitch ldz; with no
 // activation a copy of dy. dz may be null (only the column sums are wanted). partial (optional) receives the column sums of
-// each chunk of rows in fp32, [dense_sum_chunks(T, N), rows].
+// each chunk of rows in fp32, [dense_sum_chunks(T, N), rows]; of a single chunk db receives them at once, in the type.
 struct DenseGrad {
   DenseType type;
   const uint16_t* dy;
@@ -51,6 +51,7 @@ struct DenseGrad {
   uint16_t* dz;
   int64_t ldz;
   float* partial;
+  uint16_t* db;
   int T, N;                   // N: columns of dy; the gated form has 2 N columns of dz
   bool gated;
   int act;
@@ -60,6 +61,7 @@ struct DenseGrad {
 int dense_sum_chunks(int T, int n_out);
 void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_wide(const DenseGemm& g, cudaStream_t stream);   // dense_gemm.cu
+void launch_dense_wide_two(const DenseGemm& g, const DenseGemm& h, cudaStream_t stream);
 void launch_dense_narrow(const DenseGemm& g, cudaStream_t stream);  // dense_narrow.cu
 float dense_wide_us(const DenseGemm& g);      // the time that either is expected to take
 float dense_narrow_us(const DenseGemm& g);

@@ -11,6 +11,9 @@
 // (staged by its peer): an epilogue thread finds a feature's gate and up sums 128 columns apart in its own lane.
 #include <atomic>
 
+#include <algorithm>
+#include <cmath>
+
 #include "dense_tc.cuh"
 
 namespace vkernels::kernels::cuda {
@@ -30,8 +33,8 @@ struct WideBars {
 };
 constexpr int kWideSmem = kStages * kStageBytes + kEpiWarps * kStagingBytes + (int)sizeof(WideBars) + 1024;
 
-struct WideParams {
-  int M, N, K;                // N: columns of the result (gated: features)
+struct WideParams {           // one product
+  int M, N;                   // N: columns of the result (gated: features)
   int a_mn, b_mn;
   int bn;                     // rows of B a tile: a multiple of 32 from 64 to 256
   int stage_bytes;            // of one CTA: what the copies of a stage bring
@@ -45,6 +48,12 @@ struct WideParams {
   int64_t ldr, ldo, ldp;
   int direct;                 // rows of result and residual start on 16 bytes, those of preact on 32
   int wide_o;                 // ... and the result's on 32
+};
+template <int COUNT>
+struct WideLaunch {           // one product, or two that do not depend on each other: the tiles of the second follow the first's
+  CUtensorMap a[COUNT], b[COUNT];
+  WideParams p[COUNT];
+  int n_tiles;                // of both
   int* status;
 };
 
@@ -300,9 +309,9 @@ __device__ __forceinline__ void linear_columns(uint32_t tz, int width, uint32_t 
   }
 }
 
-template <int TYPE, bool GATED>
+template <int TYPE, bool GATED, int COUNT>
 __global__ void __cluster_dims__(2) __launch_bounds__(kThreads, 1)
-dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const WideParams p) {
+dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t ring = smem_u32(smem);
@@ -335,11 +344,15 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   const uint32_t tmem_base = bars->tmem_base;
   wait_for_earlier_kernels();
   const int unit = blockIdx.x >> 1, n_units = gridDim.x >> 1;
-  const int per_group = kGroupM * p.tiles_n;
+  // which product tile t belongs to, and where it lies there
   const auto place = [&](int t, int& tm, int& tn) {
-    const int first = t / per_group * kGroupM, in = t % per_group, high = min(kGroupM, p.tiles_m - first);
+    const int which = COUNT > 1 && t >= work.p[0].n_tiles;
+    const WideParams& p = work.p[which];
+    if (which) t -= work.p[0].n_tiles;
+    const int per_group = kGroupM * p.tiles_n, first = t / per_group * kGroupM, in = t % per_group, high = min(kGroupM, p.tiles_m - first);
     tm = first + in % high;
     tn = in / high;
+    return which;
   };
 
   if (warp == kEpiWarps) {
@@ -348,29 +361,33 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       Ring s;
       long long issued = 0;
       bool go = true;
-      for (int t = unit; t < p.n_tiles && go; t += n_units) {
+      for (int t = unit; t < work.n_tiles && go; t += n_units) {
         int tm, tn;
-        place(t, tm, tn);
+        const int which = place(t, tm, tn);
+        const WideParams& p = work.p[which];
+        const CUtensorMap *map_a = &work.a[which], *map_b = &work.b[which];
+        // kept in registers: of two products, each look into the parameters would be an indexed load
+        const int a_mn = p.a_mn, b_mn = p.b_mn, b_wide = p.bn > 128, k_blocks = p.k_blocks, pair_bytes = 2 * p.stage_bytes;
         const int m0 = tm * 256 + (int)rank * 128;
         const int n0 = GATED ? tn * (p.bn / 2) + (int)rank * p.N : tn * p.bn + (int)rank * (p.bn / 2);
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
+        for (int kb = 0; kb < k_blocks; ++kb) {
           const uint32_t full = smem_u32(&bars->full[s.slot]), dst = ring + s.slot * kStageBytes;
           if (!mbar_wait(smem_u32(&bars->empty[s.slot]), s.phase ^ 1u, abort_flag, 51)) {
             go = false;
             break;
           }
-          if (rank == 0) mbar_expect_tx(full, 2 * p.stage_bytes);
-          if (p.a_mn) {
-            tma_load_2d_pair(dst, &map_a, m0, kb * 64, full);
-            tma_load_2d_pair(dst + 8192, &map_a, m0 + 64, kb * 64, full);
+          if (rank == 0) mbar_expect_tx(full, pair_bytes);
+          if (a_mn) {
+            tma_load_2d_pair(dst, map_a, m0, kb * 64, full);
+            tma_load_2d_pair(dst + 8192, map_a, m0 + 64, kb * 64, full);
           } else {
-            tma_load_2d_pair(dst, &map_a, kb * 64, m0, full);
+            tma_load_2d_pair(dst, map_a, kb * 64, m0, full);
           }
-          if (p.b_mn) {
-            tma_load_2d_pair(dst + 16384, &map_b, n0, kb * 64, full);
-            if (p.bn > 128) tma_load_2d_pair(dst + 24576, &map_b, n0 + 64, kb * 64, full);
+          if (b_mn) {
+            tma_load_2d_pair(dst + 16384, map_b, n0, kb * 64, full);
+            if (b_wide) tma_load_2d_pair(dst + 24576, map_b, n0 + 64, kb * 64, full);
           } else {
-            tma_load_2d_pair(dst + 16384, &map_b, kb * 64, n0, full);
+            tma_load_2d_pair(dst + 16384, map_b, kb * 64, n0, full);
           }
           ++issued;
           s.advance(kStages);
@@ -387,24 +404,26 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   } else if (warp == kEpiWarps + 1) {
     // -------------------------------- MMAs ----------------------------------
     if (rank == 0 && elect_one()) {
-      const uint32_t idesc = operand_idesc<TYPE>(256, p.bn, p.a_mn, p.b_mn);
-      const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;   // 16 k on
       Ring s;
       int it = 0;
       bool go = true;
-      for (int t = unit; t < p.n_tiles && go; t += n_units, ++it) {
+      for (int t = unit; t < work.n_tiles && go; t += n_units, ++it) {
+        const WideParams& p = work.p[COUNT > 1 && t >= work.p[0].n_tiles];
+        const int a_mn = p.a_mn, b_mn = p.b_mn, k_blocks = p.k_blocks;
+        const uint32_t idesc = operand_idesc<TYPE>(256, p.bn, a_mn, b_mn);
+        const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;   // 16 k on
         const int buf = it & 1;
         if (!mbar_wait(smem_u32(&bars->acc_empty[buf]), ((it >> 1) & 1) ^ 1, abort_flag, 52)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + buf * 256;
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
+        for (int kb = 0; kb < k_blocks; ++kb) {
           if (!mbar_wait(smem_u32(&bars->full[s.slot]), s.phase, abort_flag, 53)) {
             go = false;
             break;
           }
           tc_fence_after();
           const uint32_t src = ring + s.slot * kStageBytes;
-          const uint64_t ad = operand_desc(src, p.a_mn), bd = operand_desc(src + 16384, p.b_mn);
+          const uint64_t ad = operand_desc(src, a_mn), bd = operand_desc(src + 16384, b_mn);
 #pragma unroll
           for (int k = 0; k < 4; ++k) tc_mma_ss_pair(d, ad + k * a_step, bd + k * b_step, idesc, (kb | k) != 0);
           tc_commit_pair(smem_u32(&bars->empty[s.slot]));
@@ -419,9 +438,9 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const int quad = warp & 3, half = warp >> 2;
     const uint32_t staging = ring + kStages * kStageBytes + warp * kStagingBytes;
     int it = 0;
-    for (int t = unit; t < p.n_tiles; t += n_units, ++it) {
+    for (int t = unit; t < work.n_tiles; t += n_units, ++it) {
       int tm, tn;
-      place(t, tm, tn);
+      const WideParams& p = work.p[place(t, tm, tn)];
       const int buf = it & 1;
       const int64_t row0 = (int64_t)tm * 256 + rank * 128 + quad * 32;
       const int rows = (int)min((int64_t)32, (int64_t)p.M - row0);
@@ -503,7 +522,7 @@ dense_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
   }
-  if (tid == 0 && bars->abort_flag != 0) atomicExch(p.status, 100 + bars->abort_flag);
+  if (tid == 0 && bars->abort_flag != 0) atomicExch(work.status, 100 + bars->abort_flag);
 }
 
 // A tensor map of one operand: boxes of 64 values along the contiguous index by `box` (k contiguous) or 64 rows.
@@ -517,50 +536,57 @@ CUtensorMap operand_map(const DenseOperand& o, int64_t rows, int K, int box) {
 // bringing A) and what comes before and after them. Measured on 2880 -> 2880, widths 256, 192, 128 and 64: 512 tokens 20.1, 17.6,
 // 13.4 and 19.1 us, 1024 tokens 22.3, 18.4, 21.2 and 27.0, 2047 tokens 35.2, 29.3, 30.4 and 43.3; with many waves the widest is
 // best or within 4 % of it (8192 tokens 101.5, 97.9, 108.5, 161.1; 8192 x 7168 -> 2048 170, 175, 193, 296).
+//
+// Two products in one launch (the gradients of x and of the weight): a pair's share is worked out for both together, tiles dealt
+// out one after the other.
 struct WidePlan {
-  int bn;
+  int bn[2];
   float us;
 };
-WidePlan plan_wide(int64_t M, int64_t N, int64_t K, bool gated, bool b_mn) {
-  const int64_t pairs = sm_count() / 2, tiles_m = (M + 255) / 256, blocks = (K + 63) / 64;
-  WidePlan best{256, 1e30f};
+float tile_us(const DenseGemm& g, int bn, float load) {
+  const float block_us = bn >= 128 ? 0.024f + 0.001f * (float)bn : 0.144f + 0.0001f * (float)bn;
+  // the more pairs are at work, the slower the narrower tiles, which bring more bytes for a product
+  load = 1.0f + 0.06f * (float)(256 - bn) / 64.0f * load;
+  if (g.b.mn_major && bn % 128 != 0) load *= 1.05f;   // B comes in boxes of 64 columns a CTA, some of them for nothing
+  return (float)((g.K + 63) / 64) * block_us * load + 1.0f;
+}
+int64_t count_tiles(const DenseGemm& g, int bn) {
+  const int64_t tile_n = g.gated ? bn / 2 : bn;
+  return ((int64_t)g.M + 255) / 256 * ((g.N + tile_n - 1) / tile_n);
+}
+WidePlan plan_wide(const DenseGemm* g, int count) {
+  const int64_t pairs = sm_count() / 2;
+  WidePlan best{{256, 256}, 1e30f};
   for (int bn = 256; bn >= 64; bn -= 32) {
-    const int64_t tile_n = gated ? bn / 2 : bn, tiles = tiles_m * ((N + tile_n - 1) / tile_n);
-    // the last wave of many: half of what its idle pairs leave undone comes back as clock and bandwidth for the others
-    const float full = (float)tiles / (float)pairs, waves = full <= 1.0f ? 1.0f : 0.5f * (full + (float)((tiles + pairs - 1) / pairs));
-    const float narrower = (float)(256 - bn) / 64.0f;
-    const float block_us = bn >= 128 ? 0.024f + 0.001f * (float)bn : 0.144f + 0.0001f * (float)bn;
-    const float ends_us = bn >= 128 ? 3.4f + 0.0148f * (float)bn : 5.4f;
-    // the more pairs are at work, the slower the narrower tiles, which bring more bytes for a product
-    float load = 1.0f + 0.06f * narrower * (full > 1.0f ? 1.0f : full);
-    if (b_mn && bn % 128 != 0) load *= 1.05f;   // B comes in boxes of 64 columns a CTA, some of them for nothing
-    const float us = ends_us + waves * ((float)blocks * block_us * load) + (waves - 1.0f) * 1.0f;
-    if (us < best.us) best = {bn, us};
+    const int64_t n0 = count_tiles(g[0], bn), q0 = n0 / pairs, r0 = n0 % pairs;
+    for (int other = 256; other >= (count > 1 ? 64 : 256); other -= 32) {
+      const int64_t n1 = count > 1 ? count_tiles(g[1], other) : 0, q1 = n1 / pairs, r1 = n1 % pairs;
+      const float full = (float)(n0 + n1) / (float)pairs, load = full < 1.0f ? full : 1.0f;
+      const float c0 = tile_us(g[0], bn, load), c1 = count > 1 ? tile_us(g[1], other, load) : 0.0f;
+      // the busiest pair: one with a tile more of the first (and of the second, if those come round), or of the second alone
+      float most = r0 > 0 ? (float)(q0 + 1) * c0 + (float)(r0 + r1 > pairs ? q1 + 1 : q1) * c1 : (float)q0 * c0 + (float)q1 * c1;
+      if (r1 > 0) most = fmaxf(most, (float)q0 * c0 + (float)(q1 + 1) * c1);
+      // of many waves, half of what idle pairs leave undone in the last comes back as clock and bandwidth for the others
+      const float mean = ((float)n0 * c0 + (float)n1 * c1) / (float)pairs;
+      const float us = (bn >= 128 ? 2.4f + 0.0148f * (float)bn : 4.4f) + (full > 1.0f ? 0.5f * (most + mean) : most);
+      if (us < best.us) best = {{bn, other}, us};
+    }
   }
   return best;
 }
 
-template <int TYPE, bool GATED>
-void launch_wide(const DenseGemm& g, cudaStream_t stream) {
-  static std::atomic<bool> configured[64];
-  int dev = 0;
-  VK_CUDA_CHECK(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || !configured[dev].load()) {
-    VK_CUDA_CHECK(cudaFuncSetAttribute(dense_wide_kernel<TYPE, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem));
-    if (dev >= 0 && dev < 64) configured[dev].store(true);
-  }
-  WideParams p{};
+template <bool GATED>
+void describe(const DenseGemm& g, int bn, WideParams& p, CUtensorMap& a, CUtensorMap& b) {
   p.M = g.M;
   p.N = g.N;
-  p.K = g.K;
   p.a_mn = g.a.mn_major;
   p.b_mn = g.b.mn_major;
-  p.bn = plan_wide(g.M, g.N, g.K, GATED, g.b.mn_major).bn;
+  p.bn = bn;
   p.stage_bytes = 16384 + (g.b.mn_major ? (p.bn > 128 ? 16384 : 8192) : p.bn * 64);
   const int tile_n = GATED ? p.bn / 2 : p.bn;
   p.tiles_m = (g.M + 255) / 256;
   p.tiles_n = (g.N + tile_n - 1) / tile_n;
-  expects((int64_t)p.tiles_m * p.tiles_n < (1ll << 30), "dense product: more than 2^30 tiles");
+  expects((int64_t)p.tiles_m * p.tiles_n < (1ll << 29), "dense product: more than 2^29 tiles");
   p.n_tiles = p.tiles_m * p.tiles_n;
   p.k_blocks = (g.K + 63) / 64;
   p.act = g.act;
@@ -579,9 +605,27 @@ void launch_wide(const DenseGemm& g, cudaStream_t stream) {
              (g.preact == nullptr || (on(g.preact, g.ldp * 4, 32) && (!GATED || g.N % 8 == 0)));
   const bool whole = (GATED ? p.bn / 4 : p.bn / 2) % 16 == 0;   // every warp's columns start on 32 bytes of a row that does
   p.wide_o = whole && on(g.out, g.ldo * 2, 32);
-  p.status = status_address();
-  const CUtensorMap a = operand_map(g.a, g.M, g.K, 128), b = operand_map(g.b, GATED ? 2 * (int64_t)g.N : g.N, g.K, p.bn / 2);
-  const int units = min(p.n_tiles, sm_count() / 2);
+  a = operand_map(g.a, g.M, g.K, 128);
+  b = operand_map(g.b, GATED ? 2 * (int64_t)g.N : g.N, g.K, p.bn / 2);
+}
+
+template <int TYPE, bool GATED, int COUNT>
+void launch_wide(const DenseGemm* g, cudaStream_t stream) {
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  VK_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !configured[dev].load()) {
+    VK_CUDA_CHECK(cudaFuncSetAttribute(dense_wide_kernel<TYPE, GATED, COUNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem));
+    if (dev >= 0 && dev < 64) configured[dev].store(true);
+  }
+  const WidePlan plan = plan_wide(g, COUNT);
+  WideLaunch<COUNT> work{};
+  for (int i = 0; i < COUNT; ++i) {
+    describe<GATED>(g[i], plan.bn[i], work.p[i], work.a[i], work.b[i]);
+    work.n_tiles += work.p[i].n_tiles;
+  }
+  work.status = status_address();
+  const int units = std::min(work.n_tiles, sm_count() / 2);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(2 * units));
   cfg.blockDim = dim3(kThreads);
@@ -591,21 +635,28 @@ void launch_wide(const DenseGemm& g, cudaStream_t stream) {
   overlap_launch(attr[0]);
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  VK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, dense_wide_kernel<TYPE, GATED>, a, b, p));
+  VK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, dense_wide_kernel<TYPE, GATED, COUNT>, work));
 }
 
 }  // namespace
 
-float dense_wide_us(const DenseGemm& g) { return plan_wide(g.M, g.N, g.K, g.gated, g.b.mn_major).us; }
+float dense_wide_us(const DenseGemm& g) { return plan_wide(&g, 1).us; }
 
 void launch_dense_wide(const DenseGemm& g, cudaStream_t stream) {
   if (g.type == kDenseBf16) {
-    if (g.gated) launch_wide<kDenseBf16, true>(g, stream);
-    else launch_wide<kDenseBf16, false>(g, stream);
+    if (g.gated) launch_wide<kDenseBf16, true, 1>(&g, stream);
+    else launch_wide<kDenseBf16, false, 1>(&g, stream);
   } else {
-    if (g.gated) launch_wide<kDenseFp16, true>(g, stream);
-    else launch_wide<kDenseFp16, false>(g, stream);
+    if (g.gated) launch_wide<kDenseFp16, true, 1>(&g, stream);
+    else launch_wide<kDenseFp16, false, 1>(&g, stream);
   }
+}
+
+// Two linear products that do not depend on each other, in one launch; the one with the longer tiles goes first.
+void launch_dense_wide_two(const DenseGemm& g, const DenseGemm& h, cudaStream_t stream) {
+  const DenseGemm two[2] = {g.K >= h.K ? g : h, g.K >= h.K ? h : g};
+  if (g.type == kDenseBf16) launch_wide<kDenseBf16, false, 2>(two, stream);
+  else launch_wide<kDenseFp16, false, 2>(two, stream);
 }
 
 }  // namespace vkernels::kernels::cuda

@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g
       }
     }
   }
-  if (g.partial == nullptr) return;
+  if (g.partial == nullptr && g.db == nullptr) return;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     sums[0][sub][column(j)] = sg[j];
@@ -196,7 +196,8 @@ __global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) s += sums[h][i][threadIdx.x];
-    g.partial[(int64_t)blockIdx.y * rows + h * g.N + col] = s;
+    if (g.db) g.db[h * g.N + col] = dense_from_f32<TYPE>(s);
+    else g.partial[(int64_t)blockIdx.y * rows + h * g.N + col] = s;
   }
 }
 
@@ -276,8 +277,10 @@ void grad_of_type(const DenseGrad& g, int chunks, cudaStream_t stream) {
 
 }  // namespace
 
-// Chunks of rows: as many as make the launch three CTAs an SM over 256 columns each, of at least 16 rows.
+// Chunks of rows: as many as make the launch three CTAs an SM over 256 columns each, of at least 16 rows; one, whose sums need no
+// further kernel, up to 64 rows.
 int dense_sum_chunks(int T, int n_out) {
+  if (T <= 64) return 1;
   const int across = (n_out + kGradCols - 1) / kGradCols;
   return std::max(1, std::min(std::max(1, 3 * 148 / across), (T + kGradStep - 1) / kGradStep));
 }
