@@ -58,25 +58,26 @@ def _plain(t, shape, dtype, index):
     return t.shape == shape and t.dtype is dtype and t.get_device() == index and t.is_contiguous() and not t.data_ptr() & 15
 
 
-def _check(name, t, dtype, device):
+def _check(name, t, dtype, index):
     if not isinstance(t, torch.Tensor):
         raise OpNotEligible(f"{name} must be a tensor")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise OpNotEligible(f"{name} must be {dtype}, like the other tensors of the call, got {t.dtype}")
-    if t.device != device:
-        raise OpNotEligible(f"{name} must be on {device}, got {t.device}")
+    if t.get_device() != index:
+        raise OpNotEligible(f"{name} must be on the device of x, got {t.device}")
 
 
 def _pitch(name, t):
     """Elements from one row of a 2-D tensor to the next."""
     T, n = t.shape
-    if n > 1 and t.stride(1) != 1:
+    row, step = t.stride()
+    if n > 1 and step != 1:
         raise OpNotEligible(f"the values of a row of {name} must be neighbours in memory")
     if T <= 1:
         return (n + 7) // 8 * 8
-    if t.stride(0) < n:
+    if row < n:
         raise OpNotEligible(f"the rows of {name} must not overlap")
-    return t.stride(0)
+    return row
 
 
 def _span(t):
@@ -113,15 +114,16 @@ def _inputs(x, w, gated, what):
         raise OpNotEligible(f"{what}: tensors expected")
     if x.dtype not in _DTYPE:
         raise OpNotEligible(f"x must be bfloat16 or float16, got {x.dtype}")
-    _check("the weight", w, x.dtype, x.device)
-    if not (x.dim() >= 1 and w.dim() == 2 and w.shape[1] == x.shape[-1]):
+    _check("the weight", w, x.dtype, x.get_device())
+    shape, wshape = x.shape, w.shape
+    if len(shape) < 1 or len(wshape) != 2 or wshape[1] != shape[-1]:
         raise OpNotEligible(f"{what}: x [..., n_in] and a weight [rows, n_in] expected")
-    if not (w.shape[1] > 0 and w.shape[0] > 0):
+    if wshape[1] < 1 or wshape[0] < 1:
         raise OpNotEligible(f"{what}: feature counts must be positive")
-    if gated and w.shape[0] % 2:
+    if gated and wshape[0] % 2:
         raise OpNotEligible("w13 must hold gate rows followed by up rows: an even row count")
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if not (x2.shape[0] < _MOST_TOKENS and w.shape[0] < _MOST_ROWS and w.shape[1] <= _MOST_IN):
+    x2 = x if len(shape) == 2 else x.reshape(-1, shape[-1])
+    if x2.shape[0] >= _MOST_TOKENS or wshape[0] >= _MOST_ROWS or wshape[1] > _MOST_IN:
         raise OpNotEligible(f"{what}: more rows or features than the kernels index")
     return x2
 
@@ -129,8 +131,8 @@ def _inputs(x, w, gated, what):
 def _bias(bias, rows, x):
     if bias is None:
         return None
-    _check("the bias", bias, x.dtype, x.device)
-    if not (bias.shape == (rows,) and (rows == 1 or bias.stride(0) == 1)):
+    _check("the bias", bias, x.dtype, x.get_device())
+    if bias.shape != (rows,) or rows > 1 and bias.stride(0) != 1:
         raise OpNotEligible(f"the bias must be contiguous [{rows}]")
     return bias.data_ptr()
 
@@ -156,8 +158,8 @@ def _resident(x):
 
 def _given_out(out, shape, x, others):
     """A result tensor of the caller, as rows."""
-    _check("out", out, x.dtype, x.device)
-    if tuple(out.shape) != tuple(shape):
+    _check("out", out, x.dtype, x.get_device())
+    if out.shape != shape:
         raise OpNotEligible(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
     _apart("out", out, others)
     out2 = _rows2d("out", out, shape[-1])
@@ -168,8 +170,8 @@ def _given_out(out, shape, x, others):
 def _result(out, out2, shape, x):
     """The result tensor, as the caller sees it and as rows."""
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-        return out, out if out.dim() == 2 else out.view(-1, shape[-1])
+        out = x.new_empty(shape)
+        return out, out if len(shape) == 2 else out.view(-1, shape[-1])
     increment_version(out)
     return out, out2
 
@@ -179,7 +181,7 @@ def _forward_work(x, ldx, w, ldw, T, n_in, rows):
     if not (x.data_ptr() & 15 or w.data_ptr() & 15 or ldx & 7 or ldw & 7):
         return None, None, 0
     nbytes = _entry("vk_cuda_dense_forward_workspace_bytes")(x.data_ptr(), ldx, w.data_ptr(), ldw, T, n_in, rows)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    work = x.new_empty((nbytes,), dtype=torch.uint8)
     return work, work.data_ptr(), nbytes
 
 
@@ -235,7 +237,7 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, b13: torch.Tensor | None = 
             raise OpNotEligible("gated_linear: out and return_preact are for calls that record no gradient")
         return _GatedLinear.apply(x, w13, b13, activation, swiglu_limit, beta, linear_beta)
     h, h2 = _result(out, out2, shape, x)
-    preact = torch.empty((T, rows), dtype=torch.float32, device=x.device) if return_preact else None
+    preact = x.new_empty((T, rows), dtype=torch.float32) if return_preact else None
     if T > 0:
         work, wp, nbytes = _forward_work(x2, ldx, w13, ldw, T, hidden, rows)
         _call("vk_cuda_gated_linear", x.get_device(), x2.data_ptr(), ldx, w13.data_ptr(), ldw, b, h2.data_ptr(), _pitch("out", h2),
@@ -298,8 +300,8 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     ldx, ldw = _pitch("x", x2), _pitch("w", w)
     r2, ldr = None, 0
     if residual is not None:
-        _check("the residual", residual, x.dtype, x.device)
-        if tuple(residual.shape) != shape:
+        _check("the residual", residual, x.dtype, x.get_device())
+        if residual.shape != shape:
             raise OpNotEligible(f"the residual must be {shape}, got {tuple(residual.shape)}")
         r2 = _rows2d("the residual", residual, n_out)
         ldr = _pitch("the residual", r2)
@@ -314,7 +316,7 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
         return _FusedLinear.apply(x, w, bias, residual, activation)
     T, n_in = x2.shape
     y, y2 = _result(out, out2, shape, x)
-    preact = torch.empty((T, n_out), dtype=torch.float32, device=x.device) if return_preact and act else None
+    preact = x.new_empty((T, n_out), dtype=torch.float32) if return_preact and act else None
     if T > 0:
         work, wp, nbytes = _forward_work(x2, ldx, w, ldw, T, n_in, n_out)
         _call("vk_cuda_fused_linear", x.get_device(), x2.data_ptr(), ldx, w.data_ptr(), ldw, b, None if r2 is None else r2.data_ptr(), ldr,
@@ -354,13 +356,13 @@ def _backward(entry, dy, x, w, preact, gated, bias_grad, x_grad, w_grad, kind):
         rows, (T, n_in) = w.shape[0], x2.shape
         n_out = rows // 2 if gated else rows
         dtype = x.dtype
-        _check("the result's gradient", dy, dtype, x.device)
-        if tuple(dy.shape) != (*x.shape[:-1], n_out):
+        _check("the result's gradient", dy, dtype, x.get_device())
+        if dy.shape != (*x.shape[:-1], n_out):
             raise OpNotEligible(f"the result's gradient must be {(*x.shape[:-1], n_out)}, got {tuple(dy.shape)}")
         dy2 = dy if dy.dim() == 2 else dy.reshape(-1, n_out)
         if preact is not None:
-            _check("preact", preact, torch.float32, x.device)
-            if tuple(preact.shape) != (T, rows):
+            _check("preact", preact, torch.float32, x.get_device())
+            if preact.shape != (T, rows):
                 raise OpNotEligible(f"preact must be {(T, rows)}, got {tuple(preact.shape)}")
         ldx, ldw, ld_dy = _pitch("x", x2), _pitch("the weight", w), _pitch("the result's gradient", dy2)
         ldp = 0 if preact is None else _pitch("preact", preact)
