@@ -12,7 +12,6 @@
 #include <atomic>
 
 #include <algorithm>
-#include <cmath>
 
 #include "dense_tc.cuh"
 
@@ -543,35 +542,47 @@ struct WidePlan {
   int bn[2];
   float us;
 };
-float tile_us(const DenseGemm& g, int bn, float load) {
-  const float block_us = bn >= 128 ? 0.024f + 0.001f * (float)bn : 0.144f + 0.0001f * (float)bn;
-  // the more pairs are at work, the slower the narrower tiles, which bring more bytes for a product
-  load = 1.0f + 0.06f * (float)(256 - bn) / 64.0f * load;
-  if (g.b.mn_major && bn % 128 != 0) load *= 1.05f;   // B comes in boxes of 64 columns a CTA, some of them for nothing
-  return (float)((g.K + 63) / 64) * block_us * load + 1.0f;
-}
-int64_t count_tiles(const DenseGemm& g, int bn) {
-  const int64_t tile_n = g.gated ? bn / 2 : bn;
-  return ((int64_t)g.M + 255) / 256 * ((g.N + tile_n - 1) / tile_n);
+constexpr int kWidths = 7;                             // 256, 224, .. 64
+constexpr int width(int i) { return 256 - 32 * i; }
+struct WideCost {
+  int whole[kWidths], rest[kWidths];                   // tiles: full rounds of all pairs, and the last one
+  float tile_us[kWidths], load_us[kWidths];            // time of a tile, and what is added to it with all pairs at work
+};
+WideCost cost_of(const DenseGemm& g, int pairs) {
+  WideCost c;
+  const float blocks = (float)((g.K + 63) / 64);
+  const int tiles_m = (int)(((int64_t)g.M + 255) / 256);
+  for (int i = 0; i < kWidths; ++i) {
+    const int bn = width(i), tile_n = g.gated ? bn / 2 : bn;
+    const int64_t tiles = (int64_t)tiles_m * ((g.N + tile_n - 1) / tile_n);
+    c.whole[i] = (int)std::min<int64_t>(tiles / pairs, 1 << 24);
+    c.rest[i] = (int)(tiles % pairs);
+    const float block_us = bn >= 128 ? 0.024f + 0.001f * (float)bn : 0.144f + 0.0001f * (float)bn;
+    // B contiguous along its own index comes in boxes of 64 columns a CTA, some of them for nothing
+    const float us = blocks * block_us * (g.b.mn_major && bn % 128 != 0 ? 1.05f : 1.0f);
+    c.tile_us[i] = us + 1.0f;
+    c.load_us[i] = us * 0.06f * (float)(256 - bn) / 64.0f;   // narrower tiles bring more bytes for a product
+  }
+  return c;
 }
 WidePlan plan_wide(const DenseGemm* g, int count) {
-  const int64_t pairs = sm_count() / 2;
+  const int pairs = sm_count() / 2;
+  const WideCost first = cost_of(g[0], pairs), second = count > 1 ? cost_of(g[1], pairs) : WideCost{};
   WidePlan best{{256, 256}, 1e30f};
-  for (int bn = 256; bn >= 64; bn -= 32) {
-    const int64_t n0 = count_tiles(g[0], bn), q0 = n0 / pairs, r0 = n0 % pairs;
-    for (int other = 256; other >= (count > 1 ? 64 : 256); other -= 32) {
-      const int64_t n1 = count > 1 ? count_tiles(g[1], other) : 0, q1 = n1 / pairs, r1 = n1 % pairs;
-      const float full = (float)(n0 + n1) / (float)pairs, load = full < 1.0f ? full : 1.0f;
-      const float c0 = tile_us(g[0], bn, load), c1 = count > 1 ? tile_us(g[1], other, load) : 0.0f;
+  for (int i = 0; i < kWidths; ++i)
+    for (int j = 0; j < (count > 1 ? kWidths : 1); ++j) {
+      const int q0 = first.whole[i], r0 = first.rest[i], q1 = count > 1 ? second.whole[j] : 0, r1 = count > 1 ? second.rest[j] : 0;
+      const float full = (float)(q0 + q1) + (float)(r0 + r1) / (float)pairs, load = full < 1.0f ? full : 1.0f;
+      const float c0 = first.tile_us[i] + load * first.load_us[i];
+      const float c1 = count > 1 ? second.tile_us[j] + load * second.load_us[j] : 0.0f;
       // the busiest pair: one with a tile more of the first (and of the second, if those come round), or of the second alone
-      float most = r0 > 0 ? (float)(q0 + 1) * c0 + (float)(r0 + r1 > pairs ? q1 + 1 : q1) * c1 : (float)q0 * c0 + (float)q1 * c1;
-      if (r1 > 0) most = fmaxf(most, (float)q0 * c0 + (float)(q1 + 1) * c1);
+      float most = (float)(r0 > 0 ? q0 + 1 : q0) * c0 + (float)(r0 > 0 && r0 + r1 > pairs ? q1 + 1 : q1) * c1;
+      if (r1 > 0) most = std::max(most, (float)q0 * c0 + (float)(q1 + 1) * c1);
       // of many waves, half of what idle pairs leave undone in the last comes back as clock and bandwidth for the others
-      const float mean = ((float)n0 * c0 + (float)n1 * c1) / (float)pairs;
-      const float us = (bn >= 128 ? 2.4f + 0.0148f * (float)bn : 4.4f) + (full > 1.0f ? 0.5f * (most + mean) : most);
-      if (us < best.us) best = {{bn, other}, us};
+      const float mean = ((float)q0 + (float)r0 / (float)pairs) * c0 + ((float)q1 + (float)r1 / (float)pairs) * c1;
+      const float us = (width(i) >= 128 ? 2.4f + 0.0148f * (float)width(i) : 4.4f) + (full > 1.0f ? 0.5f * (most + mean) : most);
+      if (us < best.us) best = {{width(i), width(j)}, us};
     }
-  }
   return best;
 }
 

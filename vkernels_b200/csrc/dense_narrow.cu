@@ -342,8 +342,11 @@ void launch_narrow(const DenseGemm& g, cudaStream_t stream) {
   p.tmem_cols = 32;
   while (p.tmem_cols < p.tile_tok) p.tmem_cols *= 2;
   const int extra = (int)sizeof(NarrowBars) + 1024;
-  // two CTAs an SM while four stages fit, so that one streams while the other starts or joins
-  const int per_sm = 4 * p.stage_bytes + extra <= 113 * 1024 ? 2 : 1;
+  // Two CTAs an SM for a handful of tokens, where one starts or joins while the other streams; above, where the join counts, one
+  // with the whole ring: half the clusters, and half the partial sums in flight between them. 2880 -> 2 x 2880 gated 9.0 us with two
+  // and 9.4 with one for 1 token, 11.9 and 10.8 for 64; 7168 -> 2 x 2048 gated 12.8 and 13.2, 16.4 and 14.2; 2880 -> 2880 6.4 and
+  // 6.4, 9.6 and 8.1.
+  const int per_sm = g.M <= 8 ? 2 : 1;
   p.stages = min(kMaxStages, ((per_sm == 2 ? 113 * 1024 : kMaxSmem) - extra) / p.stage_bytes);
   const int tile_n = GATED ? 64 : 128;
   const int tiles = (g.N + tile_n - 1) / tile_n;
@@ -389,8 +392,8 @@ void launch_narrow(const DenseGemm& g, cudaStream_t stream) {
 
 }  // namespace
 
-// Its time (us), from the bytes at the memory's rate, the start and the join. Measured: 2880 -> 2880 6.3 us for 1 token, 9.5 for
-// 64, 9.8 for 128, 12.9 for 256; 7168 -> 2 x 2048 gated 13.5, 16.7, 16.4, 19.7; 2048 -> 7168 8.3, 10.5, 13.1, 18.8.
+// Its time (us), from the bytes at the memory's rate, the start and the join. Measured: 2880 -> 2880 6.4 us for 1 token, 8.1 for
+// 64, 9.7 for 128, 12.9 for 256; 7168 -> 2 x 2048 gated 12.8, 14.2, 16.0, 19.7; 2048 -> 7168 8.4, 10.3, 13.1, 18.8.
 float dense_narrow_us(const DenseGemm& g) {
   const double rows = g.gated ? 2.0 * g.N : g.N;
   const double bytes = 2.0 * (rows * g.K + (double)g.M * g.K + (double)g.M * g.N);
