@@ -62,12 +62,13 @@ float effective_limit(bool gated, int act, float limit) { return gated && act ==
 }  // namespace
 
 // Small batches go to the kernel that cuts k over clusters, the others to the CTA pairs: whichever takes less by the sizes. The
-// line lies near 64 tokens for short reductions of many features, at 256 for long ones of few (128 tokens: 2048 -> 7168 13.1 us
-// and 11.2, 2880 -> 2880 9.8 and 12, 7168 -> 2 x 2048 gated 16.4 and 24; 256 tokens 18.8 and 11.2, 12.9 and 12.1, 19.7 and 24.6).
+// line lies near 64 tokens for short reductions of many features, at some hundred for long ones of few (128 tokens: 2048 -> 7168
+// 13.1 us and 11.2, 2880 -> 2880 9.7 and 12, 7168 -> 2 x 2048 gated 16.0 and 24; 256 tokens 18.8 and 11.2, 13.2 and 12.1, 19.9 and
+// 24.6).
 void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream) {
   if (g.M == 0 || g.N == 0) return;
   if (get_moe_impl() == MoeImpl::kSimt) launch_dense_simt(g, stream);
-  else if (!g.a.mn_major && g.M <= 256 && dense_narrow_us(g) < dense_wide_us(g)) launch_dense_narrow(g, stream);
+  else if (!g.a.mn_major && g.M <= 512 && dense_narrow_us(g) < dense_wide_us(g)) launch_dense_narrow(g, stream);
   else launch_dense_wide(g, stream);
 }
 

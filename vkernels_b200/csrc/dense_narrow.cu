@@ -1,12 +1,14 @@
 // dense_narrow.cu - products of the dense feed-forward operators for small batches: weights as the M operand, split over k.
 //
 // A decode batch reads every weight once and does next to nothing with it: the time is that of the weights' way from memory.
-// 128 weight rows are one tile (gated: 64 gate rows and the 64 up rows of the same features), up to 128 tokens, rounded up to
+// 128 weight rows are one tile (gated: 64 gate rows and the 64 up rows of the same features), up to 192 tokens, rounded up to
 // 16, are the MMA's N. The k range of a tile is cut over the CTAs of a cluster, so that all SMs stream weights however few
 // tiles there are. Every CTA leaves its partial sums [token][row] in its own shared memory, where the ring was, and after a
 // cluster barrier each adds its share of the results over the cluster, rank after rank: no atomics, no scratch in memory, the
 // same bits every time. (Sending the sums to their owner instead needs a barrier more - every ring has to be free first - and
 // took 1 to 5 us longer.)
+#include <algorithm>
+
 #include "dense_tc.cuh"
 
 namespace vkernels::kernels::cuda {
@@ -17,9 +19,7 @@ constexpr int kMaxStages = 12, kMaxSplit = 8;
 constexpr int kMaxSmem = 232448;
 constexpr int kEpiWarps = 8, kEpiThreads = 32 * kEpiWarps, kThreads = kEpiThreads + 64;   // and producer, MMA issuer
 constexpr int kAhead = 4;
-// Tokens of a tile. 256 tokens of 7168 -> 2 x 2048 gated: 24.7 us as four tiles, 19.7 as two, 22.6 as one (whose join moves twice
-// the sums over the cluster); 2880 -> 2880: 13.4, 12.9 and 13.8.
-constexpr int kMaxTileTok = 128;
+constexpr int kMaxTileTok = 192;
 constexpr int kWeightBytes = 16384;            // 128 rows x 64 k
 
 struct NarrowBars {
@@ -321,6 +321,49 @@ int resident_clusters(int split) {
   return n;
 }
 
+struct NarrowPlan {
+  int per_sm, tile_tok, tok_tiles, tiles, split, stages, stage_bytes;
+  float us;
+};
+constexpr int kExtraSmem = (int)sizeof(NarrowBars) + 1024;
+NarrowPlan plan_of(const DenseGemm& g, int tok_tiles) {
+  NarrowPlan n;
+  n.tile_tok = ((g.M + tok_tiles - 1) / tok_tiles + 15) / 16 * 16;
+  n.tok_tiles = (g.M + n.tile_tok - 1) / n.tile_tok;
+  n.stage_bytes = kWeightBytes + n.tile_tok * 128;
+  // Two CTAs an SM for a handful of tokens, where one starts or joins while the other streams; above, where the join counts, one
+  // with the whole ring: half the clusters, and half the partial sums in flight between them. 2880 -> 2 x 2880 gated 9.0 us with two
+  // and 9.4 with one for 1 token, 11.9 and 10.8 for 64; 7168 -> 2 x 2048 gated 12.8 and 13.2, 16.4 and 14.2; 2880 -> 2880 6.4 and
+  // 6.4, 9.6 and 8.1.
+  n.per_sm = g.M <= 8 ? 2 : 1;
+  n.stages = std::min(kMaxStages, ((n.per_sm == 2 ? 113 * 1024 : kMaxSmem) - kExtraSmem) / n.stage_bytes);
+  const int tile_n = g.gated ? 64 : 128;
+  n.tiles = (g.N + tile_n - 1) / tile_n * n.tok_tiles;
+  // the largest split whose clusters are all resident at once
+  n.split = std::min(kMaxSplit, (g.K + 63) / 64);
+  while (n.split > 1 && n.tiles > resident_clusters(n.split) * n.per_sm) --n.split;
+  // Its time: start, the weights' way from memory or what an SM takes in of weights and tokens - whichever is longer -, join.
+  // Measured: 2880 -> 2880 6.4 us for 1 token, 8.1 for 64, 9.7 for 128, 13.2 for 256; 7168 -> 2 x 2048 gated 12.8, 14.2, 16.0, 19.9;
+  // 2048 -> 7168 8.4, 10.3, 13.1, 18.8; 7168 -> 2048 for 300 and 512 tokens 19.1 and 20.8 (29 as CTA pairs).
+  const float rows = g.gated ? 2.0f * (float)g.N : (float)g.N, m = (float)g.M;
+  const float memory = 2.0f * (rows * (float)g.K + m * (float)g.K + m * (float)g.N) / 6.5e6f;
+  const int at_once = sm_count() * n.per_sm;
+  const float waves = (float)(((int64_t)n.tiles * n.split + at_once - 1) / at_once);
+  const float fill = waves * (float)n.per_sm * (float)g.K / (float)n.split * (256.0f + 2.0f * (float)n.tile_tok) / 130e3f;
+  n.us = 3.4f + std::max(memory, fill) + (g.M > 16 ? 0.8f : 0.0f) + 0.015f * (float)n.tile_tok;
+  return n;
+}
+// Tokens in as many tiles as take the least time: wider tiles bring the weights to fewer SMs, narrower ones join sooner. At most 192
+// (256 tokens of 7168 -> 2 x 2048 gated: 19.7 us as two tiles, 22.6 as one).
+NarrowPlan plan_narrow(const DenseGemm& g) {
+  NarrowPlan best = plan_of(g, (g.M + kMaxTileTok - 1) / kMaxTileTok);
+  for (int tiles = best.tok_tiles + 1; tiles <= (g.M + 63) / 64; ++tiles) {
+    const NarrowPlan n = plan_of(g, tiles);
+    if (n.us < best.us) best = n;
+  }
+  return best;
+}
+
 template <int TYPE, bool GATED>
 void launch_narrow(const DenseGemm& g, cudaStream_t stream) {
   static std::atomic<bool> configured[64];
@@ -330,29 +373,18 @@ void launch_narrow(const DenseGemm& g, cudaStream_t stream) {
     VK_CUDA_CHECK(cudaFuncSetAttribute(dense_narrow_kernel<TYPE, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
     if (dev >= 0 && dev < 64) configured[dev].store(true);
   }
+  const NarrowPlan n = plan_narrow(g);
   NarrowParams p{};
   p.M = g.M;
   p.N = g.N;
   p.w_mn = g.b.mn_major;
-  p.tok_tiles = (g.M + kMaxTileTok - 1) / kMaxTileTok;
-  p.tile_tok = ((g.M + p.tok_tiles - 1) / p.tok_tiles + 15) / 16 * 16;
-  p.tok_tiles = (g.M + p.tile_tok - 1) / p.tile_tok;
+  p.tile_tok = n.tile_tok;
+  p.tok_tiles = n.tok_tiles;
+  p.stages = n.stages;
+  p.stage_bytes = n.stage_bytes;
   p.k_blocks = (g.K + 63) / 64;
-  p.stage_bytes = kWeightBytes + p.tile_tok * 128;
   p.tmem_cols = 32;
   while (p.tmem_cols < p.tile_tok) p.tmem_cols *= 2;
-  const int extra = (int)sizeof(NarrowBars) + 1024;
-  // Two CTAs an SM for a handful of tokens, where one starts or joins while the other streams; above, where the join counts, one
-  // with the whole ring: half the clusters, and half the partial sums in flight between them. 2880 -> 2 x 2880 gated 9.0 us with two
-  // and 9.4 with one for 1 token, 11.9 and 10.8 for 64; 7168 -> 2 x 2048 gated 12.8 and 13.2, 16.4 and 14.2; 2880 -> 2880 6.4 and
-  // 6.4, 9.6 and 8.1.
-  const int per_sm = g.M <= 8 ? 2 : 1;
-  p.stages = min(kMaxStages, ((per_sm == 2 ? 113 * 1024 : kMaxSmem) - extra) / p.stage_bytes);
-  const int tile_n = GATED ? 64 : 128;
-  const int tiles = (g.N + tile_n - 1) / tile_n;
-  // the largest split whose clusters are all resident at once
-  int split = min(kMaxSplit, p.k_blocks);
-  while (split > 1 && (int64_t)tiles * p.tok_tiles > resident_clusters(split) * per_sm) --split;
   p.act = g.act;
   p.limit = g.limit;
   p.beta = g.beta;
@@ -375,13 +407,13 @@ void launch_narrow(const DenseGemm& g, cudaStream_t stream) {
                                                            (uint64_t)g.b.ld * 2, GATED ? 64 : 128);
   const CUtensorMap x = sm100_make_map_bf16(g.a.p, (uint64_t)g.K, (uint64_t)g.M, (uint64_t)g.a.ld * 2, (uint32_t)p.tile_tok);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(tiles * p.tok_tiles * split));
+  cfg.gridDim = dim3((unsigned)(n.tiles * n.split));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)(p.stages * p.stage_bytes + extra);
+  cfg.dynamicSmemBytes = (size_t)(p.stages * p.stage_bytes + kExtraSmem);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.x = (unsigned)n.split;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
@@ -392,13 +424,7 @@ void launch_narrow(const DenseGemm& g, cudaStream_t stream) {
 
 }  // namespace
 
-// Its time (us), from the bytes at the memory's rate, the start and the join. Measured: 2880 -> 2880 6.4 us for 1 token, 8.1 for
-// 64, 9.7 for 128, 12.9 for 256; 7168 -> 2 x 2048 gated 12.8, 14.2, 16.0, 19.7; 2048 -> 7168 8.4, 10.3, 13.1, 18.8.
-float dense_narrow_us(const DenseGemm& g) {
-  const double rows = g.gated ? 2.0 * g.N : g.N;
-  const double bytes = 2.0 * (rows * g.K + (double)g.M * g.K + (double)g.M * g.N);
-  return (float)(3.4 + bytes / 6.5e6 + (g.M > 16 ? 0.8 : 0.0) + 0.02 * g.M);
-}
+float dense_narrow_us(const DenseGemm& g) { return plan_narrow(g).us; }
 
 // A is the batch (contiguous along k), B the weight in either order.
 void launch_dense_narrow(const DenseGemm& g, cudaStream_t stream) {
