@@ -74,6 +74,12 @@ def test_out_must_not_overlap_the_inputs():
         ops.fused_linear(a, w, out=w[:4])
     with pytest.raises(ops.OpNotEligible, match="residual"):
         ops.fused_linear(t(2, 16), w, residual=a[:2], out=a[1:3])
+    wide = t(4, 40)
+    for x, out, match in ((wide[:, 24:], wide[:, :16], "CUDA"), (wide[:, :16], wide[:, 16:32], "CUDA"),     # beside one another
+                          (wide[:, 24:], wide[:, 9:25], "overlap x"), (wide[:, :16], wide[:, 15:31], "overlap x"),
+                          (wide[:3, 24:], wide[1:, :16], "CUDA"), (wide[:3, 24:], wide[1:, 20:36], "overlap x")):
+        with pytest.raises(ops.OpNotEligible, match=match):
+            ops.fused_linear(x, w, out=out)
     with pytest.raises(ops.OpNotEligible, match="CUDA"):     # the residual itself is a place for the result
         ops.fused_linear(t(2, 16), w, residual=a[:2], out=a[:2])
     with pytest.raises(ops.OpNotEligible, match="overlap w13"):
@@ -110,7 +116,7 @@ def linear_back_args(**k):
     (dict(ldx=68), b"workspace"), (dict(x=P + 2, work=P, nbytes=511), b"workspace"), (dict(ldw=66, work=P + 8, nbytes=1 << 20), b"workspace"),
     (dict(ldw=56), b"pitch"), (dict(y=None), b"null"), (dict(y=P + 1), b"odd"), (dict(ldy=63), b"pitch"), (dict(bias=P + 1), b"bias"),
     (dict(residual=P + 1, ldr=64), b"odd"), (dict(residual=P, ldr=63), b"pitch"), (dict(preact=P, ldp=63), b"pitch"), (dict(preact=P + 2, ldp=64), b"preact"),
-    (dict(act=4), b"activation"), (dict(act=-1), b"activation"), (dict(n_in=(1 << 30) + 1), b"sizes")])
+    (dict(act=4), b"activation"), (dict(act=-1), b"activation"), (dict(n_in=(1 << 27) + 1, ldx=1 << 28, ldw=1 << 28), b"sizes"), (dict(T=(1 << 27) + 1), b"sizes")])
 def test_linear_entry_refuses(bad, word):
     lib = nr.load_library()
     assert lib.vk_cuda_fused_linear(*linear_args(**bad)) == 1 and word in lib.vk_last_error(), lib.vk_last_error()

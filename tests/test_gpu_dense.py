@@ -442,3 +442,87 @@ def test_shared_expert_beside_the_routed_ones(T):
         assert torch.equal(y, want) or T > 256 and torch.allclose(y.float(), want.float(), atol=2e-2, rtol=2.0 ** -7)
     assert first.shape == y.shape
     ops.kernel_status()
+
+
+def test_columns_of_one_buffer():
+    """x, residual and result as columns of one wider buffer: read and written where they lie."""
+    x, w, b, more = tensors(70, 72, 40, "bf16")
+    wide = more(200)
+    wide[:, 8:80] = x
+    want = ops.fused_linear(x, w, b, residual=wide[:, 80:120].clone())
+    keep = wide.clone()
+    got = ops.fused_linear(wide[:, 8:80], w, b, residual=wide[:, 80:120], out=wide[:, 120:160])
+    assert torch.equal(got, want)
+    keep[:, 120:160] = want
+    assert torch.equal(wide, keep)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements in the result, the residual, x (as columns of that result) and the pre-activations."""
+    T, K, N = 266000, 64, 8256
+    x, w, b, more = tensors(T, K, N, "bf16")
+    y = ops.fused_linear(x, w, b)
+    assert y.numel() > 2 ** 31
+    some = torch.tensor([0, 1, T // 2 + 5, T - 3, T - 1], device=DEV)
+    z, mags = ref.project(x[some], w, b)
+    bound = ref.sum_error(K) * mags
+    ref.assert_within(y[some], z, bound + ref.half_step(y.dtype) * (z.abs() + bound), "y")
+    tail = y[:, N - 64:]                       # the last 64 columns: rows 16512 bytes apart
+    w13 = w[:64, :64]
+    h, preact = ops.gated_linear(tail, w13, return_preact=True)
+    assert torch.equal(h, ops.gated_linear(tail.contiguous(), w13))
+    dx, dw, _ = ops.gated_linear_backward(more(32), tail, w13, preact)
+    assert dx.shape == (T, 64) and bool(dx[some].isfinite().all())
+    before = y[some].clone()
+    del h, preact, dx, dw
+    again = ops.fused_linear(x, w, b, residual=y, out=y)         # in place: residual and result far beyond 2^31
+    value = z + before.double()
+    ref.assert_within(again[some], value, bound + 2.0 ** -23 * value.abs() + ref.half_step(y.dtype) * (value.abs() + bound), "y + y")
+    ops.kernel_status()
+
+
+_FIRST_CALL = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from vkernels_b200 import torch_ops as ops
+for T in (4, 400):
+    x = torch.randn(T, 128, device="cuda").to(torch.bfloat16)
+    w = torch.randn(192, 128, device="cuda").to(torch.bfloat16)
+    dy = torch.randn(T, 96, device="cuda").to(torch.bfloat16)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        h, preact = ops.gated_linear(x, w, return_preact=True)
+        grads = ops.gated_linear_backward(dy, x, w, preact, bias_grad=True)
+    g.replay()
+    torch.cuda.synchronize()
+    want = ops.gated_linear(x, w)
+    assert torch.equal(h, want)
+    assert all(torch.equal(a, b) for a, b in zip(grads, ops.gated_linear_backward(dy, x, w, preact, bias_grad=True)))
+print("replayed")
+# a backward pass of a graph recorded before the capture: refused with an exception, and the process lives on
+x = torch.randn(8, 64, device="cuda").to(torch.bfloat16).requires_grad_()
+w = torch.randn(32, 64, device="cuda").to(torch.bfloat16).requires_grad_()
+y = ops.gated_linear(x, w)
+torch.cuda.synchronize()
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        torch.autograd.grad(y, [x, w], torch.ones_like(y))
+except Exception as e:
+    print("refused", type(e).__name__)
+torch.cuda.synchronize()
+y = ops.gated_linear(x, w)
+y.sum().backward()
+print("alive", bool(x.grad.isfinite().all()))
+"""
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALL.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "replayed" in r.stdout and "refused" in r.stdout and "alive True" in r.stdout, (r.stdout, r.stderr[-2000:])

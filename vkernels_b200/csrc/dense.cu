@@ -16,7 +16,9 @@ size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 void check_common(DenseType type, int T, int n_in, int n_out, bool gated, int act, float limit, float beta) {
   expects(type == kDenseBf16 || type == kDenseFp16, "dense: dtype must be 0 (bf16) or 1 (fp16)");
   expects(T >= 0 && n_in > 0 && n_out > 0, "dense: T must not be negative, feature counts must be positive");
-  expects(n_in <= (1 << 30) && n_out <= (1 << 29) && T <= (1 << 30), "dense: sizes beyond 2^29 features or 2^30 tokens");
+  // (a wait inside the kernels gives up after two seconds; one tile over 2^27 values takes 0.6)
+  constexpr int kMost = 1 << 27;
+  expects(n_in <= kMost && n_out <= (gated ? kMost / 2 : kMost) && T <= kMost, "dense: sizes beyond 2^27 tokens, inputs or weight rows");
   if (gated) {
     expects(act == 0 || act == 1, "gated_linear: activation must be 0 (SwiGLU) or 1 (SiTU)");
     expects(limit >= 0.0f, "gated_linear: swiglu_limit must not be negative (0 for none)");

@@ -25,8 +25,8 @@ from .moe_fused_mxfp4 import SITU, SWIGLU
 
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1}
 _LINEAR_ACT = {None: 0, "none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
-# what the kernels index
-_MOST_TOKENS, _MOST_ROWS, _MOST_IN = 2 ** 30, 2 ** 30, 2 ** 30
+# tokens, inputs, weight rows that the kernels take
+_MOST = 2 ** 27
 
 _entries = {}
 
@@ -93,8 +93,16 @@ def _apart(name, out, others):
     for other_name, t in others:
         if t is not None:
             c, d = _span(t)
-            if a < d and c < b:
+            if a < d and c < b and not _side_by_side(out, a, t, c):
                 raise OpNotEligible(f"{name} must not overlap {other_name}")
+
+
+def _side_by_side(t, a, u, c):
+    """Whether two matrices are different columns of one wider one."""
+    if t.dim() != 2 or u.dim() != 2 or t.stride() != u.stride() or t.stride(1) != 1:
+        return False
+    pitch, gap = t.stride(0), (c - a) // t.element_size()
+    return t.shape[1] <= gap % pitch and gap % pitch + u.shape[1] <= pitch
 
 
 def _rows2d(name, t, cols):
@@ -123,8 +131,8 @@ def _inputs(x, w, gated, what):
     if gated and wshape[0] % 2:
         raise OpNotEligible("w13 must hold gate rows followed by up rows: an even row count")
     x2 = x if len(shape) == 2 else x.reshape(-1, shape[-1])
-    if x2.shape[0] >= _MOST_TOKENS or wshape[0] >= _MOST_ROWS or wshape[1] > _MOST_IN:
-        raise OpNotEligible(f"{what}: more rows or features than the kernels index")
+    if x2.shape[0] > _MOST or wshape[0] > _MOST or wshape[1] > _MOST:
+        raise OpNotEligible(f"{what}: more than 2^27 tokens, inputs or weight rows")
     return x2
 
 
@@ -211,8 +219,8 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, b13: torch.Tensor | None = 
     if out is None and type(x) is torch.Tensor and isinstance(w13, torch.Tensor):
         # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
         shape, index, dtype, wshape = x.shape, x.get_device(), x.dtype, w13.shape
-        if (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and wshape[1] == shape[1] > 0
-                and not shape[1] & 7 and 0 < wshape[0] < _MOST_ROWS and not wshape[0] & 1 and 0 < shape[0] < _MOST_TOKENS
+        if (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and _MOST >= wshape[1] == shape[1] > 0
+                and not shape[1] & 7 and 0 < wshape[0] <= _MOST and not wshape[0] & 1 and 0 < shape[0] <= _MOST
                 and (activation == SWIGLU or activation == SITU and beta > 0) and swiglu_limit >= 0
                 and _plain(x, shape, dtype, index) and _plain(w13, wshape, dtype, index)
                 and (b13 is None or _plain(b13, wshape[:1], dtype, index)) and not _wants_grad(x, w13, b13)):
@@ -280,8 +288,8 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     if out is None and type(x) is torch.Tensor and isinstance(w, torch.Tensor):
         # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
         shape, index, dtype, wshape = x.shape, x.get_device(), x.dtype, w.shape
-        if (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and wshape[1] == shape[1] > 0
-                and not shape[1] & 7 and 0 < wshape[0] < _MOST_ROWS and 0 < shape[0] < _MOST_TOKENS
+        if (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and _MOST >= wshape[1] == shape[1] > 0
+                and not shape[1] & 7 and 0 < wshape[0] <= _MOST and 0 < shape[0] <= _MOST
                 and _plain(x, shape, dtype, index) and _plain(w, wshape, dtype, index)
                 and (bias is None or _plain(bias, wshape[:1], dtype, index))
                 and (residual is None or _plain(residual, (shape[0], wshape[0]), dtype, index))
@@ -340,8 +348,8 @@ def _backward(entry, dy, x, w, preact, gated, bias_grad, x_grad, w_grad, kind):
     if type(x) is torch.Tensor and isinstance(w, torch.Tensor) and isinstance(dy, torch.Tensor):
         # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
         shape, index, dtype, wshape = x.shape, x.get_device(), x.dtype, w.shape
-        ordinary = (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and wshape[1] == shape[1] > 0
-                    and not shape[1] & 7 and 0 < wshape[0] < _MOST_ROWS and not (gated and wshape[0] & 1) and 0 < shape[0] < _MOST_TOKENS
+        ordinary = (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and _MOST >= wshape[1] == shape[1] > 0
+                    and not shape[1] & 7 and 0 < wshape[0] <= _MOST and not (gated and wshape[0] & 1) and 0 < shape[0] <= _MOST
                     and _plain(x, shape, dtype, index) and _plain(w, wshape, dtype, index)
                     and _plain(dy, (shape[0], wshape[0] >> gated), dtype, index)
                     and (preact is None or _plain(preact, (shape[0], wshape[0]), torch.float32, index)))
