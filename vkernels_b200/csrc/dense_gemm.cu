@@ -450,6 +450,8 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
       Piece ahead;   // the residual of the coming columns, on its way while the MMAs run
       if (!GATED && p.residual && p.direct && rows > 0 && col_first < p.N)
         piece_load(ahead, p.residual + row0 * p.ldr + col_first, p.ldr, rows, min(min(64, mine), p.N - col_first), lane);
+      if (!GATED && p.residual && !p.direct && row_ok)   // rows that start anywhere are fetched later, out of the L2
+        for (int c = 0; c < min(mine, p.N - col_first); c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.residual + row * p.ldr + col_first + c));
       const bool ready = mbar_wait(smem_u32(&bars->acc_full[buf]), (it >> 1) & 1, abort_flag, 54, 32);
       if (!__all_sync(0xFFFFFFFFu, ready)) break;
       tc_fence_after();
