@@ -59,7 +59,7 @@ size_t bring_operands(const uint16_t*& x, int64_t& ldx, int T, const uint16_t*& 
   if (bw) w = dst[1], ldw = pitch;
   return bx + bw;
 }
-float effective_limit(bool gated, int act, float limit) { return gated && act == 0 && limit > 0.0f ? limit : INFINITY; }
+float effective_limit(int act, float limit) { return act == 0 && limit > 0.0f ? limit : INFINITY; }
 
 }  // namespace
 
@@ -101,9 +101,7 @@ void dense_forward(const DenseForward& f, cudaStream_t stream) {
   g.K = f.n_in;
   g.gated = f.gated;
   g.act = f.act;
-  g.limit = effective_limit(f.gated, f.act, f.limit);
-  g.beta = f.beta;
-  g.linear_beta = f.linear_beta;
+  if (f.gated) g.kind = gated_kind(f.act, effective_limit(f.act, f.limit), f.beta, f.linear_beta);
   g.bias = f.bias;
   g.residual = f.residual;
   g.ldr = f.ldr;
@@ -175,9 +173,7 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
     g.N = f.n_out;
     g.gated = f.gated;
     g.act = f.act;
-    g.limit = effective_limit(f.gated, f.act, f.limit);
-    g.beta = f.beta;
-    g.linear_beta = f.linear_beta;
+    if (f.gated) g.kind = gated_kind(f.act, effective_limit(f.act, f.limit), f.beta, f.linear_beta);
     launch_dense_grad(g, stream);
     if (f.db && chunks > 1) launch_dense_sum(f.type, partial, chunks, rows, f.db, stream);
   }
@@ -185,7 +181,6 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
   const int64_t ldzz = need_dz ? ldz : f.lddy;
   DenseGemm gx{}, gw{};
   gx.type = gw.type = f.type;
-  gx.limit = gw.limit = INFINITY;
   if (f.dx) {   // dx[t, i] = sum_n dz[t, n] w[n, i]
     gx.a = {z, ldzz, false};
     gx.b = {w, ldw, true};

@@ -13,6 +13,15 @@ enum DenseType { kDenseBf16 = 0, kDenseFp16 = 1 };
 // activation of the linear projection
 enum DenseAct { kActNone = 0, kActSilu = 1, kActGelu = 2, kActGeluTanh = 3 };
 
+// The gated activation: 0 SwiGLU with its clamp (inf: none), 1 SiTU.
+struct GatedKind {
+  int act;
+  float limit, beta, linear_beta, inv_beta, inv_linear_beta;
+};
+inline GatedKind gated_kind(int act, float limit, float beta, float linear_beta) {
+  return {act, limit, beta, linear_beta, 1.0f / beta, linear_beta > 0.0f ? 1.0f / linear_beta : 0.0f};
+}
+
 // One 16-bit operand of a product: element (i, k) is p[i * ld + k], or p[k * ld + i] if mn_major (the index that is NOT
 // reduced over is the contiguous one).
 struct DenseOperand {
@@ -28,8 +37,8 @@ struct DenseGemm {
   DenseOperand a, b;
   int M, N, K;
   bool gated;
-  int act;                    // linear: DenseAct; gated: 0 SwiGLU, 1 SiTU
-  float limit, beta, linear_beta;
+  int act;                    // linear: DenseAct
+  GatedKind kind;             // gated
   const uint16_t* bias;       // or null
   const uint16_t* residual;   // or null
   int64_t ldr;
@@ -54,8 +63,8 @@ struct DenseGrad {
   uint16_t* db;
   int T, N;                   // N: columns of dy; the gated form has 2 N columns of dz
   bool gated;
-  int act;
-  float limit, beta, linear_beta;
+  int act;                    // linear: DenseAct
+  GatedKind kind;             // gated
 };
 
 int dense_sum_chunks(int T, int n_out);

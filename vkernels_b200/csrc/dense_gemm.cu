@@ -39,7 +39,7 @@ struct WideParams {           // one product
   int stage_bytes;            // of one CTA: what the copies of a stage bring
   int tiles_m, tiles_n, n_tiles, k_blocks;
   int act;
-  float limit, beta, linear_beta;
+  GatedKind kind;
   const uint16_t* bias;
   const uint16_t* residual;
   uint16_t* out;
@@ -287,8 +287,8 @@ __device__ __forceinline__ void gated_columns(uint32_t tg, uint32_t tu, int widt
     uint32_t w[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      w[j] = dense_pack<TYPE>(dense_gated(ACT, g[j * 2], u[j * 2], p.limit, p.beta, p.linear_beta),
-                              dense_gated(ACT, g[j * 2 + 1], u[j * 2 + 1], p.limit, p.beta, p.linear_beta));
+      w[j] = dense_pack<TYPE>(dense_gated(ACT, g[j * 2], u[j * 2], p.kind),
+                              dense_gated(ACT, g[j * 2 + 1], u[j * 2 + 1], p.kind));
     if (DIRECT) {
       if (at.out && n > 0) row_store(at.out + block * 16, w, n, p.wide_o);
     } else {
@@ -478,7 +478,7 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
               }
             }
             if constexpr (GATED) {
-              if (p.act == 1) gated_columns<TYPE, 1, true>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
+              if (p.kind.act == 1) gated_columns<TYPE, 1, true>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
               else gated_columns<TYPE, 0, true>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
             } else {
               if (p.residual) {
@@ -499,7 +499,7 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
               __syncwarp();
             }
             if constexpr (GATED) {
-              if (p.act == 1) gated_columns<TYPE, 1, false>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
+              if (p.kind.act == 1) gated_columns<TYPE, 1, false>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
               else gated_columns<TYPE, 0, false>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
             } else {
               linear_columns<TYPE, false>(tz, width, staging, bias, has_bias, p.residual != nullptr, at, p, lane);
@@ -603,9 +603,7 @@ void describe(const DenseGemm& g, int bn, WideParams& p, CUtensorMap& a, CUtenso
   p.n_tiles = p.tiles_m * p.tiles_n;
   p.k_blocks = (g.K + 63) / 64;
   p.act = g.act;
-  p.limit = g.limit;
-  p.beta = g.beta;
-  p.linear_beta = g.linear_beta;
+  p.kind = g.kind;
   p.bias = g.bias;
   p.residual = g.residual;
   p.out = g.out;

@@ -106,38 +106,38 @@ __device__ __forceinline__ float dense_tanh_parts(float y, float& e) {
   return fabsf(y) < 0.25f ? dense_tanh_near(y) * (e + 1.0f) : e - 1.0f;
 }
 
-// The gated product of one feature; `limit` = inf for no clamp. min.NaN / max.NaN: a NaN stays NaN. SiTU's three quotients -
+// The gated product of one feature. min.NaN / max.NaN: a NaN stays NaN. SiTU's three quotients -
 // two tanh, one sigmoid - have one reciprocal: it is bound by the special-function unit (333 x 2880 -> 2880 with biases 22.6 us
 // with one for each).
-__device__ __forceinline__ float dense_gated(int act, float g, float u, float limit, float beta, float linear_beta) {
+__device__ __forceinline__ float dense_gated(int act, float g, float u, const GatedKind& k) {
   if (act == 1) {
     float e1, e2, e3 = 0.0f, low, r;
-    const float n1 = dense_tanh_parts(g * __fdividef(1.0f, beta), e1);
+    const float n1 = dense_tanh_parts(g * k.inv_beta, e1);
     // exp(-g), finite: what is lost beyond exp(87) is below every 16-bit type's smallest value
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(low) : "f"(g * -1.4426950408889634f), "f"(125.5f));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e2) : "f"(low));
-    const float n3 = linear_beta > 0.0f ? linear_beta * dense_tanh_parts(u * __fdividef(1.0f, linear_beta), e3) : u;
+    const float n3 = k.linear_beta > 0.0f ? k.linear_beta * dense_tanh_parts(u * k.inv_linear_beta, e3) : u;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((e1 + 1.0f) * (1.0f + e2) * (e3 + 1.0f)));
-    return beta * n1 * r * n3;
+    return k.beta * n1 * r * n3;
   }
-  float lo = -limit;
+  const float limit = k.limit, lo = -limit;
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(g) : "f"(limit));
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(u) : "f"(limit));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(u) : "f"(lo));
   return g * dense_sigmoid(g) * u;
 }
 // Its gradient with respect to both pre-activations, for the gradient dh of the product.
-__device__ __forceinline__ void dense_gated_grad(int act, float dh, float g, float u, float limit, float beta, float linear_beta,
-                                                 float& dg, float& du) {
-  if (act == 1) {
-    const float p = dense_sigmoid(g), a = dense_tanh(__fdividef(g, beta));
-    const float b = linear_beta > 0.0f ? dense_tanh(__fdividef(u, linear_beta)) : 0.0f;
-    const float up = linear_beta > 0.0f ? linear_beta * b : u;
-    dg = dh * up * ((1.0f - a * a) * p + beta * a * p * (1.0f - p));
-    du = dh * (beta * a * p) * (1.0f - b * b);
+__device__ __forceinline__ void dense_gated_grad(float dh, float g, float u, const GatedKind& k, float& dg, float& du) {
+  if (k.act == 1) {
+    const bool bent = k.linear_beta > 0.0f;
+    const float p = dense_sigmoid(g), a = dense_tanh(g * k.inv_beta), b = bent ? dense_tanh(u * k.inv_linear_beta) : 0.0f;
+    const float up = bent ? k.linear_beta * b : u;
+    dg = dh * up * ((1.0f - a * a) * p + k.beta * a * p * (1.0f - p));
+    du = dh * (k.beta * a * p) * (1.0f - b * b);
     return;
   }
-  float gc = g, uc = u, lo = -limit;
+  const float limit = k.limit, lo = -limit;
+  float gc = g, uc = u;
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(gc) : "f"(limit));
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(uc) : "f"(limit));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(uc) : "f"(lo));

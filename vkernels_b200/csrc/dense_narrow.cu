@@ -34,7 +34,7 @@ struct NarrowParams {
   int tile_tok, tok_tiles;    // tokens of a tile (a multiple of 16), tiles of tokens
   int stages, stage_bytes, tmem_cols, k_blocks;
   int act;
-  float limit, beta, linear_beta;
+  GatedKind kind;
   const uint16_t* bias;
   const uint16_t* residual;
   uint16_t* out;
@@ -271,7 +271,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       }
       if (GATED) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = dense_from_f32<TYPE>(dense_gated(p.act, z[j], zu[j], p.limit, p.beta, p.linear_beta));
+        for (int j = 0; j < 4; ++j) y[j] = dense_from_f32<TYPE>(dense_gated(p.kind.act, z[j], zu[j], p.kind));
       } else {
         const float2 r0 = dense_unpack<TYPE>(r.x), r1 = dense_unpack<TYPE>(r.y);
         const float res[4] = {r0.x, r0.y, r1.x, r1.y};
@@ -386,9 +386,7 @@ void launch_narrow(const DenseGemm& g, cudaStream_t stream) {
   p.tmem_cols = 32;
   while (p.tmem_cols < p.tile_tok) p.tmem_cols *= 2;
   p.act = g.act;
-  p.limit = g.limit;
-  p.beta = g.beta;
-  p.linear_beta = g.linear_beta;
+  p.kind = g.kind;
   p.bias = g.bias;
   p.residual = g.residual;
   p.out = g.out;

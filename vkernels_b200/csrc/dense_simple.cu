@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(256) dense_simt_kernel(DenseGemm g) {
           g.preact[(int64_t)m * g.ldp + n] = zg;
           g.preact[(int64_t)m * g.ldp + g.N + n] = zu;
         }
-        g.out[(int64_t)m * g.ldo + n] = dense_from_f32<TYPE>(dense_gated(g.act, zg, zu, g.limit, g.beta, g.linear_beta));
+        g.out[(int64_t)m * g.ldo + n] = dense_from_f32<TYPE>(dense_gated(g.kind.act, zg, zu, g.kind));
       }
     } else {
 #pragma unroll
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if constexpr (GATED) {
-            dense_gated_grad(g.act, d[j], zg[i][j], zu[i][j], g.limit, g.beta, g.linear_beta, d[j], du[j]);
+            dense_gated_grad(d[j], zg[i][j], zu[i][j], g.kind, d[j], du[j]);
             su[j] += du[j];
           } else {
             if (g.preact) d[j] *= dense_act_slope(g.act, zg[i][j]);
