@@ -526,3 +526,15 @@ def test_first_call_of_a_process_inside_a_capture():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", _FIRST_CALL.format(root=root)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "replayed" in r.stdout and "refused" in r.stdout and "alive True" in r.stdout, (r.stdout, r.stderr[-2000:])
+
+
+@pytest.mark.parametrize("T,N,gap", [(1, 512, 0), (40, 333, 0), (300, 512, 0), (700, 1000, 8), (600, 333, 0), (520, 770, 3)])
+def test_result_in_place_of_the_residual(T, N, gap):
+    """Every tile reads its part of the residual before it writes it, whichever kernel runs and however the rows lie."""
+    x, w, b, more = tensors(T, 200, N, "bf16")
+    room = more(N + gap)
+    res = room[:, :N]
+    want = ops.fused_linear(x, w, b, activation="gelu", residual=res.clone())
+    beside = room[:, N:].clone()
+    assert torch.equal(ops.fused_linear(x, w, b, activation="gelu", residual=res, out=res), want)
+    assert torch.equal(room[:, N:], beside)

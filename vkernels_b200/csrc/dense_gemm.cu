@@ -1,16 +1,17 @@
-// dense_gemm.cu - products of the dense feed-forward operators on tcgen05: CTA pairs, 256 x 256 tiles.
+// dense_gemm.cu - products of the dense feed-forward operators on tcgen05: CTA pairs, tiles of 256 rows by 64 to 256 columns.
 //
 // out[m, n] = sum_k A[m, k] B[n, k] with either operand contiguous along k or along its own index (the backward products read
 // the weight, x and the gradient as they lie: the tensor map brings 64 x 64 boxes, and the matrix descriptor says which index
-// is contiguous). A pair of CTAs (cta_group::2) works on 256 rows of A and 256 of B: each CTA stages 128 of either in shared
+// is contiguous). A pair of CTAs (cta_group::2) works on 256 rows of A and up to 256 of B: each CTA stages half of either in shared
 // memory (64 k a stage, 128-byte swizzle), one thread of the leader issues the MMAs, each CTA holds its 128 result rows in
-// tensor memory. Two accumulators of 256 columns: eight epilogue warps empty one while the other fills. Persistent, tiles
+// tensor memory. Two accumulators of up to 256 columns: eight epilogue warps empty one while the other fills. Persistent, tiles
 // dealt out in groups of eight row tiles by all column tiles, so that the pairs at work share their operands in L2.
 //
-// In the gated form a tile's 256 rows of B are 128 gate rows (staged by the leader) and the 128 up rows of the same features
-// (staged by its peer): an epilogue thread finds a feature's gate and up sums 128 columns apart in its own lane.
-#include <atomic>
-
+// In the gated form half of a tile's rows of B are gate rows (staged by the leader) and half the up rows of the same features
+// (staged by its peer): an epilogue thread finds a feature's gate and up sums half a tile apart in its own lane.
+//
+// Bound by the tensor cores: 8192 x 7168 -> 2 x 2048 gated takes 299 to 310 us (1.61 to 1.55 PFLOP/s; the tensor pipe is active in
+// 97 % of the SMs' active cycles, DRAM 21 %, L2 44 %), in a loop of seconds under the power cap 357 us (1.35 PFLOP/s).
 #include <algorithm>
 
 #include "dense_tc.cuh"
@@ -177,8 +178,9 @@ __device__ __forceinline__ void row_store_f32(float* p, const float (&z)[16], in
   }
 }
 
-// The epilogue's arithmetic: columns of this thread's row, 16 at a time. Rolled loops on purpose, and one activation to a copy of the code: unrolled over the columns with the choice of activation inside, the last
-// tile of a launch waited 7 us for instructions instead of working 2.
+// The epilogue's arithmetic: columns of this thread's row, 16 at a time. Rolled loops on purpose, and one activation to a copy of
+// the code: unrolled over the columns with the choice of activation inside, the last tile of a launch waited 7 us for
+// instructions instead of working 2.
 template <int TYPE>
 __device__ __forceinline__ void load_bias(float (&b)[2], const uint16_t* p, int cols, int lane) {
 #pragma unroll
