@@ -43,13 +43,11 @@ __device__ __forceinline__ float dense_sigmoid(float v) {
 
 // tanh: beyond 1/4 through the same two instructions, 1 - 2 / (1 + exp(2 y)); below, where that would lose digits, by its
 // Taylor series to y^9 (the first term left out is 9e-9 of the value at 1/4).
-__device__ __forceinline__ float dense_tanh_near(float y) {
-  const float q = y * y;
-  return y * (1.0f + q * (-0.33333333f + q * (0.13333333f + q * (-0.053968254f + q * 0.021869489f))));
-}
 __device__ __forceinline__ float dense_tanh(float y) {
+  const float q = y * y;
+  const float near = y * (1.0f + q * (-0.33333333f + q * (0.13333333f + q * (-0.053968254f + q * 0.021869489f))));
   const float far = 1.0f - 2.0f * dense_sigmoid(-2.0f * y);
-  return fabsf(y) < 0.25f ? dense_tanh_near(y) : far;
+  return fabsf(y) < 0.25f ? near : far;
 }
 // The normal distribution up to z and e = exp(-z^2 / 2): erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x)
 // (Abramowitz and Stegun 7.1.26, off by at most 1.5e-7), x = |z| / sqrt(2); nothing cancels on either side of 0.
@@ -97,28 +95,29 @@ __device__ __forceinline__ float dense_act_slope(int act, float z) {
   }
 }
 
-// tanh(y) as a quotient, e = exp(2 y): n / (e + 1) with n = e - 1, or below 1/4, where that would lose digits, (e + 1) tanh(y)
-// by the series. y is kept below 10, where tanh is 1 to the last bit.
-__device__ __forceinline__ float dense_tanh_parts(float y, float& e) {
-  float top;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(y * 2.8853900817779268f), "f"(28.8539f));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(top));
-  return fabsf(y) < 0.25f ? dense_tanh_near(y) * (e + 1.0f) : e - 1.0f;
+// tanh(y) as a quotient n / (e + 1), e = exp(2 y) = 2^t for t = v k.t_..: n = e - 1, or below 1/32, where that would lose digits,
+// (e + 1) (y - y^3 / 3) (the next term is 1e-7 of the value). t is kept below 29, where tanh is 1 to the last bit.
+__device__ __forceinline__ float dense_tanh_parts(float t, float& e) {
+  constexpr float kHalfLn2 = 0.34657359f;      // y = t ln(2) / 2
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(t) : "f"(29.0f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  const float near = t * fmaf(t * t, -kHalfLn2 * kHalfLn2 * kHalfLn2 / 3.0f, kHalfLn2) * (e + 1.0f);
+  return fabsf(t) < 0.09f ? near : e - 1.0f;
 }
 
-// The gated product of one feature. min.NaN / max.NaN: a NaN stays NaN. SiTU's three quotients -
-// two tanh, one sigmoid - have one reciprocal: three exp2 and it are what the special-function unit does for an element (333 x 2880
-// -> 2880: 19.5 us, 22 with a reciprocal and a division each; SwiGLU 14.3).
+// The gated product of one feature. min.NaN / max.NaN: a NaN stays NaN. SiTU's three quotients - two tanh, one sigmoid - have one
+// reciprocal: three exp2 and it are what the special-function unit does for an element (333 x 2880 -> 2880: a reciprocal and a
+// division for each took 2.5 us longer).
 __device__ __forceinline__ float dense_gated(int act, float g, float u, const GatedKind& k) {
   if (act == 1) {
     float e1, e2, e3 = 0.0f, low, r;
-    const float n1 = dense_tanh_parts(g * k.inv_beta, e1);
+    const float n1 = dense_tanh_parts(g * k.t_beta, e1);
     // exp(-g), finite: what is lost beyond exp(87) is below every 16-bit type's smallest value
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(low) : "f"(g * -1.4426950408889634f), "f"(125.5f));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e2) : "f"(low));
-    const float n3 = k.linear_beta > 0.0f ? k.linear_beta * dense_tanh_parts(u * k.inv_linear_beta, e3) : u;
+    const float n3 = k.linear_beta > 0.0f ? dense_tanh_parts(u * k.t_linear, e3) : u;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((e1 + 1.0f) * (1.0f + e2) * (e3 + 1.0f)));
-    return k.beta * n1 * r * n3;
+    return k.scale * n1 * r * n3;
   }
   const float limit = k.limit, lo = -limit;
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(g) : "f"(limit));

@@ -7,6 +7,9 @@
 // cluster barrier each adds its share of the results over the cluster, rank after rank: no atomics, no scratch in memory, the
 // same bits every time. (Sending the sums to their owner instead needs a barrier more - every ring has to be free first - and
 // took 1 to 5 us longer.)
+//
+// Bound by the start (about 2 us until the first weights arrive) and the join (1 us, 2 to 3 from 64 tokens on) around the weights'
+// way: 8192 -> 8192 24 us for 1 token (134 MB, 5.6 TB/s over all), 7168 -> 2 x 2048 gated 12.8 us (59 MB), 2880 -> 2880 6.4 us (17 MB).
 #include <algorithm>
 
 #include "dense_tc.cuh"
