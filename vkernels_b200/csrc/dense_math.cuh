@@ -95,7 +95,7 @@ __device__ __forceinline__ float dense_act_slope(int act, float z) {
   }
 }
 
-// tanh(y) as a quotient n / (e + 1), e = exp(2 y) = 2^t for t = v k.t_..: n = e - 1, or below 1/32, where that would lose digits,
+// tanh(y) as a quotient n / (e + 1), e = exp(2 y) = 2^t: n = e - 1, or below 1/32, where that would lose digits,
 // (e + 1) (y - y^3 / 3) (the next term is 1e-7 of the value). t is kept below 29, where tanh is 1 to the last bit.
 __device__ __forceinline__ float dense_tanh_parts(float t, float& e) {
   constexpr float kHalfLn2 = 0.34657359f;      // y = t ln(2) / 2
@@ -126,8 +126,8 @@ __device__ __forceinline__ float dense_gated(int act, float g, float u, const Ga
   return g * dense_sigmoid(g) * u;
 }
 // Its gradient with respect to both pre-activations, for the gradient dh of the product.
-__device__ __forceinline__ void dense_gated_grad(float dh, float g, float u, const GatedKind& k, float& dg, float& du) {
-  if (k.act == 1) {
+__device__ __forceinline__ void dense_gated_grad(int act, float dh, float g, float u, const GatedKind& k, float& dg, float& du) {
+  if (act == 1) {
     const bool bent = k.linear_beta > 0.0f;
     const float p = dense_sigmoid(g), a = dense_tanh(g * k.inv_beta), b = bent ? dense_tanh(u * k.inv_linear_beta) : 0.0f;
     const float up = bent ? k.linear_beta * b : u;

@@ -112,8 +112,12 @@ constexpr int kGradRows = 4, kGradStep = 4 * kGradRows;   // rows a thread has o
 // on its way: four rows a thread before the first is worked on, the whole launch resident at once (4096 x 2880 gated: eight
 // columns a thread, one row at a time and three times as many CTAs took 41 us). VEC: a thread's four columns are neighbours, in
 // whole accesses; else 64 apart, so that a warp still reads whole lines of rows that start anywhere.
-template <int TYPE, bool GATED, bool VEC>
+// What is differentiated: the linear activations (DenseAct), then the gated ones. One to a kernel: with the choice inside, every
+// element's code holds them all (4096 x 2880 gelu: 20 us).
+enum GradForm { kGradSwiGlu = 4, kGradSiTu = 5 };
+template <int TYPE, int FORM, bool VEC>
 __global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g, int rows_per_chunk) {
+  constexpr bool GATED = FORM >= kGradSwiGlu, BENT = FORM != kActNone;
   __shared__ float sums[GATED ? 2 : 1][4][kGradCols];
   wait_for_earlier_kernels();
   const int across = threadIdx.x & 63, sub = threadIdx.x >> 6, first = blockIdx.x * kGradCols;
@@ -134,7 +138,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g
         const float* pz = g.preact + r * g.ldp + c0;
         if constexpr (VEC) {
           dy[i] = *reinterpret_cast<const uint2*>(py);
-          if (GATED || g.preact) *reinterpret_cast<float4*>(zg[i]) = *reinterpret_cast<const float4*>(pz);
+          if (BENT) *reinterpret_cast<float4*>(zg[i]) = *reinterpret_cast<const float4*>(pz);
           if constexpr (GATED) *reinterpret_cast<float4*>(zu[i]) = *reinterpret_cast<const float4*>(pz + g.N);
         } else {
           uint16_t v[4];
@@ -142,7 +146,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g
           for (int j = 0; j < 4; ++j) {
             const bool in = c0 + j * 64 < g.N;
             v[j] = in ? py[j * 64] : (uint16_t)0;
-            if (GATED || g.preact) zg[i][j] = in ? pz[j * 64] : 0.0f;
+            if (BENT) zg[i][j] = in ? pz[j * 64] : 0.0f;
             if constexpr (GATED) zu[i][j] = in ? pz[g.N + j * 64] : 0.0f;
           }
           dy[i] = make_uint2(v[0] | ((uint32_t)v[1] << 16), v[2] | ((uint32_t)v[3] << 16));
@@ -157,10 +161,10 @@ __global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if constexpr (GATED) {
-            dense_gated_grad(d[j], zg[i][j], zu[i][j], g.kind, d[j], du[j]);
+            dense_gated_grad(FORM - kGradSwiGlu, d[j], zg[i][j], zu[i][j], g.kind, d[j], du[j]);
             su[j] += du[j];
           } else {
-            if (g.preact) d[j] *= dense_act_slope(g.act, zg[i][j]);
+            if (BENT) d[j] *= dense_act_slope(FORM, zg[i][j]);
           }
           sg[j] += d[j];
         }
@@ -265,14 +269,25 @@ void launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, cudaStream_
   VK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
-template <int TYPE, bool GATED>
-void grad_of_type(const DenseGrad& g, int chunks, cudaStream_t stream) {
+template <int TYPE, int FORM>
+void grad_of_form(const DenseGrad& g, int chunks, cudaStream_t stream) {
   const auto aligned = [](const void* p, int bytes, int64_t ld) { return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0 && ld % 4 == 0); };
   const bool vec = g.N % 4 == 0 && aligned(g.dy, 8, g.lddy) && aligned(g.preact, 16, g.ldp) && aligned(g.dz, 8, g.ldz);
   const dim3 grid((g.N + kGradCols - 1) / kGradCols, chunks);
   const int rows = (g.T + chunks - 1) / chunks;
-  if (vec) launch_overlapped(dense_grad_kernel<TYPE, GATED, true>, grid, kGradThreads, stream, g, rows);
-  else launch_overlapped(dense_grad_kernel<TYPE, GATED, false>, grid, kGradThreads, stream, g, rows);
+  if (vec) launch_overlapped(dense_grad_kernel<TYPE, FORM, true>, grid, kGradThreads, stream, g, rows);
+  else launch_overlapped(dense_grad_kernel<TYPE, FORM, false>, grid, kGradThreads, stream, g, rows);
+}
+template <int TYPE>
+void grad_of_type(const DenseGrad& g, int chunks, cudaStream_t stream) {
+  switch (g.gated ? kGradSwiGlu + g.kind.act : g.preact ? g.act : (int)kActNone) {
+    case kActSilu: grad_of_form<TYPE, kActSilu>(g, chunks, stream); break;
+    case kActGelu: grad_of_form<TYPE, kActGelu>(g, chunks, stream); break;
+    case kActGeluTanh: grad_of_form<TYPE, kActGeluTanh>(g, chunks, stream); break;
+    case kGradSwiGlu: grad_of_form<TYPE, kGradSwiGlu>(g, chunks, stream); break;
+    case kGradSiTu: grad_of_form<TYPE, kGradSiTu>(g, chunks, stream); break;
+    default: grad_of_form<TYPE, kActNone>(g, chunks, stream);
+  }
 }
 
 }  // namespace
@@ -300,13 +315,8 @@ void launch_dense_simt(const DenseGemm& g, cudaStream_t stream) {
 
 void launch_dense_grad(const DenseGrad& g, cudaStream_t stream) {
   const int chunks = dense_sum_chunks(g.T, g.N);
-  if (g.type == kDenseBf16) {
-    if (g.gated) grad_of_type<kDenseBf16, true>(g, chunks, stream);
-    else grad_of_type<kDenseBf16, false>(g, chunks, stream);
-  } else {
-    if (g.gated) grad_of_type<kDenseFp16, true>(g, chunks, stream);
-    else grad_of_type<kDenseFp16, false>(g, chunks, stream);
-  }
+  if (g.type == kDenseBf16) grad_of_type<kDenseBf16>(g, chunks, stream);
+  else grad_of_type<kDenseFp16>(g, chunks, stream);
 }
 
 void launch_dense_sum(DenseType type, const float* partial, int chunks, int cols, uint16_t* db, cudaStream_t stream) {
