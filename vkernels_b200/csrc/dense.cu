@@ -40,23 +40,19 @@ size_t copy_bytes(const void* p, int64_t ld, int rows, int cols) {
   return p == nullptr || tma_ready(p, ld) ? 0 : round_up((size_t)rows * round_up((size_t)cols, 8) * 2, 256);
 }
 
-// x and w as a tensor map takes them: as they are, or copied to rows on 16 bytes at the start of the workspace. Returns the
-// bytes used; a null operand is left alone.
+// x and w as a tensor map takes them: as they are, or as copies in rows on 16 bytes at the start of the workspace, which the caller
+// has made. Returns the bytes used; a null operand is left alone.
 size_t bring_operands(const uint16_t*& x, int64_t& ldx, int T, const uint16_t*& w, int64_t& ldw, int w_rows, int cols, void* workspace,
-                      size_t workspace_bytes, cudaStream_t stream) {
+                      size_t workspace_bytes, RowCopies& c) {
   const size_t bx = copy_bytes(x, ldx, T, cols), bw = copy_bytes(w, ldw, w_rows, cols);
   if (bx + bw == 0) return 0;
   expects(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "dense: workspace must start on 16 bytes");
   expects(workspace_bytes >= bx + bw, "dense: workspace smaller than the copies of x and w that their alignment calls for");
   char* base = static_cast<char*>(workspace);
-  const uint16_t* src[2] = {x, w};
-  const int64_t lds[2] = {ldx, ldw};
-  uint16_t* dst[2] = {bx ? reinterpret_cast<uint16_t*>(base) : nullptr, bw ? reinterpret_cast<uint16_t*>(base + bx) : nullptr};
-  const int rows[2] = {T, w_rows};
-  launch_dense_copy_rows(src, lds, dst, rows, cols, stream);
+  c = {{x, w}, {bx ? reinterpret_cast<uint16_t*>(base) : nullptr, bw ? reinterpret_cast<uint16_t*>(base + bx) : nullptr}, {ldx, ldw}, {T, w_rows}, cols};
   const int64_t pitch = (int64_t)round_up((size_t)cols, 8);
-  if (bx) x = dst[0], ldx = pitch;
-  if (bw) w = dst[1], ldw = pitch;
+  if (bx) x = c.dst[0], ldx = pitch;
+  if (bw) w = c.dst[1], ldw = pitch;
   return bx + bw;
 }
 float effective_limit(int act, float limit) { return act == 0 && limit > 0.0f ? limit : INFINITY; }
@@ -91,7 +87,9 @@ void dense_forward(const DenseForward& f, cudaStream_t stream) {
   if (f.preact) check_preact(f.preact, f.ldp, rows);
   const uint16_t *x = f.x, *w = f.w;
   int64_t ldx = f.ldx, ldw = f.ldw;
-  bring_operands(x, ldx, f.T, w, ldw, rows, f.n_in, f.workspace, f.workspace_bytes, stream);
+  RowCopies copies{};
+  bring_operands(x, ldx, f.T, w, ldw, rows, f.n_in, f.workspace, f.workspace_bytes, copies);
+  launch_dense_copy_rows(copies, stream);
   DenseGemm g{};
   g.type = f.type;
   g.a = {x, ldx, false};
@@ -154,7 +152,8 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
     expects(f.workspace != nullptr && (reinterpret_cast<uintptr_t>(f.workspace) & 15u) == 0, "dense: workspace must start on 16 bytes");
     expects(f.workspace_bytes >= copies + dz_bytes + sums_bytes, "dense: workspace smaller than vk_cuda_dense_backward_workspace_bytes");
   }
-  bring_operands(x, ldx, f.T, w, ldw, rows, f.n_in, f.workspace, f.workspace_bytes, stream);
+  RowCopies made{};
+  bring_operands(x, ldx, f.T, w, ldw, rows, f.n_in, f.workspace, f.workspace_bytes, made);
   uint16_t* dz = need_dz ? reinterpret_cast<uint16_t*>(static_cast<char*>(f.workspace) + copies) : nullptr;
   if (need_dz || f.db) {
     float* partial = f.db ? reinterpret_cast<float*>(static_cast<char*>(f.workspace) + copies + dz_bytes) : nullptr;
@@ -174,8 +173,11 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
     g.gated = f.gated;
     g.act = f.act;
     if (f.gated) g.kind = gated_kind(f.act, effective_limit(f.act, f.limit), f.beta, f.linear_beta);
+    g.copies = made;
     launch_dense_grad(g, stream);
     if (f.db && chunks > 1) launch_dense_sum(f.type, partial, chunks, rows, f.db, stream);
+  } else {
+    launch_dense_copy_rows(made, stream);
   }
   const uint16_t* z = need_dz ? dz : f.dy;
   const int64_t ldzz = need_dz ? ldz : f.lddy;

@@ -52,6 +52,14 @@ struct DenseGemm {
   int64_t ldp;
 };
 
+// dst[i][r, c] = src[i][r, c] for up to two matrices (dst[i] not null), rows of dst one after the other, each on 16 bytes.
+struct RowCopies {
+  const uint16_t* src[2];
+  uint16_t* dst[2];
+  int64_t lds[2];
+  int rows[2], cols;
+};
+
 // Gradient of the pre-activations: dz = dy * act'(z), [T, rows] (linear) or [T, 2 ispp] (gated) at pitch ldz; with no
 // activation a copy of dy. dz may be null (only the column sums are wanted). partial (optional) receives the column sums of
 // each chunk of rows in fp32, [dense_sum_chunks(T, N), rows]; of a single chunk db receives them at once, in the type.
@@ -69,6 +77,7 @@ struct DenseGrad {
   bool gated;
   int act;                    // linear: DenseAct
   GatedKind kind;             // gated
+  RowCopies copies;           // made by the same launch
 };
 
 int dense_sum_chunks(int T, int n_out);
@@ -82,8 +91,7 @@ void launch_dense_simt(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_grad(const DenseGrad& g, cudaStream_t stream);
 // db[n] = sum over the chunks of partial[chunk, n], in order.
 void launch_dense_sum(DenseType type, const float* partial, int chunks, int cols, uint16_t* db, cudaStream_t stream);
-// dst[i][r, c] = src[i][r, c] for up to two matrices (dst[i] not null), rows of dst one after the other, each on 16 bytes.
-void launch_dense_copy_rows(const uint16_t* const* src, const int64_t* lds, uint16_t* const* dst, const int* rows, int cols, cudaStream_t stream);
+void launch_dense_copy_rows(const RowCopies& c, cudaStream_t stream);
 
 // ---- the operators ----
 struct DenseForward {

@@ -46,8 +46,8 @@ struct WideParams {           // one product
   uint16_t* out;
   float* preact;
   int64_t ldr, ldo, ldp;
-  int direct;                 // rows of result and residual start on 16 bytes, those of preact on 32
-  int wide_o;                 // ... and the result's on 32
+  int direct;                 // rows of result and residual start on 16 bytes
+  int wide_o, wide_p;         // rows of the result, of preact start on 32
 };
 template <int COUNT>
 struct WideLaunch {           // one product, or two that do not depend on each other: the tiles of the second follow the first's
@@ -87,7 +87,8 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 }
 __device__ __forceinline__ void sts16(uint32_t addr, uint16_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory"); }
 // Rows that start anywhere go through the staging buffer: rows x cols (at most 32 x 64), a row at a time, a value a lane; on the
-// way in, sixteen rows are fetched before the first is put down.
+// way in, sixteen rows are fetched before the first is put down. (A word a lane where the row allows it was slower: the row's
+// parity makes three cases of every access.)
 __device__ __forceinline__ void values_in(uint32_t base, const uint16_t* p, int64_t ld, int rows, int cols, int lane) {
 #pragma unroll 1
   for (int first = 0; first < 32; first += 16) {
@@ -240,7 +241,7 @@ __device__ __forceinline__ void linear_columns(uint32_t tz, int width, uint32_t 
     float z[16];
     load_columns(z, tz + block * 16);
     if (has_bias) add_bias(z, bias, block);
-    if (DIRECT && at.preact) row_store_f32(at.preact + block * 16, z, n);
+    if (at.preact) row_store_f32(at.preact + block * 16, z, n);
     if (ACT != kActNone) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) z[j] = dense_act(ACT, z[j]);
@@ -282,7 +283,7 @@ __device__ __forceinline__ void gated_columns(uint32_t tg, uint32_t tu, int widt
       add_bias(g, bias_g, block);
       add_bias(u, bias_u, block);
     }
-    if (DIRECT && at.preact) {
+    if (at.preact) {
       row_store_f32(at.preact + block * 16, g, n);
       row_store_f32(at.preact_up + block * 16, u, n);
     }
@@ -471,14 +472,16 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
         if (any) {
           RowPlace at{};
           at.cols = cols;
+          if (row_ok) at.out = p.out + row * p.ldo + col0;
+          if (row_ok && p.preact && p.wide_p) {
+            at.preact = p.preact + row * p.ldp + col0;
+            at.preact_up = at.preact + p.N;
+          }
+          if (p.preact && !p.wide_p) {
+            preact_anywhere(tz, width, staging, bias, has_bias, p.preact + row0 * p.ldp + col0, p.ldp, rows, cols, lane);
+            if (GATED) preact_anywhere(tu, width, staging, bias_u, has_bias, p.preact + row0 * p.ldp + p.N + col0, p.ldp, rows, cols, lane);
+          }
           if (p.direct) {
-            if (row_ok) {
-              at.out = p.out + row * p.ldo + col0;
-              if (p.preact) {
-                at.preact = p.preact + row * p.ldp + col0;
-                at.preact_up = at.preact + p.N;
-              }
-            }
             if constexpr (GATED) {
               if (p.kind.act == 1) gated_columns<TYPE, 1, true>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
               else gated_columns<TYPE, 0, true>(tz, tu, width, staging, bias, bias_u, has_bias, at, p, lane);
@@ -492,10 +495,6 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
               linear_columns<TYPE, true>(tz, width, staging, bias, has_bias, p.residual != nullptr, at, p, lane);
             }
           } else {
-            if (p.preact) {
-              preact_anywhere(tz, width, staging, bias, has_bias, p.preact + row0 * p.ldp + col0, p.ldp, rows, cols, lane);
-              if (GATED) preact_anywhere(tu, width, staging, bias_u, has_bias, p.preact + row0 * p.ldp + p.N + col0, p.ldp, rows, cols, lane);
-            }
             if (!GATED && p.residual) {
               values_in(staging, p.residual + row0 * p.ldr + col0, p.ldr, rows, cols, lane);
               __syncwarp();
@@ -614,8 +613,8 @@ void describe(const DenseGemm& g, int bn, WideParams& p, CUtensorMap& a, CUtenso
   p.ldo = g.ldo;
   p.ldp = g.ldp;
   const auto on = [](const void* q, int64_t ld_bytes, int bytes) { return ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)ld_bytes) & (uintptr_t)(bytes - 1)) == 0; };
-  p.direct = on(g.out, g.ldo * 2, 16) && (g.residual == nullptr || on(g.residual, g.ldr * 2, 16)) &&
-             (g.preact == nullptr || (on(g.preact, g.ldp * 4, 32) && (!GATED || g.N % 8 == 0)));
+  p.direct = on(g.out, g.ldo * 2, 16) && (g.residual == nullptr || on(g.residual, g.ldr * 2, 16));
+  p.wide_p = on(g.preact, g.ldp * 4, 32) && (!GATED || g.N % 8 == 0);
   const bool whole = (GATED ? p.bn / 4 : p.bn / 2) % 16 == 0;   // every warp's columns start on 32 bytes of a row that does
   p.wide_o = whole && on(g.out, g.ldo * 2, 32);
   a = operand_map(g.a, g.M, g.K, 128);

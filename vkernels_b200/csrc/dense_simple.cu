@@ -88,19 +88,47 @@ __global__ void __launch_bounds__(256) dense_simt_kernel(DenseGemm g) {
   }
 }
 
-// Eight neighbouring values of a row, as one 16-byte access where the row allows it.
+// Eight neighbouring values of a row.
 struct Eight {
   uint16_t v[8];
 };
-__device__ __forceinline__ Eight load_eight(const uint16_t* p, int n, bool vec) {
+// Eight values from an address that is a multiple of 2: from the words around them where the row goes on behind them.
+__device__ __forceinline__ Eight load_eight_words(const uint16_t* p, int n) {
   Eight e;
-  if (vec && n >= 8) {
-    *reinterpret_cast<uint4*>(e.v) = *reinterpret_cast<const uint4*>(p);
-  } else {
+  if (n <= 8) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) e.v[j] = j < n ? p[j] : (uint16_t)0;
+    return e;
   }
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
+  const bool odd = (reinterpret_cast<uintptr_t>(p) & 2u) != 0;
+  uint32_t v[5];
+#pragma unroll
+  for (int j = 1; j < 4; ++j) v[j] = w[j];
+  v[0] = odd ? (uint32_t)p[0] << 16 : w[0];
+  v[4] = odd ? w[4] : 0u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(e.v)[j] = odd ? __funnelshift_r(v[j], v[j + 1], 16) : v[j];
   return e;
+}
+// Copies of rows, as the `part`-th of `parts` CTAs of 256 threads: dst[r, c] = src[r, c], rows of dst on 16 bytes, filled up to whole
+// units of 8.
+__device__ __forceinline__ void copy_rows(const RowCopies& c, int part, int parts) {
+  const int units = (c.cols + 7) / 8;
+  const int64_t first = c.dst[0] != nullptr ? (int64_t)c.rows[0] * units : 0;
+  const int64_t all = first + (c.dst[1] != nullptr ? (int64_t)c.rows[1] * units : 0), step = (int64_t)parts * 256;
+#pragma unroll 2
+  for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < all; i += step) {
+    const int z = i >= first;
+    const int64_t at = z ? i - first : i;
+    const int r = all < (1ll << 31) ? (int)((uint32_t)at / (uint32_t)units) : (int)(at / units), u = (int)(at - (int64_t)r * units);
+    const Eight e = load_eight_words(c.src[z] + r * c.lds[z] + u * 8, c.cols - u * 8);
+    *reinterpret_cast<uint4*>(c.dst[z] + at * 8) = *reinterpret_cast<const uint4*>(e.v);
+  }
+}
+__global__ void __launch_bounds__(256) dense_copy_rows_kernel(RowCopies c) {
+  wait_for_earlier_kernels();
+  copy_rows(c, blockIdx.x, gridDim.x);
 }
 
 constexpr int kGradCols = 256, kGradThreads = 256;   // 64 threads across the columns, four each; four rows at a time
@@ -116,10 +144,14 @@ constexpr int kGradRows = 4, kGradStep = 4 * kGradRows;   // rows a thread has o
 // element's code holds them all (4096 x 2880 gelu: 20 us).
 enum GradForm { kGradSwiGlu = 4, kGradSiTu = 5 };
 template <int TYPE, int FORM, bool VEC>
-__global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g, int rows_per_chunk) {
+__global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g, int rows_per_chunk, int chunks) {
   constexpr bool GATED = FORM >= kGradSwiGlu, BENT = FORM != kActNone;
   __shared__ float sums[GATED ? 2 : 1][4][kGradCols];
   wait_for_earlier_kernels();
+  if ((int)blockIdx.y >= chunks) {   // operands of the products to rows on 16 bytes, on the way
+    copy_rows(g.copies, (blockIdx.y - chunks) * gridDim.x + blockIdx.x, (gridDim.y - chunks) * gridDim.x);
+    return;
+  }
   const int across = threadIdx.x & 63, sub = threadIdx.x >> 6, first = blockIdx.x * kGradCols;
   const int r_end = min(g.T, (int)(blockIdx.y + 1) * rows_per_chunk);
   const auto column = [&](int j) { return VEC ? across * 4 + j : across + j * 64; };
@@ -222,40 +254,6 @@ __global__ void __launch_bounds__(64) dense_sum_kernel(const float* __restrict__
   db[c] = dense_from_f32<TYPE>(s);
 }
 
-// dst[r, c] = src[r, c] for two matrices at once (grid z), rows of dst on 16 bytes, filled up with zeros to whole units of 8.
-struct RowCopies {
-  const uint16_t* src[2];
-  uint16_t* dst[2];
-  int64_t lds[2];
-  int rows[2];
-};
-// Eight values from an address that is a multiple of 2: from the words around them where the row goes on behind them.
-__device__ __forceinline__ Eight load_eight_words(const uint16_t* p, int n) {
-  if (n <= 8) return load_eight(p, n, false);
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
-  const bool odd = (reinterpret_cast<uintptr_t>(p) & 2u) != 0;
-  uint32_t v[5];
-#pragma unroll
-  for (int j = 1; j < 4; ++j) v[j] = w[j];
-  v[0] = odd ? (uint32_t)p[0] << 16 : w[0];
-  v[4] = odd ? w[4] : 0u;
-  Eight e;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(e.v)[j] = odd ? __funnelshift_r(v[j], v[j + 1], 16) : v[j];
-  return e;
-}
-__global__ void __launch_bounds__(256) dense_copy_rows_kernel(RowCopies c, int cols) {
-  wait_for_earlier_kernels();
-  const int z = blockIdx.z, units = (cols + 7) / 8;
-  const int64_t all = (int64_t)c.rows[z] * units, step = (int64_t)gridDim.x * 256;
-#pragma unroll 2
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
-    const int r = (int)(i / units), u = (int)(i - (int64_t)r * units);
-    const Eight e = load_eight_words(c.src[z] + r * c.lds[z] + u * 8, cols - u * 8);
-    *reinterpret_cast<uint4*>(c.dst[z] + i * 8) = *reinterpret_cast<const uint4*>(e.v);
-  }
-}
-
 template <class... P, class... A>
 void launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t stream, A... args) {
   cudaLaunchConfig_t cfg{};
@@ -269,14 +267,23 @@ void launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, cudaStream_
   VK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
+// CTAs for copies: two units of eight values a thread, eight CTAs an SM at most.
+int copy_ctas(const RowCopies& c) {
+  int64_t units = 0;
+  for (int i = 0; i < 2; ++i)
+    if (c.dst[i] != nullptr) units += (int64_t)c.rows[i] * ((c.cols + 7) / 8);
+  return (int)std::min<int64_t>((units + 511) / 512, 8 * 148);
+}
+
 template <int TYPE, int FORM>
 void grad_of_form(const DenseGrad& g, int chunks, cudaStream_t stream) {
   const auto aligned = [](const void* p, int bytes, int64_t ld) { return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0 && ld % 4 == 0); };
   const bool vec = g.N % 4 == 0 && aligned(g.dy, 8, g.lddy) && aligned(g.preact, 16, g.ldp) && aligned(g.dz, 8, g.ldz);
-  const dim3 grid((g.N + kGradCols - 1) / kGradCols, chunks);
+  const int across = (g.N + kGradCols - 1) / kGradCols;
+  const dim3 grid(across, chunks + (copy_ctas(g.copies) + across - 1) / across);
   const int rows = (g.T + chunks - 1) / chunks;
-  if (vec) launch_overlapped(dense_grad_kernel<TYPE, FORM, true>, grid, kGradThreads, stream, g, rows);
-  else launch_overlapped(dense_grad_kernel<TYPE, FORM, false>, grid, kGradThreads, stream, g, rows);
+  if (vec) launch_overlapped(dense_grad_kernel<TYPE, FORM, true>, grid, kGradThreads, stream, g, rows, chunks);
+  else launch_overlapped(dense_grad_kernel<TYPE, FORM, false>, grid, kGradThreads, stream, g, rows, chunks);
 }
 template <int TYPE>
 void grad_of_type(const DenseGrad& g, int chunks, cudaStream_t stream) {
@@ -325,19 +332,9 @@ void launch_dense_sum(DenseType type, const float* partial, int chunks, int cols
   else launch_overlapped(dense_sum_kernel<kDenseFp16>, grid, 64, stream, partial, chunks, cols, db);
 }
 
-void launch_dense_copy_rows(const uint16_t* const* src, const int64_t* lds, uint16_t* const* dst, const int* rows, int cols, cudaStream_t stream) {
-  RowCopies c{};
-  int n = 0, most = 0;
-  for (int i = 0; i < 2; ++i)
-    if (dst[i] != nullptr) {
-      c.src[n] = src[i], c.lds[n] = lds[i], c.dst[n] = dst[i], c.rows[n] = rows[i];
-      most = rows[i] > most ? rows[i] : most;
-      ++n;
-    }
-  if (n == 0) return;
-  const int64_t units = (int64_t)most * ((cols + 7) / 8);
-  const dim3 grid((unsigned)std::min<int64_t>((units + 511) / 512, 8 * 148), 1, n);
-  launch_overlapped(dense_copy_rows_kernel, grid, 256, stream, c, cols);
+void launch_dense_copy_rows(const RowCopies& c, cudaStream_t stream) {
+  const int ctas = copy_ctas(c);
+  if (ctas > 0) launch_overlapped(dense_copy_rows_kernel, dim3(ctas), 256, stream, c);
 }
 
 }  // namespace vkernels::kernels::cuda

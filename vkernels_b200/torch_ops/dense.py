@@ -184,6 +184,13 @@ def _result(out, out2, shape, x):
     return out, out2
 
 
+def _new_preact(x, T, rows):
+    """Room for fp32 pre-activations [T, rows], each row on 32 bytes."""
+    if rows & 7:
+        return x.new_empty((T, (rows + 7) // 8 * 8), dtype=torch.float32)[:, :rows]
+    return x.new_empty((T, rows), dtype=torch.float32)
+
+
 def _forward_work(x, ldx, w, ldw, T, n_in, rows):
     """(tensor to keep, pointer, bytes) of the room for copies of x and w, where their alignment calls for them."""
     if not (x.data_ptr() & 15 or w.data_ptr() & 15 or ldx & 7 or ldw & 7):
@@ -226,9 +233,9 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, b13: torch.Tensor | None = 
                 and (b13 is None or _plain(b13, wshape[:1], dtype, index)) and not _wants_grad(x, w13, b13)):
             T, rows = shape[0], wshape[0]
             h = x.new_empty((T, rows // 2))
-            preact = x.new_empty((T, rows), dtype=torch.float32) if return_preact else None
+            preact = _new_preact(x, T, rows) if return_preact else None
             _call("vk_cuda_gated_linear", index, x.data_ptr(), shape[1], w13.data_ptr(), shape[1], None if b13 is None else b13.data_ptr(),
-                  h.data_ptr(), rows // 2, None if preact is None else preact.data_ptr(), rows, _DTYPE[dtype], T, shape[1], rows // 2,
+                  h.data_ptr(), rows // 2, None if preact is None else preact.data_ptr(), (rows + 7) // 8 * 8, _DTYPE[dtype], T, shape[1], rows // 2,
                   activation, swiglu_limit, beta, linear_beta, None, 0)
             return (h, preact) if return_preact else h
     x2 = _inputs(x, w13, True, "gated_linear")
@@ -245,11 +252,11 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, b13: torch.Tensor | None = 
             raise OpNotEligible("gated_linear: out and return_preact are for calls that record no gradient")
         return _GatedLinear.apply(x, w13, b13, activation, swiglu_limit, beta, linear_beta)
     h, h2 = _result(out, out2, shape, x)
-    preact = x.new_empty((T, rows), dtype=torch.float32) if return_preact else None
+    preact = _new_preact(x, T, rows) if return_preact else None
     if T > 0:
         work, wp, nbytes = _forward_work(x2, ldx, w13, ldw, T, hidden, rows)
         _call("vk_cuda_gated_linear", x.get_device(), x2.data_ptr(), ldx, w13.data_ptr(), ldw, b, h2.data_ptr(), _pitch("out", h2),
-              None if preact is None else preact.data_ptr(), rows, _DTYPE[x.dtype], T, hidden, ispp, activation, swiglu_limit, beta,
+              None if preact is None else preact.data_ptr(), (rows + 7) // 8 * 8, _DTYPE[x.dtype], T, hidden, ispp, activation, swiglu_limit, beta,
               linear_beta, wp, nbytes)
     return (h, preact) if return_preact else h
 
@@ -296,10 +303,10 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
                 and not _wants_grad(x, w, bias, residual)):
             T, n_in, n_out = shape[0], shape[1], wshape[0]
             y = x.new_empty((T, n_out))
-            preact = x.new_empty((T, n_out), dtype=torch.float32) if return_preact and act else None
+            preact = _new_preact(x, T, n_out) if return_preact and act else None
             _call("vk_cuda_fused_linear", index, x.data_ptr(), n_in, w.data_ptr(), n_in, None if bias is None else bias.data_ptr(),
                   None if residual is None else residual.data_ptr(), n_out, y.data_ptr(), n_out,
-                  None if preact is None else preact.data_ptr(), n_out, _DTYPE[dtype], T, n_in, n_out, act, None, 0)
+                  None if preact is None else preact.data_ptr(), (n_out + 7) // 8 * 8, _DTYPE[dtype], T, n_in, n_out, act, None, 0)
             return (y, preact) if return_preact else y
     x2 = _inputs(x, w, False, "fused_linear")
     n_out = w.shape[0]
@@ -324,11 +331,11 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
         return _FusedLinear.apply(x, w, bias, residual, activation)
     T, n_in = x2.shape
     y, y2 = _result(out, out2, shape, x)
-    preact = x.new_empty((T, n_out), dtype=torch.float32) if return_preact and act else None
+    preact = _new_preact(x, T, n_out) if return_preact and act else None
     if T > 0:
         work, wp, nbytes = _forward_work(x2, ldx, w, ldw, T, n_in, n_out)
         _call("vk_cuda_fused_linear", x.get_device(), x2.data_ptr(), ldx, w.data_ptr(), ldw, b, None if r2 is None else r2.data_ptr(), ldr,
-              y2.data_ptr(), _pitch("out", y2), None if preact is None else preact.data_ptr(), n_out, _DTYPE[x.dtype], T, n_in, n_out,
+              y2.data_ptr(), _pitch("out", y2), None if preact is None else preact.data_ptr(), (n_out + 7) // 8 * 8, _DTYPE[x.dtype], T, n_in, n_out,
               act, wp, nbytes)
     return (y, preact) if return_preact else y
 
