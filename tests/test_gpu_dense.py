@@ -6,6 +6,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 import dense_oracle as ref  # noqa: E402
+from vkernels_b200 import native_runtime as nr  # noqa: E402
 from vkernels_b200 import torch_ops as ops  # noqa: E402
 
 DEV = "cuda:0"
@@ -114,6 +115,60 @@ def test_fused_linear_backward(T, K, N, dtype, impl):
             dz, error = d * slope, ref.APPROX * d.abs() * (1 + z.abs())
         for name, t, (value, bound) in zip(("dx", "dw", "db"), got, ref.gradients(dz, error, x, w, x.dtype, impl)):
             ref.assert_within(t, value, bound, f"{name} {act}")
+
+
+# One gradient with few tiles and a long sum (many tokens of few features, or a few features behind many), beside another or alone.
+LONG = [(4100, 128, 96), (9001, 70, 300), (100, 64, 4500), (300, 33, 2300), (2600, 250, 2500), (16384, 64, 64), (1, 40, 5000)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,K,N", LONG)
+def test_gradients_of_long_sums(T, K, N, dtype):
+    for gated, gap in ((False, 0), (False, 3), (True, 0)):
+        x, w, b, more = tensors(T, K, 2 * N if gated else N, dtype, gap=gap)
+        dy = more(N + gap)[:, :N]
+        d = dy.double()
+        if gated:
+            _, preact = ops.gated_linear(x, w, b, return_preact=True)
+            _, dg, du, _, mg, mu = ref.gated(preact.double(), "swiglu", 0.0)
+            dz, error = torch.cat([d * dg, d * du], 1), ref.APPROX * torch.cat([d.abs() * mg, d.abs() * mu], 1)
+            call = lambda **kw: ops.gated_linear_backward(dy, x, w, preact, **kw)  # noqa: E731
+        else:
+            dz, error = d, torch.zeros_like(d)
+            call = lambda **kw: ops.fused_linear_backward(dy, x, w, **kw)  # noqa: E731
+        wanted = ref.gradients(dz, error, x, w, x.dtype, "tcgen05")
+        both = call(bias_grad=True)
+        for name, t, (value, bound) in zip(("dx", "dw", "db"), both, wanted):
+            ref.assert_within(t, value, bound, f"{name} {gated} {gap}")
+        ref.assert_within(call(w_grad=False)[0], *wanted[0], "dx alone")
+        ref.assert_within(call(x_grad=False)[1], *wanted[1], "dw alone")
+        assert all(torch.equal(p, q) for p, q in zip(call(bias_grad=True), both))
+    torch.cuda.synchronize()
+    ops.kernel_status()
+
+
+def test_parts_of_long_sums_in_a_workspace_on_16_bytes():
+    """The sums' parts lie behind one another from the workspace's start on, which need not be a 32-byte one; nothing behind its end
+    is written, nor beside the gradients."""
+    T, K, N = 5000, 100, 90
+    x, w, _, more = tensors(T, K, N, "bf16", bias=False, gap=4)   # pitches of 104
+    dy = more(N + 6)[:, :N]                                       # 96
+    wanted = ops.fused_linear_backward(dy, x, w)[1]
+    lib = nr.load_library()
+    nbytes = lib.vk_cuda_dense_backward_workspace_bytes(x.data_ptr(), 104, w.data_ptr(), 104, T, K, N, 0)
+    room = torch.full((nbytes + 64,), 7, dtype=torch.uint8, device=DEV)
+    assert room.data_ptr() % 256 == 0
+    dw = torch.full((N, 107), 3.0, dtype=torch.bfloat16, device=DEV)
+    torch.cuda.synchronize()
+    rc = lib.vk_cuda_fused_linear_backward(dy.data_ptr(), 96, x.data_ptr(), 104, w.data_ptr(), 104, None, 0, None, K, dw.data_ptr(), 107,
+                                           None, 0, T, K, N, 0, room.data_ptr() + 16, nbytes, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, lib.vk_last_error()
+    torch.cuda.synchronize()
+    assert torch.equal(dw[:, :K], wanted) and bool((dw[:, K:] == 3).all())
+    assert bool((room[:16] == 7).all()) and bool((room[16 + nbytes:] == 7).all())
+    assert lib.vk_cuda_fused_linear_backward(dy.data_ptr(), 96, x.data_ptr(), 104, w.data_ptr(), 104, None, 0, None, K, dw.data_ptr(), 107,
+                                             None, 0, T, K, N, 0, room.data_ptr(), 4096, torch.cuda.current_stream().cuda_stream) == 1
+    lib.vk_set_last_error(0, b"")
 
 
 # ---------------------------------------------------------------------------

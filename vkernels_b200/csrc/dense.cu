@@ -107,14 +107,17 @@ void dense_forward(const DenseForward& f, cudaStream_t stream) {
   g.ldo = f.ldy;
   g.preact = f.preact;
   g.ldp = f.ldp;
+  g.split = 1;
   launch_dense_gemm(g, stream);
 }
 
 size_t dense_backward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int n_out, bool gated) {
   expects(T >= 0 && n_in > 0 && n_out > 0, "dense: T must not be negative, feature counts must be positive");
   const size_t rows = (gated ? 2 : 1) * (size_t)n_out;
+  if (T == 0) return 0;
   return copy_bytes(x, ldx, T, n_in) + copy_bytes(w, ldw, (int)rows, n_in) + round_up((size_t)T * round_up(rows, 8) * 2, 256) +
-         (size_t)dense_sum_chunks(T, n_out) * rows * 4;
+         round_up((size_t)dense_sum_chunks(T, n_out) * rows * 4, 256) + dense_parts_bytes(T, n_in, dense_split(T, n_in, (int)rows)) +
+         dense_parts_bytes((int)rows, n_in, dense_split((int)rows, n_in, T));
 }
 
 void dense_backward(const DenseBackward& f, cudaStream_t stream) {
@@ -146,11 +149,15 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
   int64_t ldx = f.ldx, ldw = f.ldw;
   const int64_t ldz = (int64_t)round_up((size_t)rows, 8);
   const size_t dz_bytes = need_dz ? round_up((size_t)f.T * ldz * 2, 256) : 0;
-  const size_t sums_bytes = f.db ? (size_t)dense_sum_chunks(f.T, f.n_out) * rows * 4 : 0;
+  const size_t sums_bytes = f.db ? round_up((size_t)dense_sum_chunks(f.T, f.n_out) * rows * 4, 256) : 0;
   const size_t copies = copy_bytes(x, ldx, f.T, f.n_in) + copy_bytes(w, ldw, rows, f.n_in);
-  if (copies + dz_bytes + sums_bytes > 0) {
+  const bool cut = get_moe_impl() != MoeImpl::kSimt;
+  const int split_x = f.dx && cut ? dense_split(f.T, f.n_in, rows) : 1, split_w = f.dw && cut ? dense_split(rows, f.n_in, f.T) : 1;
+  const size_t parts_x = dense_parts_bytes(f.T, f.n_in, split_x), parts_w = dense_parts_bytes(rows, f.n_in, split_w);
+  const size_t needed = copies + dz_bytes + sums_bytes + parts_x + parts_w;
+  if (needed > 0) {
     expects(f.workspace != nullptr && (reinterpret_cast<uintptr_t>(f.workspace) & 15u) == 0, "dense: workspace must start on 16 bytes");
-    expects(f.workspace_bytes >= copies + dz_bytes + sums_bytes, "dense: workspace smaller than vk_cuda_dense_backward_workspace_bytes");
+    expects(f.workspace_bytes >= needed, "dense: workspace smaller than vk_cuda_dense_backward_workspace_bytes");
   }
   RowCopies made{};
   bring_operands(x, ldx, f.T, w, ldw, rows, f.n_in, f.workspace, f.workspace_bytes, made);
@@ -183,6 +190,10 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
   const int64_t ldzz = need_dz ? ldz : f.lddy;
   DenseGemm gx{}, gw{};
   gx.type = gw.type = f.type;
+  gx.split = split_x;
+  gw.split = split_w;
+  gx.parts = reinterpret_cast<float*>(static_cast<char*>(f.workspace) + copies + dz_bytes + sums_bytes);
+  gw.parts = reinterpret_cast<float*>(reinterpret_cast<char*>(gx.parts) + parts_x);
   if (f.dx) {   // dx[t, i] = sum_n dz[t, n] w[n, i]
     gx.a = {z, ldzz, false};
     gx.b = {w, ldw, true};

@@ -50,6 +50,10 @@ struct DenseGemm {
   int64_t ldo;
   float* preact;              // or null
   int64_t ldp;
+  // k in `split` parts, if more than one: the sums of each part go to `parts`, [split][M, dense_part_pitch(N)] fp32, and out is made of
+  // them by launch_dense_join. Plain linear products only.
+  int split;
+  float* parts;
 };
 
 // dst[i][r, c] = src[i][r, c] for up to two matrices (dst[i] not null), rows of dst one after the other, each on 16 bytes.
@@ -81,6 +85,12 @@ struct DenseGrad {
 };
 
 int dense_sum_chunks(int T, int n_out);
+// Parts that k is cut into where a plain product has fewer tiles than a third of the CTA pairs and k is long.
+int dense_split(int M, int N, int K);
+inline int64_t dense_part_pitch(int N) { return ((int64_t)N + 7) / 8 * 8; }
+inline size_t dense_parts_bytes(int M, int N, int split) { return split > 1 ? (size_t)split * (size_t)M * (size_t)dense_part_pitch(N) * 4 : 0; }
+// out = the parts' sum, in order, of up to two products (split > 1).
+void launch_dense_join(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_wide(const DenseGemm& g, cudaStream_t stream);   // dense_gemm.cu
 void launch_dense_wide_two(const DenseGemm& g, const DenseGemm& h, cudaStream_t stream);

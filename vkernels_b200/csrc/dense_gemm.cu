@@ -39,11 +39,13 @@ struct WideParams {           // one product
   int bn;                     // rows of B a tile: a multiple of 32 from 64 to 256
   int stage_bytes;            // of one CTA: what the copies of a stage bring
   int tiles_m, tiles_n, n_tiles, k_blocks;
+  int split, part_tiles;      // parts of k, tiles of one part (the parts' tiles follow one another)
+  int64_t plane;              // from one part's sums to the next's
   int act;
   GatedKind kind;
   const uint16_t* bias;
   const uint16_t* residual;
-  uint16_t* out;
+  uint16_t* out;              // null: the sums of every part to preact
   float* preact;
   int64_t ldr, ldo, ldp;
   int direct;                 // rows of result and residual start on 16 bytes
@@ -346,11 +348,13 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
   const uint32_t tmem_base = bars->tmem_base;
   wait_for_earlier_kernels();
   const int unit = blockIdx.x >> 1, n_units = gridDim.x >> 1;
-  // which product tile t belongs to, and where it lies there
-  const auto place = [&](int t, int& tm, int& tn) {
+  // which product tile t belongs to, and where and of which part of k it lies there
+  const auto place = [&](int t, int& tm, int& tn, int& part) {
     const int which = COUNT > 1 && t >= work.p[0].n_tiles;
     const WideParams& p = work.p[which];
     if (which) t -= work.p[0].n_tiles;
+    part = p.split > 1 ? t / p.part_tiles : 0;
+    t -= part * p.part_tiles;
     const int per_group = kGroupM * p.tiles_n, first = t / per_group * kGroupM, in = t % per_group, high = min(kGroupM, p.tiles_m - first);
     tm = first + in % high;
     tn = in / high;
@@ -364,15 +368,16 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
       long long issued = 0;
       bool go = true;
       for (int t = unit; t < work.n_tiles && go; t += n_units) {
-        int tm, tn;
-        const int which = place(t, tm, tn);
+        int tm, tn, part;
+        const int which = place(t, tm, tn, part);
         const WideParams& p = work.p[which];
+        const int kb0 = (int)((int64_t)p.k_blocks * part / p.split), kb1 = (int)((int64_t)p.k_blocks * (part + 1) / p.split);
         const CUtensorMap *map_a = &work.a[which], *map_b = &work.b[which];
         // kept in registers: of two products, each look into the parameters would be an indexed load
-        const int a_mn = p.a_mn, b_mn = p.b_mn, b_wide = p.bn > 128, k_blocks = p.k_blocks, pair_bytes = 2 * p.stage_bytes;
+        const int a_mn = p.a_mn, b_mn = p.b_mn, b_wide = p.bn > 128, pair_bytes = 2 * p.stage_bytes;
         const int m0 = tm * 256 + (int)rank * 128;
         const int n0 = GATED ? tn * (p.bn / 2) + (int)rank * p.N : tn * p.bn + (int)rank * (p.bn / 2);
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           const uint32_t full = smem_u32(&bars->full[s.slot]), dst = ring + s.slot * kStageBytes;
           if (!mbar_wait(smem_u32(&bars->empty[s.slot]), s.phase ^ 1u, abort_flag, 51)) {
             go = false;
@@ -410,15 +415,17 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
       int it = 0;
       bool go = true;
       for (int t = unit; t < work.n_tiles && go; t += n_units, ++it) {
-        const WideParams& p = work.p[COUNT > 1 && t >= work.p[0].n_tiles];
-        const int a_mn = p.a_mn, b_mn = p.b_mn, k_blocks = p.k_blocks;
+        int tm, tn, part;
+        const WideParams& p = work.p[place(t, tm, tn, part)];
+        const int kb0 = (int)((int64_t)p.k_blocks * part / p.split), kb1 = (int)((int64_t)p.k_blocks * (part + 1) / p.split);
+        const int a_mn = p.a_mn, b_mn = p.b_mn;
         const uint32_t idesc = operand_idesc<TYPE>(256, p.bn, a_mn, b_mn);
         const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;   // 16 k on
         const int buf = it & 1;
         if (!mbar_wait(smem_u32(&bars->acc_empty[buf]), ((it >> 1) & 1) ^ 1, abort_flag, 52)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + buf * 256;
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(smem_u32(&bars->full[s.slot]), s.phase, abort_flag, 53)) {
             go = false;
             break;
@@ -427,7 +434,7 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
           const uint32_t src = ring + s.slot * kStageBytes;
           const uint64_t ad = operand_desc(src, a_mn), bd = operand_desc(src + 16384, b_mn);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tc_mma_ss_pair(d, ad + k * a_step, bd + k * b_step, idesc, (kb | k) != 0);
+          for (int k = 0; k < 4; ++k) tc_mma_ss_pair(d, ad + k * a_step, bd + k * b_step, idesc, ((kb - kb0) | k) != 0);
           tc_commit_pair(smem_u32(&bars->empty[s.slot]));
           s.advance(kStages);
         }
@@ -441,8 +448,8 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
     const uint32_t staging = ring + kStages * kStageBytes + warp * kStagingBytes;
     int it = 0;
     for (int t = unit; t < work.n_tiles; t += n_units, ++it) {
-      int tm, tn;
-      const WideParams& p = work.p[place(t, tm, tn)];
+      int tm, tn, part;
+      const WideParams& p = work.p[place(t, tm, tn, part)];
       const int buf = it & 1;
       const int64_t row0 = (int64_t)tm * 256 + rank * 128 + quad * 32;
       const int rows = (int)min((int64_t)32, (int64_t)p.M - row0);
@@ -472,14 +479,15 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
         if (any) {
           RowPlace at{};
           at.cols = cols;
-          if (row_ok) at.out = p.out + row * p.ldo + col0;
+          if (row_ok && p.out) at.out = p.out + row * p.ldo + col0;
+          float* const sums = p.preact + (GATED ? 0 : part * p.plane);
           if (row_ok && p.preact && p.wide_p) {
-            at.preact = p.preact + row * p.ldp + col0;
+            at.preact = sums + row * p.ldp + col0;
             at.preact_up = at.preact + p.N;
           }
           if (p.preact && !p.wide_p) {
-            preact_anywhere(tz, width, staging, bias, has_bias, p.preact + row0 * p.ldp + col0, p.ldp, rows, cols, lane);
-            if (GATED) preact_anywhere(tu, width, staging, bias_u, has_bias, p.preact + row0 * p.ldp + p.N + col0, p.ldp, rows, cols, lane);
+            preact_anywhere(tz, width, staging, bias, has_bias, sums + row0 * p.ldp + col0, p.ldp, rows, cols, lane);
+            if (GATED) preact_anywhere(tu, width, staging, bias_u, has_bias, sums + row0 * p.ldp + p.N + col0, p.ldp, rows, cols, lane);
           }
           if (p.direct) {
             if constexpr (GATED) {
@@ -545,6 +553,8 @@ struct WidePlan {
   int bn[2];
   float us;
 };
+// Tiles of a product whose k is cut are as wide as it is, up to 256.
+int split_width(int N) { return N >= 256 ? 256 : std::max(64, (N + 31) / 32 * 32); }
 constexpr int kWidths = 7;                             // 256, 224, .. 64
 constexpr int width(int i) { return 256 - 32 * i; }
 struct WideCost {
@@ -553,11 +563,11 @@ struct WideCost {
 };
 WideCost cost_of(const DenseGemm& g, int pairs) {
   WideCost c;
-  const float blocks = (float)((g.K + 63) / 64);
+  const float blocks = (float)((g.K + 63) / 64) / (float)g.split;
   const int tiles_m = (int)(((int64_t)g.M + 255) / 256);
   for (int i = 0; i < kWidths; ++i) {
-    const int bn = width(i), tile_n = g.gated ? bn / 2 : bn;
-    const int64_t tiles = (int64_t)tiles_m * ((g.N + tile_n - 1) / tile_n);
+    const int bn = g.split > 1 ? split_width(g.N) : width(i), tile_n = g.gated ? bn / 2 : bn;
+    const int64_t tiles = (int64_t)tiles_m * ((g.N + tile_n - 1) / tile_n) * g.split;
     c.whole[i] = (int)std::min<int64_t>(tiles / pairs, 1 << 24);
     c.rest[i] = (int)(tiles % pairs);
     const float block_us = bn >= 128 ? 0.024f + 0.001f * (float)bn : 0.144f + 0.0001f * (float)bn;
@@ -584,7 +594,7 @@ WidePlan plan_wide(const DenseGemm* g, int count) {
       // of many waves, half of what idle pairs leave undone in the last comes back as clock and bandwidth for the others
       const float mean = ((float)q0 + (float)r0 / (float)pairs) * c0 + ((float)q1 + (float)r1 / (float)pairs) * c1;
       const float us = (width(i) >= 128 ? 2.4f + 0.0148f * (float)width(i) : 4.4f) + (full > 1.0f ? 0.5f * (most + mean) : most);
-      if (us < best.us) best = {{width(i), width(j)}, us};
+      if (us < best.us) best = {{g[0].split > 1 ? split_width(g[0].N) : width(i), count > 1 && g[1].split > 1 ? split_width(g[1].N) : width(j)}, us};
     }
   return best;
 }
@@ -601,25 +611,32 @@ void describe(const DenseGemm& g, int bn, WideParams& p, CUtensorMap& a, CUtenso
   p.tiles_m = (g.M + 255) / 256;
   p.tiles_n = (g.N + tile_n - 1) / tile_n;
   expects((int64_t)p.tiles_m * p.tiles_n < (1ll << 29), "dense product: more than 2^29 tiles");
-  p.n_tiles = p.tiles_m * p.tiles_n;
+  expects(g.split == 1 || (!GATED && !g.bias && !g.residual && !g.preact && g.act == kActNone && g.parts), "dense product: only plain products are cut along k");
+  p.split = g.split;
+  p.part_tiles = p.tiles_m * p.tiles_n;
+  p.n_tiles = p.part_tiles * p.split;
   p.k_blocks = (g.K + 63) / 64;
   p.act = g.act;
   p.kind = g.kind;
   p.bias = g.bias;
   p.residual = g.residual;
-  p.out = g.out;
-  p.preact = g.preact;
+  p.out = g.split > 1 ? nullptr : g.out;
+  p.preact = g.split > 1 ? g.parts : g.preact;
   p.ldr = g.ldr;
   p.ldo = g.ldo;
-  p.ldp = g.ldp;
+  p.ldp = g.split > 1 ? dense_part_pitch(g.N) : g.ldp;
+  p.plane = (int64_t)g.M * p.ldp;
   const auto on = [](const void* q, int64_t ld_bytes, int bytes) { return ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)ld_bytes) & (uintptr_t)(bytes - 1)) == 0; };
-  p.direct = on(g.out, g.ldo * 2, 16) && (g.residual == nullptr || on(g.residual, g.ldr * 2, 16));
-  p.wide_p = on(g.preact, g.ldp * 4, 32) && (!GATED || g.N % 8 == 0);
+  p.direct = (g.split > 1 || on(g.out, g.ldo * 2, 16)) && (g.residual == nullptr || on(g.residual, g.ldr * 2, 16));
+  p.wide_p = on(p.preact, p.ldp * 4, 32) && (!GATED || g.N % 8 == 0);
   const bool whole = (GATED ? p.bn / 4 : p.bn / 2) % 16 == 0;   // every warp's columns start on 32 bytes of a row that does
   p.wide_o = whole && on(g.out, g.ldo * 2, 32);
   a = operand_map(g.a, g.M, g.K, 128);
   b = operand_map(g.b, GATED ? 2 * (int64_t)g.N : g.N, g.K, p.bn / 2);
 }
+
+// What the parts of a cut sum cost more: a launch, and their way through the L2.
+float join_us(const DenseGemm& g) { return g.split > 1 ? 2.0f + 4e-7f * (float)dense_parts_bytes(g.M, g.N, g.split) : 0.0f; }
 
 template <int TYPE, bool GATED, int COUNT>
 void launch_wide(const DenseGemm* g, cudaStream_t stream) {
@@ -652,7 +669,7 @@ void launch_wide(const DenseGemm* g, cudaStream_t stream) {
 
 }  // namespace
 
-float dense_wide_us(const DenseGemm& g) { return plan_wide(&g, 1).us; }
+float dense_wide_us(const DenseGemm& g) { return plan_wide(&g, 1).us + join_us(g); }
 
 void launch_dense_wide(const DenseGemm& g, cudaStream_t stream) {
   if (g.type == kDenseBf16) {
@@ -662,13 +679,42 @@ void launch_dense_wide(const DenseGemm& g, cudaStream_t stream) {
     if (g.gated) launch_wide<kDenseFp16, true, 1>(&g, stream);
     else launch_wide<kDenseFp16, false, 1>(&g, stream);
   }
+  if (g.split > 1) launch_dense_join(g, stream);
 }
 
-// Two linear products that do not depend on each other, in one launch; the one with the longer tiles goes first.
+// As many parts as there are pairs for, of at least eight blocks of k each, where that saves a tile 32 blocks or more (9 us, of which
+// the join takes back 3 to 6).
+int dense_split(int M, int N, int K) {
+  constexpr int kPairs = 74;
+  const int bn = split_width(N), blocks = (K + 63) / 64;
+  const int64_t tiles = ((int64_t)M + 255) / 256 * (((int64_t)N + bn - 1) / bn);
+  if (tiles * 2 > kPairs) return 1;
+  const int split = std::min((int)(kPairs / tiles), blocks / 8);
+  return blocks - blocks / std::max(split, 1) >= 32 ? split : 1;
+}
+
+// Two linear products that do not depend on each other, in one launch; the one with the longer tiles goes first. Either is cut only
+// where the other does not fill the pairs as well (8192 tokens of 256 features, gated, 4096 wide: two products of 32 tiles take
+// 136 us as they are, 156 cut in halves).
 void launch_dense_wide_two(const DenseGemm& g, const DenseGemm& h, cudaStream_t stream) {
-  const DenseGemm two[2] = {g.K >= h.K ? g : h, g.K >= h.K ? h : g};
-  if (g.type == kDenseBf16) launch_wide<kDenseBf16, false, 2>(two, stream);
-  else launch_wide<kDenseFp16, false, 2>(two, stream);
+  DenseGemm best[2];
+  float best_us = 1e30f;
+  for (int cut = 3; cut >= 0; --cut) {
+    if (((cut & 1) && g.split == 1) || ((cut & 2) && h.split == 1)) continue;
+    DenseGemm two[2] = {g, h};
+    if (!(cut & 1)) two[0].split = 1;
+    if (!(cut & 2)) two[1].split = 1;
+    if (two[0].K / two[0].split < two[1].K / two[1].split) std::swap(two[0], two[1]);
+    const float us = g.split == 1 && h.split == 1 ? 0.0f : plan_wide(two, 2).us + join_us(two[0]) + join_us(two[1]);
+    if (us < best_us) {
+      best_us = us;
+      best[0] = two[0], best[1] = two[1];
+    }
+  }
+  if (g.type == kDenseBf16) launch_wide<kDenseBf16, false, 2>(best, stream);
+  else launch_wide<kDenseFp16, false, 2>(best, stream);
+  for (const DenseGemm& b : best)
+    if (b.split > 1) launch_dense_join(b, stream);
 }
 
 }  // namespace vkernels::kernels::cuda

@@ -237,6 +237,38 @@ __global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g
   }
 }
 
+// The result of a product whose k was cut: the parts' sums, in order, four columns a thread, eight parts on their way at a time. The
+// parts come out of the L2 as a rule (a cut product is a small one: at most 74 tiles of parts, 19 MB).
+template <int TYPE>
+__global__ void __launch_bounds__(256) dense_join_kernel(DenseGemm g, int64_t pitch) {
+  wait_for_earlier_kernels();
+  const int64_t plane = g.M * pitch;
+  const int across = (int)(pitch / 4);
+  const bool vec = ((reinterpret_cast<uintptr_t>(g.out) & 7u) | (g.ldo & 3)) == 0;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)g.M * across; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / across;
+    const int n = (int)(i - m * across) * 4, left = g.N - n;
+    if (left <= 0) continue;
+    const float* p = g.parts + m * pitch + n;
+    float z[4] = {};
+    for (int s = 0; s < g.split; s += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = s + j < g.split ? *reinterpret_cast<const float4*>(p + (s + j) * plane) : make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[0] += v[j].x, z[1] += v[j].y, z[2] += v[j].z, z[3] += v[j].w;
+    }
+    uint16_t* q = g.out + m * g.ldo + n;
+    if (vec && left >= 4) {
+      *reinterpret_cast<uint2*>(q) = make_uint2(dense_pack<TYPE>(z[0], z[1]), dense_pack<TYPE>(z[2], z[3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < left) q[j] = dense_from_f32<TYPE>(z[j]);
+    }
+  }
+}
+
 // Column sums of the chunks, in order; 16 loads at a time on their way.
 template <int TYPE>
 __global__ void __launch_bounds__(64) dense_sum_kernel(const float* __restrict__ partial, int chunks, int cols, uint16_t* __restrict__ db) {
@@ -330,6 +362,13 @@ void launch_dense_sum(DenseType type, const float* partial, int chunks, int cols
   const dim3 grid((cols + 63) / 64);
   if (type == kDenseBf16) launch_overlapped(dense_sum_kernel<kDenseBf16>, grid, 64, stream, partial, chunks, cols, db);
   else launch_overlapped(dense_sum_kernel<kDenseFp16>, grid, 64, stream, partial, chunks, cols, db);
+}
+
+void launch_dense_join(const DenseGemm& g, cudaStream_t stream) {
+  const int64_t pitch = dense_part_pitch(g.N), fours = (int64_t)g.M * (pitch / 4);
+  const dim3 grid((unsigned)std::min<int64_t>((fours + 255) / 256, 16 * 148));
+  if (g.type == kDenseBf16) launch_overlapped(dense_join_kernel<kDenseBf16>, grid, 256, stream, g, pitch);
+  else launch_overlapped(dense_join_kernel<kDenseFp16>, grid, 256, stream, g, pitch);
 }
 
 void launch_dense_copy_rows(const RowCopies& c, cudaStream_t stream) {
