@@ -39,7 +39,7 @@ struct WideParams {           // one product
   int bn;                     // rows of B a tile: a multiple of 32 from 64 to 256
   int stage_bytes;            // of one CTA: what the copies of a stage bring
   int tiles_m, tiles_n, n_tiles, k_blocks;
-  int split, part_tiles;      // parts of k, tiles of one part (the parts' tiles follow one another)
+  int part_tiles, part_blocks;   // of one part of k: its tiles (the parts' follow one another) and blocks
   int64_t plane;              // from one part's sums to the next's
   int act;
   GatedKind kind;
@@ -353,8 +353,11 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
     const int which = COUNT > 1 && t >= work.p[0].n_tiles;
     const WideParams& p = work.p[which];
     if (which) t -= work.p[0].n_tiles;
-    part = p.split > 1 ? t / p.part_tiles : 0;
-    t -= part * p.part_tiles;
+    part = 0;
+    if (!GATED && t >= p.part_tiles) {
+      part = t / p.part_tiles;
+      t -= part * p.part_tiles;
+    }
     const int per_group = kGroupM * p.tiles_n, first = t / per_group * kGroupM, in = t % per_group, high = min(kGroupM, p.tiles_m - first);
     tm = first + in % high;
     tn = in / high;
@@ -371,7 +374,7 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
         int tm, tn, part;
         const int which = place(t, tm, tn, part);
         const WideParams& p = work.p[which];
-        const int kb0 = (int)((int64_t)p.k_blocks * part / p.split), kb1 = (int)((int64_t)p.k_blocks * (part + 1) / p.split);
+        const int kb0 = part * p.part_blocks, kb1 = min(kb0 + p.part_blocks, p.k_blocks);
         const CUtensorMap *map_a = &work.a[which], *map_b = &work.b[which];
         // kept in registers: of two products, each look into the parameters would be an indexed load
         const int a_mn = p.a_mn, b_mn = p.b_mn, b_wide = p.bn > 128, pair_bytes = 2 * p.stage_bytes;
@@ -417,7 +420,7 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
       for (int t = unit; t < work.n_tiles && go; t += n_units, ++it) {
         int tm, tn, part;
         const WideParams& p = work.p[place(t, tm, tn, part)];
-        const int kb0 = (int)((int64_t)p.k_blocks * part / p.split), kb1 = (int)((int64_t)p.k_blocks * (part + 1) / p.split);
+        const int kb0 = part * p.part_blocks, kb1 = min(kb0 + p.part_blocks, p.k_blocks);
         const int a_mn = p.a_mn, b_mn = p.b_mn;
         const uint32_t idesc = operand_idesc<TYPE>(256, p.bn, a_mn, b_mn);
         const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;   // 16 k on
@@ -563,7 +566,7 @@ struct WideCost {
 };
 WideCost cost_of(const DenseGemm& g, int pairs) {
   WideCost c;
-  const float blocks = (float)((g.K + 63) / 64) / (float)g.split;
+  const float blocks = (float)(((g.K + 63) / 64 + g.split - 1) / g.split);
   const int tiles_m = (int)(((int64_t)g.M + 255) / 256);
   for (int i = 0; i < kWidths; ++i) {
     const int bn = g.split > 1 ? split_width(g.N) : width(i), tile_n = g.gated ? bn / 2 : bn;
@@ -612,10 +615,10 @@ void describe(const DenseGemm& g, int bn, WideParams& p, CUtensorMap& a, CUtenso
   p.tiles_n = (g.N + tile_n - 1) / tile_n;
   expects((int64_t)p.tiles_m * p.tiles_n < (1ll << 29), "dense product: more than 2^29 tiles");
   expects(g.split == 1 || (!GATED && !g.bias && !g.residual && !g.preact && g.act == kActNone && g.parts), "dense product: only plain products are cut along k");
-  p.split = g.split;
   p.part_tiles = p.tiles_m * p.tiles_n;
-  p.n_tiles = p.part_tiles * p.split;
+  p.n_tiles = p.part_tiles * g.split;
   p.k_blocks = (g.K + 63) / 64;
+  p.part_blocks = (p.k_blocks + g.split - 1) / g.split;
   p.act = g.act;
   p.kind = g.kind;
   p.bias = g.bias;
@@ -689,8 +692,8 @@ int dense_split(int M, int N, int K) {
   const int bn = split_width(N), blocks = (K + 63) / 64;
   const int64_t tiles = ((int64_t)M + 255) / 256 * (((int64_t)N + bn - 1) / bn);
   if (tiles * 2 > kPairs) return 1;
-  const int split = std::min((int)(kPairs / tiles), blocks / 8);
-  return blocks - blocks / std::max(split, 1) >= 32 ? split : 1;
+  const int most = std::max(std::min((int)(kPairs / tiles), blocks / 8), 1), each = (blocks + most - 1) / most;
+  return blocks - each >= 32 ? (blocks + each - 1) / each : 1;   // (no part is empty)
 }
 
 // Two linear products that do not depend on each other, in one launch; the one with the longer tiles goes first. Either is cut only
