@@ -53,9 +53,20 @@ def _call(name, index, *args):
         nr.check(rc, name)
 
 
-def _plain(t, shape, dtype, index):
-    """Whether a tensor is just what the kernels read: contiguous, of this shape and type, on this device and on 16 bytes."""
-    return t.shape == shape and t.dtype is dtype and t.get_device() == index and t.is_contiguous() and not t.data_ptr() & 15
+def _matrix(t, shape, dtype, index):
+    """The row pitch of a matrix that is just what the kernels read (this shape and type, this device, rows of neighbours), else 0."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index:
+        row, step = t.stride()
+        if step == 1:
+            if shape[0] == 1:
+                return shape[1] + 7 & -8
+            if row >= shape[1]:
+                return row
+    return 0
+
+
+def _vector(t, n, dtype, index):
+    return t.dtype is dtype and t.shape == (n,) and t.get_device() == index and t.is_contiguous()
 
 
 def _check(name, t, dtype, index):
@@ -187,15 +198,18 @@ def _result(out, out2, shape, x):
 def _new_preact(x, T, rows):
     """Room for fp32 pre-activations [T, rows], each row on 32 bytes."""
     if rows & 7:
-        return x.new_empty((T, (rows + 7) // 8 * 8), dtype=torch.float32)[:, :rows]
+        return x.new_empty_strided((T, rows), (rows + 7 & -8, 1), dtype=torch.float32)
     return x.new_empty((T, rows), dtype=torch.float32)
 
 
-def _forward_work(x, ldx, w, ldw, T, n_in, rows):
+_NO_ROOM = (None, None, 0)
+
+
+def _forward_work(x, xp, ldx, wp, ldw, T, n_in, rows):
     """(tensor to keep, pointer, bytes) of the room for copies of x and w, where their alignment calls for them."""
-    if not (x.data_ptr() & 15 or w.data_ptr() & 15 or ldx & 7 or ldw & 7):
-        return None, None, 0
-    nbytes = _entry("vk_cuda_dense_forward_workspace_bytes")(x.data_ptr(), ldx, w.data_ptr(), ldw, T, n_in, rows)
+    if not ((xp | wp) & 15 or (ldx | ldw) & 7):
+        return _NO_ROOM
+    nbytes = _entry("vk_cuda_dense_forward_workspace_bytes")(xp, ldx, wp, ldw, T, n_in, rows)
     work = x.new_empty((nbytes,), dtype=torch.uint8)
     return work, work.data_ptr(), nbytes
 
@@ -227,16 +241,18 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, b13: torch.Tensor | None = 
         # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
         shape, index, dtype, wshape = x.shape, x.get_device(), x.dtype, w13.shape
         if (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and _MOST >= wshape[1] == shape[1] > 0
-                and not shape[1] & 7 and 0 < wshape[0] <= _MOST and not wshape[0] & 1 and 0 < shape[0] <= _MOST
+                and 0 < wshape[0] <= _MOST and not wshape[0] & 1 and 0 < shape[0] <= _MOST
                 and (activation == SWIGLU or activation == SITU and beta > 0) and swiglu_limit >= 0
-                and _plain(x, shape, dtype, index) and _plain(w13, wshape, dtype, index)
-                and (b13 is None or _plain(b13, wshape[:1], dtype, index)) and not _wants_grad(x, w13, b13)):
+                and (ldx := _matrix(x, shape, dtype, index)) and (ldw := _matrix(w13, wshape, dtype, index))
+                and (b13 is None or _vector(b13, wshape[0], dtype, index)) and not _wants_grad(x, w13, b13)):
             T, rows = shape[0], wshape[0]
             h = x.new_empty((T, rows // 2))
             preact = _new_preact(x, T, rows) if return_preact else None
-            _call("vk_cuda_gated_linear", index, x.data_ptr(), shape[1], w13.data_ptr(), shape[1], None if b13 is None else b13.data_ptr(),
-                  h.data_ptr(), rows // 2, None if preact is None else preact.data_ptr(), (rows + 7) // 8 * 8, _DTYPE[dtype], T, shape[1], rows // 2,
-                  activation, swiglu_limit, beta, linear_beta, None, 0)
+            xp, wp = x.data_ptr(), w13.data_ptr()
+            work, room, nbytes = _forward_work(x, xp, ldx, wp, ldw, T, shape[1], rows) if (xp | wp) & 15 or (ldx | ldw) & 7 else _NO_ROOM
+            _call("vk_cuda_gated_linear", index, xp, ldx, wp, ldw, None if b13 is None else b13.data_ptr(),
+                  h.data_ptr(), rows // 2, None if preact is None else preact.data_ptr(), rows + 7 & -8, _DTYPE[dtype], T, shape[1], rows // 2,
+                  activation, swiglu_limit, beta, linear_beta, room, nbytes)
             return (h, preact) if return_preact else h
     x2 = _inputs(x, w13, True, "gated_linear")
     _gated_kind(activation, swiglu_limit, beta)
@@ -254,10 +270,10 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, b13: torch.Tensor | None = 
     h, h2 = _result(out, out2, shape, x)
     preact = _new_preact(x, T, rows) if return_preact else None
     if T > 0:
-        work, wp, nbytes = _forward_work(x2, ldx, w13, ldw, T, hidden, rows)
+        work, room, nbytes = _forward_work(x, x2.data_ptr(), ldx, w13.data_ptr(), ldw, T, hidden, rows)
         _call("vk_cuda_gated_linear", x.get_device(), x2.data_ptr(), ldx, w13.data_ptr(), ldw, b, h2.data_ptr(), _pitch("out", h2),
-              None if preact is None else preact.data_ptr(), (rows + 7) // 8 * 8, _DTYPE[x.dtype], T, hidden, ispp, activation, swiglu_limit, beta,
-              linear_beta, wp, nbytes)
+              None if preact is None else preact.data_ptr(), rows + 7 & -8, _DTYPE[x.dtype], T, hidden, ispp, activation, swiglu_limit, beta,
+              linear_beta, room, nbytes)
     return (h, preact) if return_preact else h
 
 
@@ -295,18 +311,21 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     if out is None and type(x) is torch.Tensor and isinstance(w, torch.Tensor):
         # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
         shape, index, dtype, wshape = x.shape, x.get_device(), x.dtype, w.shape
+        T, n_out, ldr = shape[0] if shape else 0, wshape[0] if wshape else 0, 0
         if (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and _MOST >= wshape[1] == shape[1] > 0
-                and not shape[1] & 7 and 0 < wshape[0] <= _MOST and 0 < shape[0] <= _MOST
-                and _plain(x, shape, dtype, index) and _plain(w, wshape, dtype, index)
-                and (bias is None or _plain(bias, wshape[:1], dtype, index))
-                and (residual is None or _plain(residual, (shape[0], wshape[0]), dtype, index))
+                and 0 < n_out <= _MOST and 0 < T <= _MOST
+                and (ldx := _matrix(x, shape, dtype, index)) and (ldw := _matrix(w, wshape, dtype, index))
+                and (bias is None or _vector(bias, n_out, dtype, index))
+                and (residual is None or (ldr := _matrix(residual, (T, n_out), dtype, index)))
                 and not _wants_grad(x, w, bias, residual)):
-            T, n_in, n_out = shape[0], shape[1], wshape[0]
+            n_in = shape[1]
             y = x.new_empty((T, n_out))
             preact = _new_preact(x, T, n_out) if return_preact and act else None
-            _call("vk_cuda_fused_linear", index, x.data_ptr(), n_in, w.data_ptr(), n_in, None if bias is None else bias.data_ptr(),
-                  None if residual is None else residual.data_ptr(), n_out, y.data_ptr(), n_out,
-                  None if preact is None else preact.data_ptr(), (n_out + 7) // 8 * 8, _DTYPE[dtype], T, n_in, n_out, act, None, 0)
+            xp, wp = x.data_ptr(), w.data_ptr()
+            work, room, nbytes = _forward_work(x, xp, ldx, wp, ldw, T, n_in, n_out) if (xp | wp) & 15 or (ldx | ldw) & 7 else _NO_ROOM
+            _call("vk_cuda_fused_linear", index, xp, ldx, wp, ldw, None if bias is None else bias.data_ptr(),
+                  None if residual is None else residual.data_ptr(), ldr, y.data_ptr(), n_out,
+                  None if preact is None else preact.data_ptr(), n_out + 7 & -8, _DTYPE[dtype], T, n_in, n_out, act, room, nbytes)
             return (y, preact) if return_preact else y
     x2 = _inputs(x, w, False, "fused_linear")
     n_out = w.shape[0]
@@ -333,10 +352,10 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     y, y2 = _result(out, out2, shape, x)
     preact = _new_preact(x, T, n_out) if return_preact and act else None
     if T > 0:
-        work, wp, nbytes = _forward_work(x2, ldx, w, ldw, T, n_in, n_out)
+        work, room, nbytes = _forward_work(x, x2.data_ptr(), ldx, w.data_ptr(), ldw, T, n_in, n_out)
         _call("vk_cuda_fused_linear", x.get_device(), x2.data_ptr(), ldx, w.data_ptr(), ldw, b, None if r2 is None else r2.data_ptr(), ldr,
-              y2.data_ptr(), _pitch("out", y2), None if preact is None else preact.data_ptr(), (n_out + 7) // 8 * 8, _DTYPE[x.dtype], T, n_in, n_out,
-              act, wp, nbytes)
+              y2.data_ptr(), _pitch("out", y2), None if preact is None else preact.data_ptr(), n_out + 7 & -8, _DTYPE[x.dtype], T, n_in, n_out,
+              act, room, nbytes)
     return (y, preact) if return_preact else y
 
 
@@ -351,20 +370,18 @@ def fused_linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pr
 
 
 def _backward(entry, dy, x, w, preact, gated, bias_grad, x_grad, w_grad, kind):
-    ordinary = False
+    ordinary, ldp = False, 0
     if type(x) is torch.Tensor and isinstance(w, torch.Tensor) and isinstance(dy, torch.Tensor):
         # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
         shape, index, dtype, wshape = x.shape, x.get_device(), x.dtype, w.shape
         ordinary = (len(shape) == 2 and index >= 0 and dtype in _DTYPE and len(wshape) == 2 and _MOST >= wshape[1] == shape[1] > 0
-                    and not shape[1] & 7 and 0 < wshape[0] <= _MOST and not (gated and wshape[0] & 1) and 0 < shape[0] <= _MOST
-                    and _plain(x, shape, dtype, index) and _plain(w, wshape, dtype, index)
-                    and _plain(dy, (shape[0], wshape[0] >> gated), dtype, index)
-                    and (preact is None or _plain(preact, (shape[0], wshape[0]), torch.float32, index)))
+                    and 0 < wshape[0] <= _MOST and not (gated and wshape[0] & 1) and 0 < shape[0] <= _MOST
+                    and (ldx := _matrix(x, shape, dtype, index)) and (ldw := _matrix(w, wshape, dtype, index))
+                    and (ld_dy := _matrix(dy, (shape[0], wshape[0] >> gated), dtype, index))
+                    and (preact is None or (ldp := _matrix(preact, (shape[0], wshape[0]), torch.float32, index))))
     if ordinary:
         (T, n_in), rows = shape, wshape[0]
-        n_out = ld_dy = rows >> gated
-        ldx = ldw = n_in
-        ldp = rows
+        n_out = rows >> gated
         dy2, x2 = dy, x
     else:
         x2 = _inputs(x, w, gated, entry[8:])
