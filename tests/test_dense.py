@@ -80,6 +80,9 @@ def test_out_must_not_overlap_the_inputs():
                           (wide[:3, 24:], wide[1:, :16], "CUDA"), (wide[:3, 24:], wide[1:, 20:36], "overlap x")):
         with pytest.raises(ops.OpNotEligible, match=match):
             ops.fused_linear(x, w, out=out)
+    one = t(1, 16).as_strided((1, 16), (0, 1))               # a single row, of any pitch
+    with pytest.raises(ops.OpNotEligible, match="overlap x"):
+        ops.fused_linear(one, w, out=one.as_strided((1, 16), (0, 1)))
     with pytest.raises(ops.OpNotEligible, match="CUDA"):     # the residual itself is a place for the result
         ops.fused_linear(t(2, 16), w, residual=a[:2], out=a[:2])
     with pytest.raises(ops.OpNotEligible, match="overlap w13"):
@@ -155,6 +158,16 @@ def test_workspace_sizes():
     assert fwd(P + 2, 64, P, 64, 4, 64, 64) == 4 * 64 * 2 and fwd(P, 64, P, 70, 4, 60, 3) == 512   # 3 rows of 64, in whole 256 bytes
     assert back(P, 64, P, 64, 100, 64, 13, 1) >= 100 * 32 * 2 + 26 * 4
     assert back(P + 2, 64, P, 64, 100, 64, 13, 1) >= back(P, 64, P, 64, 100, 64, 13, 1) + 100 * 64 * 2
+    # one of 74 tiles' worth of parts for each gradient with a long sum: 5000 tokens of 64 x 64, 9 parts of [64, 64] fp32
+    assert back(P, 64, P, 64, 5000, 64, 64, 0) >= back(P, 64, P, 64, 100, 64, 64, 0) + 9 * 64 * 64 * 4
+    for most in (2 ** 27 + 1, 2 ** 30, 2 ** 31 - 1):
+        for sizes in ((most, 64, 64), (100, most, 64), (100, 64, most)):
+            for gated in (0, 1):
+                lib.vk_set_last_error(0, b"")
+                assert back(P, 64, P, 64, *sizes, gated) == 0 and b"2^27" in lib.vk_last_error()
+            lib.vk_set_last_error(0, b"")
+            assert fwd(P, 64, P, 64, *sizes) == 0 and b"2^27" in lib.vk_last_error()
+    lib.vk_set_last_error(0, b"")
     assert fwd(P, 64, P, 64, -1, 64, 64) == 0 and lib.vk_last_error_code() == 1
     lib.vk_set_last_error(0, b"")
     assert back(P, 64, P, 64, -1, 64, 8, 0) == 0 and lib.vk_last_error_code() == 1

@@ -406,6 +406,16 @@ def test_recording_refuses_what_it_cannot_do():
         y.backward(torch.ones_like(y))
 
 
+def test_what_is_not_a_tensor_is_refused():
+    x, w13, b, more = tensors(8, 64, 32, "bf16")
+    dy = more(32)
+    for call in (lambda: ops.gated_linear(x, w13, [0.0] * 32), lambda: ops.fused_linear(x, w13, [0.0] * 32), lambda: ops.fused_linear(x, w13, residual=1.0),
+                 lambda: ops.fused_linear_backward(dy, x, w13, 1.0, activation="silu"), lambda: ops.fused_linear_backward(None, x, w13),
+                 lambda: ops.gated_linear_backward(dy[:, :16], x, w13, "none"), lambda: ops.fused_linear(x.cpu(), w13), lambda: ops.fused_linear(x, w13.cpu())):
+        with pytest.raises(ops.OpNotEligible):
+            call()
+
+
 def test_directional_differences():
     """The recorded gradients against differences of the forward operator itself, along the gradient: fp16 results are good to
     2^-11 of themselves each, the step moves the loss by a tenth."""

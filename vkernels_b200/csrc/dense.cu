@@ -13,12 +13,15 @@ bool tma_ready(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(
 bool even(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
-void check_common(DenseType type, int T, int n_in, int n_out, bool gated, int act, float limit, float beta) {
-  expects(type == kDenseBf16 || type == kDenseFp16, "dense: dtype must be 0 (bf16) or 1 (fp16)");
+void check_sizes(int T, int n_in, int n_out, bool gated) {
   expects(T >= 0 && n_in > 0 && n_out > 0, "dense: T must not be negative, feature counts must be positive");
   // (a wait inside the kernels gives up after two seconds; one tile over 2^27 values takes 0.6)
   constexpr int kMost = 1 << 27;
   expects(n_in <= kMost && n_out <= (gated ? kMost / 2 : kMost) && T <= kMost, "dense: sizes beyond 2^27 tokens, inputs or weight rows");
+}
+void check_common(DenseType type, int T, int n_in, int n_out, bool gated, int act, float limit, float beta) {
+  expects(type == kDenseBf16 || type == kDenseFp16, "dense: dtype must be 0 (bf16) or 1 (fp16)");
+  check_sizes(T, n_in, n_out, gated);
   if (gated) {
     expects(act == 0 || act == 1, "gated_linear: activation must be 0 (SwiGLU) or 1 (SiTU)");
     expects(limit >= 0.0f, "gated_linear: swiglu_limit must not be negative (0 for none)");
@@ -71,7 +74,7 @@ void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream) {
 }
 
 size_t dense_forward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int w_rows) {
-  expects(T >= 0 && n_in > 0 && w_rows > 0, "dense: T must not be negative, feature counts must be positive");
+  check_sizes(T, n_in, w_rows, false);
   return T == 0 ? 0 : copy_bytes(x, ldx, T, n_in) + copy_bytes(w, ldw, w_rows, n_in);
 }
 
@@ -112,7 +115,7 @@ void dense_forward(const DenseForward& f, cudaStream_t stream) {
 }
 
 size_t dense_backward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int n_out, bool gated) {
-  expects(T >= 0 && n_in > 0 && n_out > 0, "dense: T must not be negative, feature counts must be positive");
+  check_sizes(T, n_in, n_out, gated);
   const size_t rows = (gated ? 2 : 1) * (size_t)n_out;
   if (T == 0) return 0;
   return copy_bytes(x, ldx, T, n_in) + copy_bytes(w, ldw, (int)rows, n_in) + round_up((size_t)T * round_up(rows, 8) * 2, 256) +

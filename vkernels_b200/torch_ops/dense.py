@@ -66,7 +66,7 @@ def _matrix(t, shape, dtype, index):
 
 
 def _vector(t, n, dtype, index):
-    return t.dtype is dtype and t.shape == (n,) and t.get_device() == index and t.is_contiguous()
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (n,) and t.get_device() == index and t.is_contiguous()
 
 
 def _check(name, t, dtype, index):
@@ -113,7 +113,7 @@ def _side_by_side(t, a, u, c):
     if t.dim() != 2 or u.dim() != 2 or t.stride() != u.stride() or t.stride(1) != 1:
         return False
     pitch, gap = t.stride(0), (c - a) // t.element_size()
-    return t.shape[1] <= gap % pitch and gap % pitch + u.shape[1] <= pitch
+    return pitch > 0 and t.shape[1] <= gap % pitch and gap % pitch + u.shape[1] <= pitch
 
 
 def _rows2d(name, t, cols):
@@ -316,7 +316,7 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
                 and 0 < n_out <= _MOST and 0 < T <= _MOST
                 and (ldx := _matrix(x, shape, dtype, index)) and (ldw := _matrix(w, wshape, dtype, index))
                 and (bias is None or _vector(bias, n_out, dtype, index))
-                and (residual is None or (ldr := _matrix(residual, (T, n_out), dtype, index)))
+                and (residual is None or isinstance(residual, torch.Tensor) and (ldr := _matrix(residual, (T, n_out), dtype, index)))
                 and not _wants_grad(x, w, bias, residual)):
             n_in = shape[1]
             y = x.new_empty((T, n_out))
@@ -378,7 +378,7 @@ def _backward(entry, dy, x, w, preact, gated, bias_grad, x_grad, w_grad, kind):
                     and 0 < wshape[0] <= _MOST and not (gated and wshape[0] & 1) and 0 < shape[0] <= _MOST
                     and (ldx := _matrix(x, shape, dtype, index)) and (ldw := _matrix(w, wshape, dtype, index))
                     and (ld_dy := _matrix(dy, (shape[0], wshape[0] >> gated), dtype, index))
-                    and (preact is None or (ldp := _matrix(preact, (shape[0], wshape[0]), torch.float32, index))))
+                    and (preact is None or isinstance(preact, torch.Tensor) and (ldp := _matrix(preact, (shape[0], wshape[0]), torch.float32, index))))
     if ordinary:
         (T, n_in), rows = shape, wshape[0]
         n_out = rows >> gated
