@@ -292,7 +292,7 @@ def test_same_bits_every_time_and_on_every_stream():
         assert all(torch.equal(a, b) for a, b in zip(g, first))
 
 
-@pytest.mark.parametrize("T", [1, 48, 300])
+@pytest.mark.parametrize("T", [1, 48, 300, 4100])
 def test_captured_graphs_share_nothing(T):
     """Two graphs of forward and backward, captured on one stream and replayed on two at once, on new inputs."""
     cases = []
