@@ -56,7 +56,7 @@ struct DenseGemm {
   float* parts;
 };
 
-// dst[i][r, c] = src[i][r, c] for up to two matrices (dst[i] not null), rows of dst one after the other, each on 16 bytes.
+// dst[i][r, c] = src[i][r, c] for up to two matrices (dst[i] not null), rows of dst one after the other, each on 32 bytes.
 struct RowCopies {
   const uint16_t* src[2];
   uint16_t* dst[2];

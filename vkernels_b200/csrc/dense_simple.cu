@@ -111,10 +111,11 @@ __device__ __forceinline__ Eight load_eight_words(const uint16_t* p, int n) {
   for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(e.v)[j] = odd ? __funnelshift_r(v[j], v[j + 1], 16) : v[j];
   return e;
 }
-// Copies of rows, as the `part`-th of `parts` CTAs of 256 threads: dst[r, c] = src[r, c], rows of dst on 16 bytes, filled up to whole
-// units of 8.
+constexpr int copy_units(int cols) { return (cols + 15) / 16 * 2; }
+// Copies of rows, as the `part`-th of `parts` CTAs of 256 threads: dst[r, c] = src[r, c], rows of dst on 32 bytes, filled up to whole
+// pairs of units of 8.
 __device__ __forceinline__ void copy_rows(const RowCopies& c, int part, int parts) {
-  const int units = (c.cols + 7) / 8;
+  const int units = copy_units(c.cols);
   const int64_t first = c.dst[0] != nullptr ? (int64_t)c.rows[0] * units : 0;
   const int64_t all = first + (c.dst[1] != nullptr ? (int64_t)c.rows[1] * units : 0), step = (int64_t)parts * 256;
 #pragma unroll 2
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) dense_grad_kernel(DenseGrad g
   constexpr bool GATED = FORM >= kGradSwiGlu, BENT = FORM != kActNone;
   __shared__ float sums[GATED ? 2 : 1][4][kGradCols];
   wait_for_earlier_kernels();
-  if ((int)blockIdx.y >= chunks) {   // operands of the products to rows on 16 bytes, on the way
+  if ((int)blockIdx.y >= chunks) {   // operands of the products to rows on 32 bytes, on the way
     copy_rows(g.copies, (blockIdx.y - chunks) * gridDim.x + blockIdx.x, (gridDim.y - chunks) * gridDim.x);
     return;
   }
@@ -303,7 +304,7 @@ void launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, cudaStream_
 int copy_ctas(const RowCopies& c) {
   int64_t units = 0;
   for (int i = 0; i < 2; ++i)
-    if (c.dst[i] != nullptr) units += (int64_t)c.rows[i] * ((c.cols + 7) / 8);
+    if (c.dst[i] != nullptr) units += (int64_t)c.rows[i] * copy_units(c.cols);
   return (int)std::min<int64_t>((units + 511) / 512, 8 * 148);
 }
 
