@@ -406,7 +406,8 @@ int vk_cuda_fused_moe_mxfp4_rows(const uint64_t* a_rows, const uint8_t* w13, con
  * *_backward: gradients for the gradient of the result (dh / dy); each of dx, dw (dw13), db (db13) may be NULL. The activation
  *   arguments and preact are those of the forward call (preact unused for activation 0 of the linear form); the residual's
  *   gradient is dy. The gradient of z is rounded to the type once, as the products' operand, in the workspace
- *   (vk_cuda_dense_backward_workspace_bytes bytes); db sums it unrounded. */
+ *   (vk_cuda_dense_backward_workspace_bytes bytes, which also hold fp32 parts of gradients that are long sums of few values); db sums
+ *   it unrounded. */
 int vk_cuda_gated_linear(const void* x, int64_t ldx, const void* w13, int64_t ldw, const void* b13, void* h, int64_t ldh,
                          float* preact, int64_t ldp, int dtype, int T, int hidden, int ispp, int activation, float swiglu_limit,
                          float beta, float linear_beta, void* workspace, size_t workspace_bytes, void* stream);

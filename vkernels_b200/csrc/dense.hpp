@@ -85,11 +85,11 @@ struct DenseGrad {
 };
 
 int dense_sum_chunks(int T, int n_out);
-// Parts that k is cut into where a plain product has fewer tiles than a third of the CTA pairs and k is long.
+// Parts that k is cut into at most: more than one where a plain product has few tiles and k is long.
 int dense_split(int M, int N, int K);
 inline int64_t dense_part_pitch(int N) { return ((int64_t)N + 7) / 8 * 8; }
 inline size_t dense_parts_bytes(int M, int N, int split) { return split > 1 ? (size_t)split * (size_t)M * (size_t)dense_part_pitch(N) * 4 : 0; }
-// out = the parts' sum, in order, of up to two products (split > 1).
+// out = the parts' sums, added in order (split > 1).
 void launch_dense_join(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_wide(const DenseGemm& g, cudaStream_t stream);   // dense_gemm.cu
@@ -135,7 +135,7 @@ struct DenseBackward {
 void dense_forward(const DenseForward& f, cudaStream_t stream);
 void dense_backward(const DenseBackward& f, cudaStream_t stream);
 // Workspace: copies of x and w where a tensor map does not take them as they are; of the backward pass also the gradient of the
-// pre-activations and the chunks' column sums.
+// pre-activations, the chunks' column sums and the parts of gradients that are cut along k.
 size_t dense_forward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int w_rows);
 size_t dense_backward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int n_in, int n_out, bool gated);
 
