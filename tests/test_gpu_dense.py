@@ -143,6 +143,7 @@ def test_gradients_of_long_sums(T, K, N, dtype):
         ref.assert_within(call(w_grad=False)[0], *wanted[0], "dx alone")
         ref.assert_within(call(x_grad=False)[1], *wanted[1], "dw alone")
         assert all(torch.equal(p, q) for p, q in zip(call(bias_grad=True), both))
+        assert torch.equal(call(x_grad=False, w_grad=False, bias_grad=True)[2], both[2])
     torch.cuda.synchronize()
     ops.kernel_status()
 

@@ -169,6 +169,7 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
   RowCopies made{};
   bring_operands(x, ldx, f.T, w, ldw, rows, f.n_in, f.workspace, f.workspace_bytes, made);
   uint16_t* dz = need_dz ? reinterpret_cast<uint16_t*>(static_cast<char*>(f.workspace) + copies) : nullptr;
+  DenseSums sums{};
   if (need_dz || f.db) {
     float* partial = f.db ? reinterpret_cast<float*>(static_cast<char*>(f.workspace) + copies + dz_bytes) : nullptr;
     DenseGrad g{};
@@ -189,7 +190,7 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
     if (f.gated) g.kind = gated_kind(f.act, effective_limit(f.act, f.limit), f.beta, f.linear_beta);
     g.copies = made;
     launch_dense_grad(g, stream);
-    if (f.db && chunks > 1) launch_dense_sum(f.type, partial, chunks, rows, f.db, stream);
+    if (f.db && chunks > 1) sums = {partial, chunks, rows, f.db};
   } else {
     launch_dense_copy_rows(made, stream);
   }
@@ -221,9 +222,10 @@ void dense_backward(const DenseBackward& f, cudaStream_t stream) {
   }
   // both in one launch: the tiles of one fill what the other leaves idle (1001 tokens, 1504 -> 2 x 1024: 21.3 us as two)
   if (f.dx && f.dw && get_moe_impl() != MoeImpl::kSimt) {
-    launch_dense_wide_two(gx, gw, stream);
+    launch_dense_wide_two(gx, gw, sums, stream);
     return;
   }
+  launch_dense_sum(f.type, sums, stream);
   if (f.dx) launch_dense_gemm(gx, stream);
   if (f.dw) launch_dense_gemm(gw, stream);
 }

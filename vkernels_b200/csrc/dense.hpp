@@ -84,6 +84,13 @@ struct DenseGrad {
   RowCopies copies;           // made by the same launch
 };
 
+// db[n] = sum over the chunks of partial[chunk, n] (db null: nothing to do).
+struct DenseSums {
+  const float* partial;
+  int chunks, cols;
+  uint16_t* db;
+};
+
 int dense_sum_chunks(int T, int n_out);
 // Parts that k is cut into at most: more than one where a plain product has few tiles and k is long.
 int dense_split(int M, int N, int K);
@@ -93,14 +100,13 @@ inline size_t dense_parts_bytes(int M, int N, int split) { return split > 1 ? (s
 void launch_dense_join(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_gemm(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_wide(const DenseGemm& g, cudaStream_t stream);   // dense_gemm.cu
-void launch_dense_wide_two(const DenseGemm& g, const DenseGemm& h, cudaStream_t stream);
+void launch_dense_wide_two(const DenseGemm& g, const DenseGemm& h, const DenseSums& sums, cudaStream_t stream);
 void launch_dense_narrow(const DenseGemm& g, cudaStream_t stream);  // dense_narrow.cu
 float dense_wide_us(const DenseGemm& g);      // the time that either is expected to take
 float dense_narrow_us(const DenseGemm& g);
 void launch_dense_simt(const DenseGemm& g, cudaStream_t stream);
 void launch_dense_grad(const DenseGrad& g, cudaStream_t stream);
-// db[n] = sum over the chunks of partial[chunk, n], in order.
-void launch_dense_sum(DenseType type, const float* partial, int chunks, int cols, uint16_t* db, cudaStream_t stream);
+void launch_dense_sum(DenseType type, const DenseSums& sums, cudaStream_t stream);
 void launch_dense_copy_rows(const RowCopies& c, cudaStream_t stream);
 
 // ---- the operators ----

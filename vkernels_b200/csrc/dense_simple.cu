@@ -136,7 +136,7 @@ constexpr int kGradCols = 256, kGradThreads = 256;   // 64 threads across the co
 constexpr int kGradRows = 4, kGradStep = 4 * kGradRows;   // rows a thread has on their way, rows a CTA takes at once
 
 // dz = dy * act'(z) and the column sums of a chunk of rows, in one pass: one CTA per 256 columns of dy and chunk. A column's
-// sum is added by one thread per fourth row in fp32, the fourths in order, the chunks by dense_sum_kernel: no atomics, the same
+// sum is added by one thread per fourth row in fp32, the fourths in order, the chunks by sum_chunks: no atomics, the same
 // result every time. The sums are of the unrounded gradients. Bound by memory (dy and z in, dz out), as long as enough of it is
 // on its way: four rows a thread before the first is worked on, the whole launch resident at once (4096 x 2880 gated: eight
 // columns a thread, one row at a time and three times as many CTAs took 41 us). VEC: a thread's four columns are neighbours, in
@@ -270,21 +270,12 @@ __global__ void __launch_bounds__(256) dense_join_kernel(DenseGemm g, int64_t pi
   }
 }
 
-// Column sums of the chunks, in order; 16 loads at a time on their way.
+// Column sums of the chunks where no launch of products follows that takes them along.
 template <int TYPE>
-__global__ void __launch_bounds__(64) dense_sum_kernel(const float* __restrict__ partial, int chunks, int cols, uint16_t* __restrict__ db) {
+__global__ void __launch_bounds__(256) dense_sum_kernel(DenseSums q) {
+  __shared__ float room[8][32];
   wait_for_earlier_kernels();
-  const int c = blockIdx.x * 64 + threadIdx.x;
-  if (c >= cols) return;
-  float s = 0.0f;
-  for (int i = 0; i < chunks; i += 16) {
-    float v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = i + j < chunks ? partial[(int64_t)(i + j) * cols + c] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) s += v[j];
-  }
-  db[c] = dense_from_f32<TYPE>(s);
+  sum_chunks<TYPE>(q, blockIdx.x, gridDim.x, threadIdx.x >> 5, threadIdx.x & 31, room);
 }
 
 template <class... P, class... A>
@@ -359,10 +350,11 @@ void launch_dense_grad(const DenseGrad& g, cudaStream_t stream) {
   else grad_of_type<kDenseFp16>(g, chunks, stream);
 }
 
-void launch_dense_sum(DenseType type, const float* partial, int chunks, int cols, uint16_t* db, cudaStream_t stream) {
-  const dim3 grid((cols + 63) / 64);
-  if (type == kDenseBf16) launch_overlapped(dense_sum_kernel<kDenseBf16>, grid, 64, stream, partial, chunks, cols, db);
-  else launch_overlapped(dense_sum_kernel<kDenseFp16>, grid, 64, stream, partial, chunks, cols, db);
+void launch_dense_sum(DenseType type, const DenseSums& sums, cudaStream_t stream) {
+  if (sums.db == nullptr) return;
+  const dim3 grid(std::min((sums.cols + 31) / 32, 8 * 148));
+  if (type == kDenseBf16) launch_overlapped(dense_sum_kernel<kDenseBf16>, grid, 256, stream, sums);
+  else launch_overlapped(dense_sum_kernel<kDenseFp16>, grid, 256, stream, sums);
 }
 
 void launch_dense_join(const DenseGemm& g, cudaStream_t stream) {
