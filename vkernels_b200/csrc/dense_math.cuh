@@ -162,6 +162,7 @@ __device__ __forceinline__ void sum_chunks(const DenseSums& q, int cta, int ctas
       for (int j = 0; j < 16; ++j) s += v[j];
     }
     room[warp][lane] = s;
+    __syncwarp();   // bar.sync takes a warp's lanes as one; those behind the last column have not loaded
     asm volatile("bar.sync 1, 256;" ::: "memory");
     if (warp == 0 && c < q.cols) {
       s = room[0][lane];
@@ -169,6 +170,7 @@ __device__ __forceinline__ void sum_chunks(const DenseSums& q, int cta, int ctas
       for (int i = 1; i < 8; ++i) s += room[i][lane];
       q.db[c] = dense_from_f32<TYPE>(s);
     }
+    __syncwarp();
     asm volatile("bar.sync 1, 256;" ::: "memory");
   }
 }

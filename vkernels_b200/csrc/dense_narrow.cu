@@ -220,6 +220,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
   }
   tc_fence_before();
+  __syncwarp();   // the cluster barrier is .aligned: a warp's lanes arrive as one
   if (split > 1) cluster_sync_all();
   else __syncthreads();
 
@@ -290,6 +291,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   }
 
   // ------------------------------ teardown ---------------------------------
+  __syncwarp();   // lanes leave the join one by one
   if (split > 1) cluster_sync_all();   // nobody reads this CTA's partial sums any more
   else __syncthreads();
   if (warp == kEpiWarps + 1)

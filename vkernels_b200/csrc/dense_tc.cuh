@@ -15,7 +15,10 @@ int* sm100_status_address();
 
 namespace {
 
+// .aligned: the whole warp executes it as one. Its lanes part before it wherever rows behind the last are not stored, and nothing but
+// the barrier brings them together for certain.
 __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* v) {
+  __syncwarp();
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
