@@ -1,0 +1,53 @@
+"""-m gpu: the dense feed-forward where its tensors lie in one another's memory, and calls that must not go through."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from vkernels_b200 import torch_ops as ops  # noqa: E402
+
+DEV = "cuda:0"
+
+
+def layers(T, grad=False):
+    """A small routed layer with and one without a bf16 always-on expert, that expert, and activations for them."""
+    from gpu_common import make_case
+    from vkernels_b200 import synthetic as syn
+    from vkernels_b200.experts import layer_from_config
+    from vkernels_b200.feedforward import DenseFeedForward
+
+    cfg = syn.scaled(syn.CONFIGS["c0"], H=512, I=256, E=8, top_k=2)
+    w, A, r = make_case(cfg, T, backend="torch")
+    g = torch.Generator(device=DEV)
+    g.manual_seed(3)
+    ispp = 192
+    w13 = (torch.randn(2 * ispp, cfg.H, generator=g, device=DEV) / cfg.H ** 0.5).to(torch.bfloat16).requires_grad_(grad)
+    w2 = (torch.randn(cfg.H, ispp, generator=g, device=DEV) / ispp ** 0.5).to(torch.bfloat16).requires_grad_(grad)
+    ffn = DenseFeedForward(w13, w2)
+    return layer_from_config(cfg, w, r, max_tokens=T), layer_from_config(cfg, w, r, max_tokens=T, shared_ffn=ffn), ffn, A
+
+
+def same(got, want, T):
+    """Bit by bit, but for batches whose routed part adds with atomics."""
+    return torch.equal(got, want) or T > 256 and torch.allclose(got.float(), want.float(), atol=2e-2, rtol=2.0 ** -7)
+
+
+@pytest.mark.parametrize("T", [1, 40, 600])
+def test_layer_result_where_its_activations_lie(T):
+    """The always-on expert sees the activations although the result takes their place: given as out_bf16, overlapping by a row
+    less, and in the layer's own result buffer, when one call's result is the next one's input."""
+    routed, layer, ffn, A = layers(T)
+    want = ffn(A, routed(A))
+    assert not same(ffn(routed(A).clone(), routed(A)), want, T)      # what the expert would add for the routed result
+    x = A.clone()
+    got = layer(x, out_bf16=x)
+    assert got is x and same(x, want, T)
+    room = torch.empty(T + 1, A.shape[1], dtype=A.dtype, device=DEV)
+    room[1:] = A
+    assert same(layer(room[1:], out_bf16=room[:T]), want, T)
+    first = layer(A)
+    keep = first.clone()
+    want = ffn(keep, routed(keep))
+    assert same(layer(first), want, T)
+    torch.cuda.synchronize()
+    ops.kernel_status()

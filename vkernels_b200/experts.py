@@ -256,10 +256,12 @@ class FusedMoEMxfp4:
                                       store_slots=store_slots)
 
     def forward(self, x: torch.Tensor, *, logits: torch.Tensor | None = None, out_bf16=None):
-        """route -> align -> gate/up -> down+combine (+ shared_ffn), all on the current stream."""
+        """route -> align -> gate/up -> down+combine (+ shared_ffn), all on the current stream. The result may take x's place:
+        ``out_bf16`` may be x or overlap it, and x may be the result of the call before."""
         ops.require(x.dim() == 2 and x.shape[1] == self.hidden, "x must be [T, hidden]")
         bufs = self._buffers(x.shape[0])
         T = x.shape[0]
+        product = self._shared_product(x)
         if T * self.slots <= 1024 and (logits is not None or self.router_weight is not None):
             # decode-size batch: router top-k and alignment in one kernel
             with _region("moe:apply.route"):
@@ -271,18 +273,25 @@ class FusedMoEMxfp4:
                     renorm=self.renorm, scaling=self.scaling, n_shared=self.n_shared, max_EM=self._em_bound(T),
                     out=(bufs["ids"].view(T, self.slots), bufs["w"].view(T, self.slots), bufs["sids"], bufs["eids"],
                          bufs["out_em"]))
-            return self._add_shared(x, self.experts(x, ids, w, bufs, out_bf16=out_bf16, aligned=(sids, eids)))
+            return self._add_shared(product, self.experts(x, ids, w, bufs, out_bf16=out_bf16, aligned=(sids, eids)))
         with _region("moe:apply.route"):
             ids, w = self.route(x, bufs, logits=logits)
-        return self._add_shared(x, self.experts(x, ids, w, bufs, out_bf16=out_bf16))
+        return self._add_shared(product, self.experts(x, ids, w, bufs, out_bf16=out_bf16))
 
-    def _add_shared(self, x, y):
-        """y, with the always-on expert's result added in place (the routed result is its residual)."""
+    def _shared_product(self, x):
+        """The always-on expert's gated projection, made before the routed experts write their result: that may lie where x does."""
         if self.shared_ffn is None:
-            return y
+            return None
         T = x.shape[0]
         with _region("moe:apply.shared"):
-            return self.shared_ffn(x, y, out=y, product=self.arena.take("shared", T * self.shared_ffn.ispp).view(T, -1))
+            return self.shared_ffn.product(x, out=self.arena.take("shared", T * self.shared_ffn.ispp).view(T, self.shared_ffn.ispp))
+
+    def _add_shared(self, product, y):
+        """y, with the always-on expert's result added in place (the routed result is its residual)."""
+        if product is None:
+            return y
+        with _region("moe:apply.shared"):
+            return self.shared_ffn.project(product, y, out=y)
 
     __call__ = forward
 

@@ -32,11 +32,18 @@ class DenseFeedForward:
         self.hidden, self.ispp = w2.shape
         self.kind = dict(activation=activation, swiglu_limit=swiglu_limit, beta=beta, linear_beta=linear_beta)
 
+    def product(self, x: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The gated projection alone: ``[..., ispp]`` for x ``[..., hidden]``."""
+        return ops.gated_linear(x, self.w13, self.b13, out=out, **self.kind)
+
+    def project(self, h: torch.Tensor, residual: torch.Tensor | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The second projection alone: ``[..., hidden]`` for a product h ``[..., ispp]``."""
+        return ops.fused_linear(h, self.w2, self.b2, residual=residual, out=out)
+
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, *, out: torch.Tensor | None = None,
                 product: torch.Tensor | None = None) -> torch.Tensor:
         """y ``[..., hidden]`` for x ``[..., hidden]``. ``out`` (it may be the residual) and ``product`` (``[..., ispp]``, the gated
         projection's result) are places for the results that the caller keeps."""
-        h = ops.gated_linear(x, self.w13, self.b13, out=product, **self.kind)
-        return ops.fused_linear(h, self.w2, self.b2, residual=residual, out=out)
+        return self.project(self.product(x, out=product), residual, out=out)
 
     __call__ = forward
