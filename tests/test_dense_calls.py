@@ -1,0 +1,36 @@
+"""Dense feed-forward, calls that are refused before anything reaches the GPU: places for results that lie in what is still read,
+arguments that are no tensors, forward-mode differentiation."""
+import pytest
+import torch
+
+from vkernels_b200 import torch_ops as ops
+
+BF = torch.bfloat16
+
+
+def t(*shape, dtype=BF):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def test_feed_forward_places_must_not_overlap_what_is_read_later():
+    """The product is written before the residual and the second projection are read; the result after the first one's weights, which
+    the next call needs."""
+    from vkernels_b200.feedforward import DenseFeedForward
+
+    H, ispp = 16, 8
+    w13, w2, room, x, res = t(2 * ispp, H), t(H, ispp), t(256), t(4, H), t(4, H)
+    b13, b2 = room[64:64 + 2 * ispp], room[192:192 + H]
+    ffn = DenseFeedForward(w13, w2, b13=b13, b2=b2)
+    for kw, match in ((dict(product=res[:2].view(4, ispp)), "product must not overlap the residual"),
+                      (dict(product=res[:, 4:12]), "product must not overlap the residual"),
+                      (dict(product=w2[4:8]), "product must not overlap w2"),
+                      (dict(product=room[200:200 + 4 * ispp].view(4, ispp)), "product must not overlap b2"),
+                      (dict(out=w13[:4]), "out must not overlap w13"),
+                      (dict(out=room[72:72 + 4 * H].view(4, H)), "out must not overlap b13"),
+                      (dict(product=[0.0]), "tensor"), (dict(out=[0.0]), "tensor")):
+        with pytest.raises(ops.OpNotEligible, match=match):
+            ffn(x, res, **kw)
+    wide = t(4, H + ispp)
+    for r, kw in ((res, dict(product=t(4, ispp))), (wide[:, :H], dict(product=wide[:, H:])), (res, dict(out=res)), (res, dict(out=x)), (None, dict(out=x))):
+        with pytest.raises(ops.OpNotEligible, match="CUDA"):      # not in the way of one another: on to the operators
+            ffn(x, r, **kw)

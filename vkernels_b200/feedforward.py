@@ -42,8 +42,13 @@ class DenseFeedForward:
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, *, out: torch.Tensor | None = None,
                 product: torch.Tensor | None = None) -> torch.Tensor:
-        """y ``[..., hidden]`` for x ``[..., hidden]``. ``out`` (it may be the residual) and ``product`` (``[..., ispp]``, the gated
-        projection's result) are places for the results that the caller keeps."""
+        """y ``[..., hidden]`` for x ``[..., hidden]``. ``out`` (it may be the residual, or x) and ``product`` (``[..., ispp]``, the
+        gated projection's result) are places for the results that the caller keeps; ``product`` is written before the residual and
+        the second projection's weights are read, and must not overlap them."""
+        if product is not None:
+            ops.require_apart("product", product, ("the residual", residual), ("w2", self.w2), ("b2", self.b2))
+        if out is not None:
+            ops.require_apart("out", out, ("w13", self.w13), ("b13", self.b13))
         return self.project(self.product(x, out=product), residual, out=out)
 
     __call__ = forward

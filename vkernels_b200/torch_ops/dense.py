@@ -69,9 +69,13 @@ def _vector(t, n, dtype, index):
     return isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (n,) and t.get_device() == index and t.is_contiguous()
 
 
-def _check(name, t, dtype, index):
+def _check_tensor(name, t):
     if not isinstance(t, torch.Tensor):
         raise OpNotEligible(f"{name} must be a tensor")
+
+
+def _check(name, t, dtype, index):
+    _check_tensor(name, t)
     if t.dtype is not dtype:
         raise OpNotEligible(f"{name} must be {dtype}, like the other tensors of the call, got {t.dtype}")
     if t.get_device() != index:
@@ -106,6 +110,15 @@ def _apart(name, out, others):
             c, d = _span(t)
             if a < d and c < b and not _side_by_side(out, a, t, c):
                 raise OpNotEligible(f"{name} must not overlap {other_name}")
+
+
+def require_apart(name, out, *others):
+    """Refuses a tensor `out`, called `name`, that shares memory with any of the others: pairs of a name and a tensor or None."""
+    _check_tensor(name, out)
+    for other_name, t in others:
+        if t is not None:
+            _check_tensor(other_name, t)
+    _apart(name, out, others)
 
 
 def _side_by_side(t, a, u, c):
