@@ -17,13 +17,17 @@ enum DenseAct { kActNone = 0, kActSilu = 1, kActGelu = 2, kActGeluTanh = 3 };
 struct GatedKind {
   int act;
   float limit, beta, linear_beta, inv_beta, inv_linear_beta;
-  float t_beta, t_linear, scale;   // 2 log2(e) / beta, the same of linear_beta, and the product of both (of beta alone without a bend)
+  float t_beta, t_linear;     // 2 log2(e) / beta, the same of linear_beta
+  float scale;                // 2^-kSituLift beta linear_beta (beta alone without a bend)
 };
+// Powers of two by which SiTU's denominators are taken smaller, so that their product stays in fp32's range.
+constexpr int kSituLift = 60;
+constexpr float kSituLifted = 1.0f / (float)(1ull << kSituLift);
 inline GatedKind gated_kind(int act, float limit, float beta, float linear_beta) {
   constexpr float kTwoLog2e = 2.8853900817779268f;
   const bool bent = linear_beta > 0.0f;
   const float inv = 1.0f / beta, inv_linear = bent ? 1.0f / linear_beta : 0.0f;
-  return {act, limit, beta, linear_beta, inv, inv_linear, kTwoLog2e / beta, bent ? kTwoLog2e / linear_beta : 0.0f, bent ? beta * linear_beta : beta};
+  return {act, limit, beta, linear_beta, inv, inv_linear, kTwoLog2e / beta, bent ? kTwoLog2e / linear_beta : 0.0f, kSituLifted * (bent ? beta * linear_beta : beta)};
 }
 
 // One 16-bit operand of a product: element (i, k) is p[i * ld + k], or p[k * ld + i] if mn_major (the index that is NOT

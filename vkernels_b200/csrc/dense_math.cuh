@@ -107,17 +107,20 @@ __device__ __forceinline__ float dense_tanh_parts(float t, float& e) {
 
 // The gated product of one feature. min.NaN / max.NaN: a NaN stays NaN. SiTU's three quotients - two tanh, one sigmoid - have one
 // reciprocal: three exp2 and it are what the special-function unit does for an element (333 x 2880 -> 2880: a reciprocal and a
-// division for each took 2.5 us longer).
+// division for each took 2.5 us longer). The denominators' product passes fp32's range - 2^29 from up's tanh alone, exp(-g) from
+// the sigmoid - so the sigmoid's is taken 2^-60 times, and k.scale holds the 2^-60 that takes it back: the quotient becomes 0 only
+// where exp(-g) times up's denominator passes 2^186, from g = -109 on for the largest up, where the sigmoid is 5e-48.
 __device__ __forceinline__ float dense_gated(int act, float g, float u, const GatedKind& k) {
   if (act == 1) {
-    float e1, e2, e3 = 0.0f, low, r;
+    float e1, e2, e3 = 0.0f, r, n3 = k.scale, last = u;
     const float n1 = dense_tanh_parts(g * k.t_beta, e1);
-    // exp(-g), finite: what is lost beyond exp(87) is below every 16-bit type's smallest value
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(low) : "f"(g * -1.4426950408889634f), "f"(125.5f));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e2) : "f"(low));
-    const float n3 = k.linear_beta > 0.0f ? dense_tanh_parts(u * k.t_linear, e3) : u;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((e1 + 1.0f) * (1.0f + e2) * (e3 + 1.0f)));
-    return k.scale * n1 * r * n3;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e2) : "f"(fmaf(g, -1.4426950408889634f, -(float)kSituLift)));
+    if (k.linear_beta > 0.0f) {
+      n3 = dense_tanh_parts(u * k.t_linear, e3);
+      last = k.scale;
+    }
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((e1 + 1.0f) * (e2 + kSituLifted) * (e3 + 1.0f)));
+    return n1 * r * n3 * last;
   }
   const float limit = k.limit, lo = -limit;
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(g) : "f"(limit));
