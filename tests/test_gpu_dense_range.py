@@ -4,6 +4,8 @@ far tails.
 A pre-activation is put in exactly: x has one value that is not 0, a weight row one that meets it. Bounds count roundings (see
 dense_oracle); an exponential's argument v is itself rounded, by at most 2^-22 |v| for each function here, which moves the value by
 that much of itself."""
+import math
+
 import pytest
 import torch
 
@@ -52,3 +54,32 @@ def test_situ_far_from_zero(T, dtype, beta, linear_beta, impl):
     error = (ref.APPROX + 2.0 ** -22 * g.abs()) * value.abs()
     bound = error + ref.half_step(dt) * (value.abs() + error) + ref.tiny(dt)
     ref.assert_within(got, value.expand(T, N), bound.expand(T, N), "h")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T", [1, 600])
+def test_gelu_tail_is_good_relatively(T, dtype, impl):
+    """Value and slope of gelu (erf) for negative arguments, down to where the value leaves the type's range: within a rounding of
+    their own size, not of z's."""
+    dt = ref.TYPES[dtype]
+    z = -torch.linspace(0.0, 13.0 if dtype == "bf16" else 6.0, 1601, dtype=torch.float64, device=DEV).to(dt).unique()
+    N = z.numel()
+    w = torch.zeros(N, 8, dtype=dt, device=DEV)
+    w[:, 0] = z
+    x = torch.zeros(T, 8, dtype=dt, device=DEV)
+    x[:, 0] = 1.0
+    y, preact = ops.fused_linear(x, w, activation="gelu", return_preact=True)
+    z = z.double()
+    assert torch.equal(preact, z.float().expand(T, N))
+    cdf, density = 0.5 * torch.special.erfc(-z / math.sqrt(2)), torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    h, rel = ref.half_step(dt), ref.APPROX + 2.0 ** -22 * z * z
+    value = z * cdf
+    error = rel * value.abs()
+    bound = error + h * (value.abs() + error) + ref.tiny(dt)
+    ref.assert_within(y, value.expand(T, N), bound.expand(T, N), "y")
+    # the gradient of the bias of one token is the slope itself, rounded once
+    _, _, db = ops.fused_linear_backward(torch.ones(1, N, dtype=dt, device=DEV), x[:1], w, preact[:1], activation="gelu", bias_grad=True,
+                                         x_grad=False, w_grad=False)
+    slope = cdf + z * density
+    error = rel * (cdf + z.abs() * density)
+    ref.assert_within(db, slope, error + h * (slope.abs() + error) + ref.tiny(dt), "slope")
