@@ -34,3 +34,23 @@ def test_feed_forward_places_must_not_overlap_what_is_read_later():
     for r, kw in ((res, dict(product=t(4, ispp))), (wide[:, :H], dict(product=wide[:, H:])), (res, dict(out=res)), (res, dict(out=x)), (None, dict(out=x))):
         with pytest.raises(ops.OpNotEligible, match="CUDA"):      # not in the way of one another: on to the operators
             ffn(x, r, **kw)
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation is not offered; what carries a tangent is refused by name, under no_grad too."""
+    import torch.autograd.forward_ad as fwd
+
+    x, w, b, res, dy, preact = t(2, 8), t(16, 8), t(16), t(2, 16), t(2, 16), t(2, 16, dtype=torch.float32)
+    with fwd.dual_level():
+        dual = lambda v: fwd.make_dual(v, torch.ones_like(v))  # noqa: E731
+        for call in (lambda: ops.gated_linear(dual(x), w), lambda: ops.gated_linear(x, w, dual(b)), lambda: ops.gated_linear(x, w, out=dual(t(2, 8))),
+                     lambda: ops.fused_linear(x, dual(w)), lambda: ops.fused_linear(x, w, residual=dual(res)),
+                     lambda: ops.fused_linear_backward(dual(dy), x, w), lambda: ops.gated_linear_backward(t(2, 8), x, w, dual(preact))):
+            with pytest.raises(ops.OpNotEligible, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(ops.OpNotEligible, match="forward-mode"):
+                call()
+        with pytest.raises(ops.OpNotEligible, match="CUDA"):      # a level alone changes nothing
+            ops.fused_linear(x, w, b)
+    with pytest.raises(ops.OpNotEligible, match="CUDA"):
+        ops.fused_linear(x, w, b)

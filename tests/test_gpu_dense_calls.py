@@ -51,3 +51,29 @@ def test_layer_result_where_its_activations_lie(T):
     assert same(layer(first), want, T)
     torch.cuda.synchronize()
     ops.kernel_status()
+
+
+def test_dual_tensors_are_refused():
+    """Forward-mode differentiation is not offered: a tangent is refused, not dropped, on the direct path and behind it."""
+    import torch.autograd.forward_ad as fwd
+
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    r = lambda *s: torch.randn(s, generator=g, device=DEV).to(torch.bfloat16)  # noqa: E731
+    x, w, b, res, dy = r(8, 64), r(32, 64), r(32), r(8, 32), r(8, 32)
+    _, preact = ops.fused_linear(x, w, b, activation="silu", return_preact=True)
+    plain = ops.fused_linear(x, w, b, residual=res)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: ops.gated_linear(dual(x), w), lambda: ops.gated_linear(x, dual(w), b), lambda: ops.gated_linear(x, w, dual(b)),
+                     lambda: ops.fused_linear(dual(x), w), lambda: ops.fused_linear(x, dual(w)), lambda: ops.fused_linear(x, w, dual(b)),
+                     lambda: ops.fused_linear(x, w, residual=dual(res)), lambda: ops.fused_linear(x.view(2, 4, 64), dual(w)),
+                     lambda: ops.fused_linear(x, w, residual=res, out=dual(res)),
+                     lambda: ops.fused_linear_backward(dual(dy), x, w, preact, activation="silu"),
+                     lambda: ops.fused_linear_backward(dy, x, w, dual(preact), activation="silu"),
+                     lambda: ops.gated_linear_backward(dual(dy)[:, :16], x, w, preact)):
+            with pytest.raises(ops.OpNotEligible, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(ops.OpNotEligible, match="forward-mode"):
+                call()
+        assert torch.equal(ops.fused_linear(x, w, b, residual=res), plain)      # a level alone changes nothing

@@ -11,11 +11,12 @@ on the current stream, allocate through torch only, and may be captured.
 
 Called with gradients enabled and an input that requires one, the two operators record themselves for ``backward()``; that
 form cannot be captured into a CUDA graph (capture the forward call with ``return_preact=True`` and ``*_backward`` instead, which
-record nothing).
+record nothing). Forward-mode differentiation is not offered: a tensor with a tangent is refused.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -177,6 +178,14 @@ def _wants_grad(*tensors):
     return False
 
 
+def _no_tangent(*tensors):
+    """Refuses a tensor that carries a tangent of forward-mode differentiation (there is none outside a dual level)."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:      # (asking a tensor costs 3 us)
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise OpNotEligible("forward-mode differentiation is not offered: a tensor of the call carries a tangent")
+
+
 def _no_capture():
     if torch.cuda.is_current_stream_capturing():
         raise OpNotEligible("recording for backward() cannot be captured into a CUDA graph: capture the forward call with "
@@ -250,6 +259,7 @@ def gated_linear(x: torch.Tensor, w13: torch.Tensor, b13: torch.Tensor | None = 
 
     ``return_preact``: also return what ``gated_linear_backward`` needs, the pre-activations in fp32, ``[T, 2 * ispp]`` (T: all
     leading dimensions of x together)."""
+    _no_tangent(x, w13, b13, out)
     if out is None and type(x) is torch.Tensor and isinstance(w13, torch.Tensor):
         # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
         shape, index, dtype, wshape = x.shape, x.get_device(), x.dtype, w13.shape
@@ -321,6 +331,7 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     ``return_preact``: also return what ``fused_linear_backward`` needs: the pre-activations in fp32, ``[T, n_out]``, or None
     where there is no activation."""
     act = _linear_kind(activation)
+    _no_tangent(x, w, bias, residual, out)
     if out is None and type(x) is torch.Tensor and isinstance(w, torch.Tensor):
         # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
         shape, index, dtype, wshape = x.shape, x.get_device(), x.dtype, w.shape
@@ -383,6 +394,7 @@ def fused_linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pr
 
 
 def _backward(entry, dy, x, w, preact, gated, bias_grad, x_grad, w_grad, kind):
+    _no_tangent(dy, x, w, preact)
     ordinary, ldp = False, 0
     if type(x) is torch.Tensor and isinstance(w, torch.Tensor) and isinstance(dy, torch.Tensor):
         # the ordinary call, checked at once: what it does not cover is looked at below piece by piece
