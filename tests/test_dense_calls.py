@@ -54,3 +54,23 @@ def test_tangents_are_refused():
             ops.fused_linear(x, w, b)
     with pytest.raises(ops.OpNotEligible, match="CUDA"):
         ops.fused_linear(x, w, b)
+
+
+def test_layer_that_cannot_record_refuses_before_it_starts():
+    """A layer whose always-on expert holds parameters: refused before any of its buffers is touched, unless gradients are off."""
+    from vkernels_b200.experts import FusedMoEMxfp4
+    from vkernels_b200.feedforward import DenseFeedForward
+
+    for which in range(4):
+        parts = [t(32, 8), t(8, 16), t(32), t(8)]
+        parts[which].requires_grad_()
+        layer = FusedMoEMxfp4.__new__(FusedMoEMxfp4)
+        layer.shared_ffn = DenseFeedForward(parts[0], parts[1], b13=parts[2], b2=parts[3])
+        layer.hidden = 8
+        layer._buffers = lambda T: {}
+        with pytest.raises(ops.OpNotEligible, match="records no gradient"):
+            layer.forward(t(4, 8))
+        with torch.no_grad():
+            assert not layer.shared_ffn.records(t(4, 8))
+    ffn = DenseFeedForward(t(32, 8), t(8, 16))
+    assert not ffn.records(t(4, 8), None) and ffn.records(t(4, 8).requires_grad_())

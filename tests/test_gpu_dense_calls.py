@@ -77,3 +77,25 @@ def test_dual_tensors_are_refused():
             with torch.no_grad(), pytest.raises(ops.OpNotEligible, match="forward-mode"):
                 call()
         assert torch.equal(ops.fused_linear(x, w, b, residual=res), plain)      # a level alone changes nothing
+
+
+def test_layer_records_nothing_and_says_so_before_any_work():
+    """The routed experts record no gradient: with a feed-forward of parameters, or activations, that require one the layer is called
+    under no_grad; elsewhere it refuses before it writes anything."""
+    routed, layer, ffn, A = layers(40, grad=True)
+    with torch.no_grad():
+        want = ffn(A, routed(A)).clone()
+        assert torch.equal(layer(A), want)
+        graph, y = layer.capture(A)
+        graph.replay()
+        assert torch.equal(y, want)
+    out = torch.full_like(A, 7.0)
+    with pytest.raises(ops.OpNotEligible, match="records no gradient"):
+        layer(A, out_bf16=out)
+    frozen_routed, frozen, _, A = layers(40)
+    with pytest.raises(ops.OpNotEligible, match="records no gradient"):
+        frozen(A.clone().requires_grad_(), out_bf16=out)
+    torch.cuda.synchronize()
+    assert bool((out == 7).all())
+    with torch.inference_mode():
+        assert torch.equal(layer(A), want)

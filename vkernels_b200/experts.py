@@ -88,7 +88,8 @@ class FusedMoEMxfp4:
                  beta: float = 4.0, linear_beta: float = 25.0, b13=None, b2=None,
                  max_tokens: int = DEFAULT_TOKEN_BUDGET, block_size: int = 16, prepack: bool = False, shared_ffn=None):
         """``shared_ffn`` (``feedforward.DenseFeedForward``): an always-on expert in bf16, for checkpoints that do not hold it
-        among the MXFP4 experts (those take ``n_shared``); ``forward`` adds its result to the routed experts'.
+        among the MXFP4 experts (those take ``n_shared``); ``forward`` adds its result to the routed experts'. The layer records
+        no gradient: where the feed-forward's weights (or x) require one, call it under ``torch.no_grad()``; elsewhere it refuses.
 
         ``prepack``: also keep the weights in the prepacked form (``ops.prepack_weights``; about as
         large as the checkpoint form again) and run decode-size batches from it - their kernels
@@ -282,6 +283,8 @@ class FusedMoEMxfp4:
         """The always-on expert's gated projection, made before the routed experts write their result: that may lie where x does."""
         if self.shared_ffn is None:
             return None
+        ops.require(not self.shared_ffn.records(x), "the layer records no gradient, and its shared_ffn's weights or x require one: "
+                                                    "call it under torch.no_grad()")
         T = x.shape[0]
         with _region("moe:apply.shared"):
             return self.shared_ffn.product(x, out=self.arena.take("shared", T * self.shared_ffn.ispp).view(T, self.shared_ffn.ispp))

@@ -32,6 +32,10 @@ class DenseFeedForward:
         self.hidden, self.ispp = w2.shape
         self.kind = dict(activation=activation, swiglu_limit=swiglu_limit, beta=beta, linear_beta=linear_beta)
 
+    def records(self, *inputs: torch.Tensor | None) -> bool:
+        """Whether a call with these inputs records itself for ``backward()``."""
+        return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*inputs, self.w13, self.w2, self.b13, self.b2))
+
     def product(self, x: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
         """The gated projection alone: ``[..., ispp]`` for x ``[..., hidden]``."""
         return ops.gated_linear(x, self.w13, self.b13, out=out, **self.kind)
