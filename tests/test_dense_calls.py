@@ -74,3 +74,13 @@ def test_layer_that_cannot_record_refuses_before_it_starts():
             assert not layer.shared_ffn.records(t(4, 8))
     ffn = DenseFeedForward(t(32, 8), t(8, 16))
     assert not ffn.records(t(4, 8), None) and ffn.records(t(4, 8).requires_grad_())
+
+
+def test_a_place_that_is_no_tensor_is_refused_beside_a_residual():
+    for out in ([0.0], 1.0, "y"):
+        with pytest.raises(ops.OpNotEligible, match="out must be a tensor"):
+            ops.fused_linear(t(2, 8), t(16, 8), residual=t(2, 16), out=out)
+        with pytest.raises(ops.OpNotEligible, match="out must be a tensor"):
+            ops.fused_linear(t(2, 8), t(16, 8), out=out)
+        with pytest.raises(ops.OpNotEligible, match="out must be a tensor"):
+            ops.gated_linear(t(2, 8), t(16, 8), out=out)

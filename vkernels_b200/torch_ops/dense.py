@@ -365,6 +365,7 @@ def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
         ldr = _pitch("the residual", r2)
     out2 = None
     if out is not None:
+        _check_tensor("out", out)
         in_place = residual is not None and out.data_ptr() == residual.data_ptr() and out.stride() == residual.stride()
         out2 = _given_out(out, shape, x, (("x", x), ("w", w), ("the bias", bias), ("the residual", None if in_place else residual)))
     _resident(x)
