@@ -27,7 +27,7 @@ inline GatedKind gated_kind(int act, float limit, float beta, float linear_beta)
   constexpr float kTwoLog2e = 2.8853900817779268f;
   const bool bent = linear_beta > 0.0f;
   const float inv = 1.0f / beta, inv_linear = bent ? 1.0f / linear_beta : 0.0f;
-  return {act, limit, beta, linear_beta, inv, inv_linear, kTwoLog2e / beta, bent ? kTwoLog2e / linear_beta : 0.0f, kSituLifted * (bent ? beta * linear_beta : beta)};
+  return {act, limit, beta, linear_beta, inv, inv_linear, kTwoLog2e / beta, bent ? kTwoLog2e / linear_beta : 0.0f, kSituLifted * beta * (bent ? linear_beta : 1.0f)};
 }
 
 // One 16-bit operand of a product: element (i, k) is p[i * ld + k], or p[k * ld + i] if mn_major (the index that is NOT
