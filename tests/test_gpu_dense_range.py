@@ -1,5 +1,5 @@
 """-m gpu: the dense feed-forward's activations over the range of their arguments, value by value against the definition in 64 bits:
-far tails.
+far tails, every constant of SiTU; offsets beyond 32 bits in every operand, and a dense layer's features.
 
 A pre-activation is put in exactly: x has one value that is not 0, a weight row one that meets it. Bounds count roundings (see
 dense_oracle); an exponential's argument v is itself rounded, by at most 2^-22 |v| for each function here, which moves the value by
@@ -83,3 +83,127 @@ def test_gelu_tail_is_good_relatively(T, dtype, impl):
     slope = cdf + z * density
     error = rel * (cdf + z.abs() * density)
     ref.assert_within(db, slope, error + h * (slope.abs() + error) + ref.tiny(dt), "slope")
+
+
+@pytest.mark.parametrize("beta,linear_beta", [(1.5, 6.0), (4.0, 0.0), (0.5, -1.0), (30.0, 100.0)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,K,N", [(1, 256, 72), (17, 640, 130), (129, 192, 64), (300, 320, 257), (600, 136, 96)])
+def test_situ_with_other_constants(T, K, N, dtype, beta, linear_beta, impl):
+    """Forward and backward of SiTU with constants that are not the defaults, up left unbent among them."""
+    dt = ref.TYPES[dtype]
+    g = torch.Generator(device=DEV)
+    g.manual_seed(T + 7 * K + 13 * N)
+    r = lambda *s: torch.randn(s, generator=g, device=DEV)  # noqa: E731
+    x, w, b, dh = r(T, K).to(dt), (r(2 * N, K) * (1.5 / K ** 0.5)).to(dt), (0.3 * r(2 * N)).to(dt), r(T, N).to(dt)
+    kw = dict(activation=ops.SITU, beta=beta, linear_beta=linear_beta)
+    h, preact = ops.gated_linear(x, w, b, return_preact=True, **kw)
+    assert torch.equal(h, ops.gated_linear(x, w, b, **kw))
+    z, mags = ref.project(x, w, b)
+    value, _, _, made_of, _, _ = ref.gated(z, "situ", 0.0, beta, linear_beta)
+    # |dh/dg| <= |up| (1.2 + beta / 4): (1 - a^2) p <= 1, |a| p (1 - p) <= 1 / 4; |dh/du| <= |gate| <= min(|g|, beta)
+    zb = z.abs() + ref.sum_error(K, impl) * mags
+    up = zb[:, N:].clamp(max=linear_beta) if linear_beta > 0 else zb[:, N:]
+    dz = ref.sum_error(K, impl) * mags
+    error = up * (1.2 + beta / 4) * dz[:, :N] + zb[:, :N].clamp(max=beta) * dz[:, N:] + ref.APPROX * made_of
+    ref.assert_within(h, value, error + ref.half_step(dt) * (value.abs() + error) + ref.tiny(dt), "h")
+    got = ops.gated_linear_backward(dh, x, w, preact, bias_grad=True, **kw)
+    _, dg, du, _, mg, mu = ref.gated(preact.double(), "situ", 0.0, beta, linear_beta)
+    d = dh.double()
+    dz = torch.cat([d * dg, d * du], 1)
+    error = ref.APPROX * torch.cat([d.abs() * mg, d.abs() * mu], 1)
+    for name, t, (v, bound) in zip(("dx", "dw13", "db13"), got, ref.gradients(dz, error, x, w, dt, impl)):
+        ref.assert_within(t, v, bound, name)
+
+
+def test_offsets_beyond_32_bits_in_the_backward_pass():
+    """More than 2^31 pre-activations: kept by the forward call, read by the gradient's kernel, whose result and both products then
+    pass 2^31 elements too. Rows and columns at the ends and in the middle against the definition."""
+    T, K, N, act = 266000, 64, 8256, "silu"
+    g = torch.Generator(device=DEV)
+    g.manual_seed(7)
+    r = lambda *s: torch.randn(s, generator=g, device=DEV)  # noqa: E731
+    dt = torch.bfloat16
+    x, w, b = r(T, K).to(dt), (r(N, K) * (1.5 / K ** 0.5)).to(dt), (0.3 * r(N)).to(dt)
+    y, preact = ops.fused_linear(x, w, b, activation=act, return_preact=True)
+    assert preact.numel() > 2 ** 31
+    rows = torch.tensor([0, 1, T // 2 + 5, 260111, 260112, T - 3, T - 1], device=DEV)   # 260112 * 8256 is just above 2^31
+    z, mags = ref.project(x[rows], w, b)
+    dz = ref.sum_error(K) * mags
+    ref.assert_within(preact[rows], z, dz + 2.0 ** -23 * z.abs() + 1e-37, "preact")
+    value, _ = ref.linear_act(z, act)
+    error = 1.2 * dz + ref.APPROX * z.abs()
+    ref.assert_within(y[rows], value, error + ref.half_step(dt) * (value.abs() + error) + ref.tiny(dt), "y")
+    dy = y                                        # any values do as the result's gradient: its own memory is the forward call's
+    dx, dw, db = ops.fused_linear_backward(dy, x, w, preact, activation=act, bias_grad=True)
+    cols = torch.tensor([0, 1, N // 2 + 1, N - 8, N - 1], device=DEV)
+
+    def operand(of_dy, of_z):
+        d, zz = of_dy.double(), of_z.double()
+        return d * ref.linear_act(zz, act)[1], ref.APPROX * d.abs() * (1 + zz.abs())
+    grad, error = operand(dy[rows], preact[rows])
+    ref.assert_within(dx[rows], *ref.gradients(grad, error, x[rows], w, dt)[0], "dx")
+    grad, error = operand(dy[:, cols], preact[:, cols])
+    _, (dw64, dw_bound), (db64, db_bound) = ref.gradients(grad, error, x, w[cols], dt)
+    ref.assert_within(dw[cols], dw64, dw_bound, "dw")
+    ref.assert_within(db[cols], db64, db_bound, "db")
+    torch.cuda.synchronize()
+    ops.kernel_status()
+
+
+def test_strided_operand_beyond_32_bits_in_the_backward_pass():
+    """x as the last columns of a matrix of more than 2^31 elements: both gradients are those of a copy of it."""
+    T, K, N = 266000, 64, 32
+    g = torch.Generator(device=DEV)
+    g.manual_seed(8)
+    dt = torch.bfloat16
+    wide = torch.zeros(T, 8256, dtype=dt, device=DEV)
+    wide[:, -K:] = torch.randn(T, K, generator=g, device=DEV)
+    x = wide[:, -K:]
+    w13 = (torch.randn(2 * N, K, generator=g, device=DEV) * (1.5 / K ** 0.5)).to(dt)
+    dh = torch.randn(T, N, generator=g, device=DEV).to(dt)
+    h, preact = ops.gated_linear(x, w13, return_preact=True)
+    dx, dw, db = ops.gated_linear_backward(dh, x, w13, preact, bias_grad=True)
+    near = x.contiguous()
+    h2, preact2 = ops.gated_linear(near, w13, return_preact=True)
+    assert torch.equal(h, h2) and torch.equal(preact, preact2)
+    _, dg, du, _, mg, mu = ref.gated(preact.double(), "swiglu", 0.0)
+    d = dh.double()
+    grad, error = torch.cat([d * dg, d * du], 1), ref.APPROX * torch.cat([d.abs() * mg, d.abs() * mu], 1)
+    for name, t, (v, bound) in zip(("dx", "dw13", "db13"), (dx, dw, db), ref.gradients(grad, error, near, w13, dt)):
+        ref.assert_within(t, v, bound, name)
+    torch.cuda.synchronize()
+    ops.kernel_status()
+
+
+@pytest.mark.parametrize("T", [1, 70, 300])
+def test_features_of_a_wide_dense_layer(T):
+    """7168 -> 2 x 18432 gated and 18432 -> 7168, forward and backward."""
+    H, ispp, dt = 7168, 18432, torch.bfloat16
+    g = torch.Generator(device=DEV)
+    g.manual_seed(T)
+    r = lambda *s: torch.randn(s, generator=g, device=DEV)  # noqa: E731
+    x, w13, w2, dh, dy = r(T, H).to(dt), (r(2 * ispp, H) * (1.5 / H ** 0.5)).to(dt), (r(H, ispp) / ispp ** 0.5).to(dt), r(T, ispp).to(dt), r(T, H).to(dt)
+    h, preact = ops.gated_linear(x, w13, swiglu_limit=7.0, return_preact=True)
+    half = ref.half_step(dt)
+    z, mags = ref.project(x, w13)
+    dz = ref.sum_error(H) * mags
+    ref.assert_within(preact, z, dz + 2.0 ** -23 * z.abs() + 1e-37, "preact")
+    value, _, _, made_of, _, _ = ref.gated(z, "swiglu", 7.0)
+    sg, su = ref.gated_slopes_bound(z, "swiglu", 7.0)
+    error = sg * dz[:, :ispp] + su * dz[:, ispp:] + ref.APPROX * made_of
+    ref.assert_within(h, value, error + half * (value.abs() + error) + ref.tiny(dt), "h")
+    y, (z2, mags2) = ops.fused_linear(h, w2, residual=x), ref.project(h, w2)
+    value = z2 + x.double()
+    error = ref.sum_error(ispp) * mags2 + 2.0 ** -23 * value.abs()
+    ref.assert_within(y, value, error + half * (value.abs() + error) + ref.tiny(dt), "y")
+    _, dg, du, _, mg, mu = ref.gated(preact.double(), "swiglu", 7.0)
+    d = dh.double()
+    grad, error = torch.cat([d * dg, d * du], 1), ref.APPROX * torch.cat([d.abs() * mg, d.abs() * mu], 1)
+    got = ops.gated_linear_backward(dh, x, w13, preact, swiglu_limit=7.0, bias_grad=True)
+    for name, t, (v, bound) in zip(("dx", "dw13", "db13"), got, ref.gradients(grad, error, x, w13, dt)):
+        ref.assert_within(t, v, bound, name)
+    got = ops.fused_linear_backward(dy, h, w2, bias_grad=True)
+    for name, t, (v, bound) in zip(("dh", "dw2", "db2"), got, ref.gradients(dy.double(), torch.zeros_like(z2), h, w2, dt)):
+        ref.assert_within(t, v, bound, name)
+    torch.cuda.synchronize()
+    ops.kernel_status()
