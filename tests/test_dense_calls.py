@@ -84,3 +84,11 @@ def test_a_place_that_is_no_tensor_is_refused_beside_a_residual():
             ops.fused_linear(t(2, 8), t(16, 8), out=out)
         with pytest.raises(ops.OpNotEligible, match="out must be a tensor"):
             ops.gated_linear(t(2, 8), t(16, 8), out=out)
+
+
+def test_no_rows_have_any_stride():
+    """Of a batch of no tokens an expanded gradient is one number's strides: there is nothing to refuse in it."""
+    none = torch.ones((), dtype=BF).expand(0, 16)
+    for call in (lambda: ops.fused_linear_backward(none, t(0, 8), t(16, 8)), lambda: ops.fused_linear(t(8, 0).T, t(16, 8), residual=none)):
+        with pytest.raises(ops.OpNotEligible, match="CUDA"):
+            call()

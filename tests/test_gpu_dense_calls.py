@@ -99,3 +99,13 @@ def test_layer_records_nothing_and_says_so_before_any_work():
     assert bool((out == 7).all())
     with torch.inference_mode():
         assert torch.equal(layer(A), want)
+
+
+def test_recorded_gradients_of_no_tokens():
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    w13, w, b = (torch.randn(s, generator=g, device=DEV).to(torch.bfloat16).requires_grad_() for s in ((32, 64), (64, 16), (64,)))
+    x = torch.empty(0, 64, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    y = ops.fused_linear(ops.gated_linear(x, w13), w, b, activation="gelu", residual=x)
+    grads = torch.autograd.grad(y.sum(), [x, w13, w, b])
+    assert [tuple(t.shape) for t in grads] == [(0, 64), (32, 64), (64, 16), (64,)] and not any(bool(t.any()) for t in grads)

@@ -87,7 +87,7 @@ def _pitch(name, t):
     """Elements from one row of a 2-D tensor to the next."""
     T, n = t.shape
     row, step = t.stride()
-    if n > 1 and step != 1:
+    if T > 0 and n > 1 and step != 1:      # (of no rows, an expanded gradient has any)
         raise OpNotEligible(f"the values of a row of {name} must be neighbours in memory")
     if T <= 1:
         return (n + 7) // 8 * 8
