@@ -101,6 +101,95 @@ def test_layer_records_nothing_and_says_so_before_any_work():
         assert torch.equal(layer(A), want)
 
 
+def test_forked_capture():
+    """Calls on two streams of one capture, forked and joined: each result is that of its own inputs on every replay."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(2)
+    r = lambda *s: torch.randn(s, generator=g, device=DEV)  # noqa: E731
+    for T in (3, 300):
+        x = r(T, 256).to(torch.bfloat16)
+        w13, wa, wb, wc = ((r(n, k) / k ** 0.5).to(torch.bfloat16) for n, k in ((512, 256), (256, 256), (256, 256), (256, 256)))
+
+        def step(side=None):
+            h, preact = ops.gated_linear(x, w13, return_preact=True)
+            main = torch.cuda.current_stream()
+            if side is not None:
+                side.wait_stream(main)
+            with torch.cuda.stream(side or main):
+                a = ops.fused_linear(h, wa, activation="silu")
+                da, dwa, _ = ops.fused_linear_backward(a, h, wa)
+            b = ops.fused_linear(h, wb, activation="gelu")
+            dx, dw13, db = ops.gated_linear_backward(h, x, w13, preact, bias_grad=True)
+            if side is not None:
+                main.wait_stream(side)
+            return [a, b, da, dwa, dx, dw13, db, ops.fused_linear(a, wc, residual=b), ops.fused_linear(da, wc, residual=dx)]
+        step()
+        torch.cuda.synchronize()
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph):
+            got = step(side)
+        for _ in range(5):
+            x.mul_(-0.75)
+            graph.replay()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(got, step()))
+    ops.kernel_status()
+
+
+def test_calls_from_two_threads():
+    """Two threads, a stream each, call at once: every result has its own inputs' bits."""
+    import threading
+
+    g = torch.Generator(device=DEV)
+    g.manual_seed(4)
+    r = lambda *s: torch.randn(s, generator=g, device=DEV).to(torch.bfloat16)  # noqa: E731
+    jobs = [(r(T, 264), r(2 * 72, 264), r(T, 72)) for T in (5, 90, 700)]
+
+    def step(x, w13, dh):
+        h, preact = ops.gated_linear(x, w13, return_preact=True)
+        return (h, *ops.gated_linear_backward(dh, x, w13, preact, bias_grad=True))
+    want = [step(*j) for j in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(first):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(60):
+                    k = (first + i) % len(jobs)
+                    got = step(*jobs[k])
+                    if not all(torch.equal(p, q) for p, q in zip(got, want[k])):
+                        wrong.append(k)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    ops.kernel_status()
+
+
+@pytest.mark.parametrize("T", [1, 20, 600])
+def test_feed_forward_in_place_of_its_input(T):
+    """x as the residual and as the place for the result, and the product beside it in one buffer."""
+    from vkernels_b200.feedforward import DenseFeedForward
+
+    g = torch.Generator(device=DEV)
+    g.manual_seed(T)
+    r = lambda *s: torch.randn(s, generator=g, device=DEV).to(torch.bfloat16)  # noqa: E731
+    x, w13, w2 = r(T, 128), r(2 * 96, 128) * 0.1, r(128, 96) * 0.1
+    ffn = DenseFeedForward(w13, w2, swiglu_limit=5.0)
+    want = ffn(x, x)
+    wide = r(T, 128 + 96)
+    wide[:, :128] = x
+    assert torch.equal(ffn(wide[:, :128], wide[:, :128], out=wide[:, :128], product=wide[:, 128:]), want)
+    assert torch.equal(wide[:, :128], want) and torch.equal(wide[:, 128:], ffn.product(x))
+    assert ffn(x, x, out=x) is x and torch.equal(x, want)
+
+
 def test_recorded_gradients_of_no_tokens():
     g = torch.Generator(device=DEV)
     g.manual_seed(1)
