@@ -405,7 +405,8 @@ int vk_cuda_fused_moe_mxfp4_rows(const uint64_t* a_rows, const uint8_t* w13, con
  *   first, into a workspace of vk_cuda_dense_forward_workspace_bytes bytes (0: none needed, NULL will do).
  * *_backward: gradients for the gradient of the result (dh / dy); each of dx, dw (dw13), db (db13) may be NULL. The activation
  *   arguments and preact are those of the forward call (preact unused for activation 0 of the linear form); the residual's
- *   gradient is dy. The gradient of z is rounded to the type once, as the products' operand, in the workspace
+ *   gradient is dy. The gradient of z is rounded to the type once, as the products' operand (fp16: 0 below 3e-8, infinite beyond
+ *   65504), in the workspace
  *   (vk_cuda_dense_backward_workspace_bytes bytes, which also hold fp32 parts of gradients that are long sums of few values); db sums
  *   it unrounded. */
 int vk_cuda_gated_linear(const void* x, int64_t ldx, const void* w13, int64_t ldw, const void* b13, void* h, int64_t ldh,

@@ -352,8 +352,8 @@ dense_wide_kernel(const __grid_constant__ WideLaunch<COUNT> work) {
   wait_for_earlier_kernels();
   const int unit = blockIdx.x >> 1, n_units = gridDim.x >> 1;
   // A pair's tile in round `it`. Of two products the rounds behind the one in which the second begins are dealt out from the other
-  // end: what is left for the last goes first to pairs that had no long tile in that one (1001 tokens, 1504 -> 2 x 1027: 24.2 us
-  // for the backward pass with all rounds in one order, 21.0 so; 4096 tokens, 1024 -> 1024 20.5 and 17.0).
+  // end: what is left for the last goes first to pairs that had no long tile in that one (1001 tokens, 1504 -> 2 x 1027: 23.9 us
+  // for the backward pass with all rounds in one order, 19.8 so; 4096 tokens, 1024 -> 1024 20.1 and 16.2).
   const int turn = COUNT > 1 ? work.p[0].n_tiles / n_units : 0;
   const auto tile_of = [&](int it) { return it * n_units + (COUNT > 1 && it > turn ? n_units - 1 - unit : unit); };
   // which product tile t belongs to, and where and of which part of k it lies there
@@ -708,7 +708,8 @@ void launch_dense_wide(const DenseGemm& g, cudaStream_t stream) {
 }
 
 // As many parts as there are pairs for, of at least eight blocks of k each, where that saves a tile 32 blocks or more (9 us, of which
-// the join takes back 3 to 6).
+// the join takes back 3 to 6). The pairs are those of a B200's 148 SMs, written down because the workspace's size is asked for without a
+// device; where a device has fewer, the parts are the same and take more rounds.
 int dense_split(int M, int N, int K) {
   constexpr int kPairs = 74;
   const int bn = split_width(N), blocks = (K + 63) / 64;

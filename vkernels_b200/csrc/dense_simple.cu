@@ -291,7 +291,7 @@ void launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, cudaStream_
   VK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
-// CTAs for copies: two units of eight values a thread, eight CTAs an SM at most.
+// CTAs for copies: two units of eight values a thread, eight CTAs an SM (of a B200's 148) at most.
 int copy_ctas(const RowCopies& c) {
   int64_t units = 0;
   for (int i = 0; i < 2; ++i)
@@ -324,7 +324,7 @@ void grad_of_type(const DenseGrad& g, int chunks, cudaStream_t stream) {
 }  // namespace
 
 // Chunks of rows: as many as make the launch three CTAs an SM over 256 columns each, of at least 16 rows; one, whose sums need no
-// further kernel, up to 64 rows.
+// further kernel, up to 64 rows. The workspace's size follows from it and is asked for without a device: 148 SMs, a B200's.
 int dense_sum_chunks(int T, int n_out) {
   if (T <= 64) return 1;
   const int across = (n_out + kGradCols - 1) / kGradCols;

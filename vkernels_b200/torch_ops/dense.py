@@ -11,7 +11,8 @@ on the current stream, allocate through torch only, and may be captured.
 
 Called with gradients enabled and an input that requires one, the two operators record themselves for ``backward()``; that
 form cannot be captured into a CUDA graph (capture the forward call with ``return_preact=True`` and ``*_backward`` instead, which
-record nothing). Forward-mode differentiation is not offered: a tensor with a tangent is refused.
+record nothing). The backward pass rounds the gradient of the pre-activations to the type once, as its products' operand: in
+fp16 that is 0 below 3e-8 and infinite beyond 65504, so losses are scaled as for any fp16 training. Forward-mode differentiation is not offered: a tensor with a tangent is refused.
 """
 from __future__ import annotations
 
