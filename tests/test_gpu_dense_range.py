@@ -207,3 +207,34 @@ def test_features_of_a_wide_dense_layer(T):
         ref.assert_within(t, v, bound, name)
     torch.cuda.synchronize()
     ops.kernel_status()
+
+
+@pytest.mark.parametrize("T,K,N", [(2 ** 27, 8, 8), (2, 2 ** 27, 8), (2, 8, 2 ** 27)])
+def test_largest_sizes(T, K, N):
+    """The documented limits, 2^27 tokens, inputs or weight rows. Operands of -1 and 1: every sum is a whole number that fp32 holds in
+    any order (below 2^24; these are random walks of at most 2^27 steps, 12000 wide), so results are those numbers, rounded once."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+    sign = lambda *s: torch.randint(0, 2, s, generator=g, device=DEV, dtype=torch.int8).mul_(2).sub_(1).to(torch.bfloat16)  # noqa: E731
+    x, w, dy = sign(T, K), sign(N, K), sign(T, N)
+
+    def product(a, b):
+        """a b^T, exactly, a long sum in pieces"""
+        total = torch.zeros(a.shape[0], b.shape[0], dtype=torch.float64, device=DEV)
+        for i in range(0, a.shape[1], 2 ** 24):
+            total += a[:, i:i + 2 ** 24].double() @ b[:, i:i + 2 ** 24].double().T
+        return total
+
+    def check(got, a, b, what):
+        """Rows and columns at both ends where a or b is long, all of them where both are short."""
+        rows, cols = (torch.arange(n, device=DEV) if n <= 64 else torch.tensor([0, 1, 2, n // 2 + 3, n - 2, n - 1], device=DEV) for n in got.shape)
+        want = product(a[rows], b[cols])
+        assert torch.equal(got[rows][:, cols], want.to(got.dtype)), what
+        assert bool(got.isfinite().all()), what
+    check(ops.fused_linear(x, w), x, w, "y")
+    dx, dw, db = ops.fused_linear_backward(dy, x, w, bias_grad=True)
+    check(dx, dy, w.T, "dx")
+    check(dw, dy.T, x.T, "dw")
+    check(db[:, None], dy.T, torch.ones(1, T, dtype=dy.dtype, device=DEV), "db")
+    torch.cuda.synchronize()
+    ops.kernel_status()
