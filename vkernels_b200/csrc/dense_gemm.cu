@@ -204,6 +204,13 @@ __device__ __forceinline__ void load_columns(float (&z)[16], uint32_t taddr) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) z[j] = __uint_as_float(v[j]);
 }
+__device__ __forceinline__ void load_columns_two(float (&z)[16], uint32_t taddr, float (&y)[16], uint32_t uaddr) {
+  uint32_t v[16], u[16];
+  tc_ld16_two(taddr, v, uaddr, u);
+  tc_wait_ld();
+#pragma unroll
+  for (int j = 0; j < 16; ++j) z[j] = __uint_as_float(v[j]), y[j] = __uint_as_float(u[j]);
+}
 // Up to 64 pre-activations of this thread's row to rows of memory that start anywhere, 32 at a time through the staging buffer.
 __device__ __forceinline__ void preact_anywhere(uint32_t tz, int width, uint32_t staging, const float (&bias)[2], bool has_bias, float* p,
                                                 int64_t ld, int rows, int cols, int lane) {
@@ -282,8 +289,7 @@ __device__ __forceinline__ void gated_columns(uint32_t tg, uint32_t tu, int widt
   for (int block = 0; block * 16 < width; ++block) {
     const int n = at.cols - block * 16;
     float g[16], u[16];
-    load_columns(g, tg + block * 16);
-    load_columns(u, tu + block * 16);
+    load_columns_two(g, tg + block * 16, u, tu + block * 16);
     if (has_bias) {
       add_bias(g, bias_g, block);
       add_bias(u, bias_u, block);
